@@ -391,8 +391,9 @@ def _sparse(s):
     hkv, page, budget = c["hkv"], c["page"], c["budget"]
     per = table.shape[1]
     pages = (ctx + page - 1) // page
-    # queries in 16 bits, bounds in 8: the products and sums of the score are whole numbers below 2^53
-    sq = (q.abs().amax(-1).double() / 32767).float()
+    # queries in 16 bits (two signed bytes: 127 * 256 at most), bounds in 8: the score's products and sums are whole
+    # numbers below 2^53
+    sq = (q.abs().amax(-1).double() / 32512).float()
     qi = torch.round(q / torch.where(sq > 0, sq, torch.ones_like(sq))[..., None]).double()
     qi = qi.view(batch, hkv, hq // hkv, hd)
     bounds = s["bounds"][table].transpose(1, 2)  # [batch][hkv][pages][2][hd]
@@ -495,7 +496,7 @@ def exact(case, seed):
             for h in range(hkv):
                 heads = slice(h * (hq // hkv), (h + 1) * (hq // hkv))
                 q = s["q"][i, heads]
-                step = (q.abs().max(-1, keepdim=True).values.double() / 32767).float()
+                step = (q.abs().max(-1, keepdim=True).values.double() / 32512).float()
                 qi = (q / step).round().double()
                 b = s["bounds"][at, h].double()
                 dot = torch.maximum(qi[:, None] * b[None, :, 0], qi[:, None] * b[None, :, 1]).sum(-1)
