@@ -344,6 +344,78 @@ ZC_API int32_t zcu_moe_set_router(void* moe, const float* w, size_t bytes);
 ZC_API int32_t zcu_moe_forward(void* moe, const float* xnorm, const float* router_logits, float* residual, int32_t T,
                                int32_t* sel_idx, float* sel_w);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * One step of a mixed serving batch: operators over many requests at once whose state lives on the device.
+ * They enqueue only, own no scratch (calls on different streams and captured graphs share nothing) and depend
+ * on no order of atomics: the same inputs give the same bits.
+ * ------------------------------------------------------------------------------------------------------- */
+
+/* Block tables and slot maps from request lengths: PagedKvCache's bookkeeping (Memory/PagedKvCache.cs:105-271)
+ * on the device.  A pool is page_table [max_rows][max_pages], seq_len [max_rows] (tokens stored per table row),
+ * free_pages [num_pages], whose first *free_count entries are a stack of free page ids.
+ * reserve: request b adds n_new[b] tokens (below 0: none) to table row rows[b] (rows NULL: row b, batch <=
+ * max_rows).  Its tokens are entries [start[b], start[b + 1]) of the step's token arrays, `tokens` long; its pages
+ * come off the top of the stack, in request order.  granted[b] is 0, and nothing of the request changes, when its row
+ * is out of range or named by an earlier request of the call, when it would pass max_pages pages or the end of the
+ * token arrays, or when the stack does not hold its pages and those of the requests before it.  Per token: slots =
+ * page * page_size + slot, positions, token_rows (its table row) and ctx_len = position + 1; tokens of refused
+ * requests and behind the last request get slot -1, position 0, row -1, ctx_len 0.
+ * trim: row rows[b] keeps min(new_len[b], its length) tokens (0 frees the sequence); pages behind them go back to the
+ * stack, the last request's last page first, and their table entries become -1.  A reserve whose lengths are trimmed
+ * back leaves the stack as it was.
+ * -6 when batch and max_rows exceed one CTA's shared memory (20 bytes a request, and 4 a table row with `rows`, over
+ * 220 KB). */
+ZC_API int32_t zcu_pages_reserve(int32_t* page_table, int32_t* seq_len, int32_t* free_pages, int32_t* free_count,
+                                 int32_t max_rows, int32_t max_pages, int32_t num_pages, int32_t page_size,
+                                 const int32_t* rows, const int32_t* n_new, int32_t batch, int32_t tokens,
+                                 int32_t* start, int64_t* slots, int32_t* positions, int32_t* token_rows,
+                                 int32_t* ctx_len, int32_t* granted, void* stream);
+ZC_API int32_t zcu_pages_trim(int32_t* page_table, int32_t* seq_len, int32_t* free_pages, int32_t* free_count,
+                              int32_t max_rows, int32_t max_pages, int32_t num_pages, int32_t page_size,
+                              const int32_t* rows, const int32_t* new_len, int32_t batch, void* stream);
+
+/* K/V rows k, v [tokens][hkv][hd] (in_dtype 0 = fp32, 1 = fp16; k_stride, v_stride elements between tokens) into
+ * paged pools addressed as in zcu_paged_attention (kv_dtype 0 = fp32, 1 = fp16 rounded to nearest), token t at
+ * slots[t] = page * page_size + slot; slots outside [0, num_pages * page_size) are skipped.  hd 32, 64, 128 or 256.
+ * bounds int8 [num_pages][hkv][2][hd] and scales fp32 [num_pages][hkv] (both or neither) receive, for every page
+ * written, 8-bit bounds of its stored keys: scale = max|k| / 127, lo = floor(min k / scale), hi = ceil(max k / scale)
+ * per dimension (0 for a page whose largest key is 0 or not finite).  A page holds its slots up to the last one that
+ * the call writes; the tokens that a call writes to one page stand in consecutive entries and ascending slots.
+ * Pointers and strides in whole 4-element pieces (16 bytes of fp32, 8 of fp16). */
+ZC_API int32_t zcu_append_kv(const void* k, const void* v, int32_t in_dtype, int64_t k_stride, int64_t v_stride,
+                             const int64_t* slots, int32_t tokens, void* k_pool, void* v_pool, int32_t kv_dtype,
+                             int32_t hkv, int32_t hd, int32_t page_size, int32_t num_pages, int64_t page_stride,
+                             int64_t slot_stride, int64_t head_stride, int8_t* bounds, float* scales, void* stream);
+
+/* Per-request rules on logits [rows][vocab] (dtype 0 = fp32, 1 = fp16, 2 = bf16; strides in elements) before zcu_sample,
+ * written as fp32 to out (which may be the logits themselves when these are fp32; no other overlap).  For token t of
+ * row r, with `seen` whether t stands in the row's history and c how often it stands behind the prompt:
+ *   v = logit;  seen: v = v > 0 ? v / repetition : v * repetition;  v -= frequency * c;  c > 0: v -= presence;
+ *   v += the row's biases of t;  mask bit 0: v = -inf.
+ * (LlmSampler's penalty, Sampling/LlmSampler.cs:39-57, divides once per occurrence; this one once per token.)
+ * Every array is device memory and may be NULL (no such rule):
+ *   past [past_count][past_cap], past_len [past_count]: the history, prompt first; prompt_len [past_count] (NULL: 0);
+ *     row r reads row past_rows[r] (NULL: r; outside [0, past_count): no history).  Ids outside [0, vocab) are skipped.
+ *   repetition, frequency, presence [rows] (NULL: 1, 0, 0)
+ *   bias_start [rows + 1]: row r's entries of bias_ids / bias [n_bias]; a token named twice gets both, in list order
+ *   mask [masks][mask_stride] 32-bit words, bit t % 32 of word t / 32 set = allowed; row r reads mask mask_rows[r]
+ *     (NULL: r; outside [0, masks): unmasked)
+ * -6 for a vocab above 409,600. */
+typedef struct {
+  const int32_t *past, *past_len, *prompt_len, *past_rows;
+  int32_t past_cap, past_count;
+  const float *repetition, *frequency, *presence;
+  const int32_t *bias_start, *bias_ids;
+  const float* bias;
+  int32_t n_bias, masks;
+  const uint32_t* mask;
+  const int32_t* mask_rows;
+  int64_t mask_stride;
+} zcu_logits_rules;
+ZC_API int32_t zcu_process_logits(const void* logits, int32_t dtype, int64_t logits_stride, float* out,
+                                  int64_t out_stride, int32_t rows, int32_t vocab, const zcu_logits_rules* rules,
+                                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,420 @@
+"""Block tables, paged append, page-sparse attention, adapters and logits rules against plain 64-bit restatements."""
+import numpy as np
+import pytest
+import torch
+
+from zeroplatform_b200 import ops
+from zeroplatform_b200._lib import ZcError
+
+pytestmark = pytest.mark.gpu
+
+
+def dev(a, dtype=None):
+    t = torch.from_numpy(np.ascontiguousarray(a))
+    return (t if dtype is None else t.to(dtype)).cuda()
+
+
+def ints(a):
+    return torch.tensor(a, dtype=torch.int32, device="cuda")
+
+
+# ---------------------------------------------------------------------------------------------------------
+# block tables
+# ---------------------------------------------------------------------------------------------------------
+
+
+class Pool:
+    """The page pool's rules on the host."""
+
+    def __init__(self, rng, max_rows, max_pages, num_pages, page):
+        self.page = page
+        self.table = np.full((max_rows, max_pages), -1, np.int64)
+        self.lens = np.zeros(max_rows, np.int64)
+        self.free = np.zeros(num_pages, np.int64)
+        self.free[:] = rng.permutation(num_pages)
+        self.count = num_pages
+
+    def reserve(self, rows, new, tokens):
+        start, granted, named, pages = [0], [], set(), 0
+        slots = np.full(tokens, -1, np.int64)
+        pos, row_of, ctx = np.zeros(tokens, np.int64), np.full(tokens, -1, np.int64), np.zeros(tokens, np.int64)
+        top = self.count
+        for r, n in zip(rows, new):
+            n = max(int(n), 0)
+            start.append(start[-1] + n)
+            ok = 0 <= r < len(self.lens) and r not in named
+            named.add(r)
+            if ok:
+                old = int(self.lens[r])
+                ok = old + n <= self.table.shape[1] * self.page and start[-1] <= tokens
+            if ok:
+                have, need = -(-old // self.page), -(-(old + n) // self.page)
+                pages += need - have
+                ok = pages <= top
+            granted.append(int(ok))
+            if not ok:
+                continue
+            for c in range(have, need):
+                self.count -= 1
+                self.table[r, c] = self.free[self.count]
+            for i in range(n):
+                t, p = start[-2] + i, old + i
+                slots[t] = self.table[r, p // self.page] * self.page + p % self.page
+                pos[t], row_of[t], ctx[t] = p, r, p + 1
+            self.lens[r] = old + n
+        return np.array(start), slots, pos, row_of, ctx, np.array(granted)
+
+    def trim(self, rows, new):
+        named = set()
+        use = []
+        for r, n in zip(rows, new):
+            use.append(0 <= r < len(self.lens) and r not in named)
+            named.add(r)
+        for (r, n), ok in reversed(list(zip(zip(rows, new), use))):
+            if not ok:
+                continue
+            keep = min(max(int(n), 0), int(self.lens[r]))
+            for c in range(-(-int(self.lens[r]) // self.page) - 1, -(-keep // self.page) - 1, -1):
+                self.free[self.count] = self.table[r, c]
+                self.count += 1
+                self.table[r, c] = -1
+            self.lens[r] = keep
+
+
+def upload(p):
+    return (dev(p.table, torch.int32), dev(p.lens, torch.int32), dev(p.free, torch.int32), ints([p.count]))
+
+
+def same_pool(p, d):
+    assert d[3].item() == p.count
+    np.testing.assert_array_equal(d[0].cpu().numpy(), p.table)
+    np.testing.assert_array_equal(d[1].cpu().numpy(), p.lens)
+    np.testing.assert_array_equal(d[2].cpu().numpy(), p.free)
+
+
+def same_plan(plan, want):
+    for name, got, ref in zip(plan._fields, plan, want):
+        np.testing.assert_array_equal(got.cpu().numpy(), ref, err_msg=name)
+
+
+@pytest.mark.parametrize("batch,max_rows,max_pages,num_pages,page,hi", [
+    (1, 1, 4, 4, 16, 9), (3, 7, 8, 20, 16, 40), (64, 64, 40, 1500, 16, 3), (130, 200, 33, 2100, 8, 70),
+    (37, 64, 9, 200, 5, 30), (1500, 2000, 4, 3000, 16, 12)])
+def test_pages_follow_the_host(batch, max_rows, max_pages, num_pages, page, hi):
+    """Steps of ragged requests on a pool that runs full, each trimmed a little: every array as the host has it."""
+    rng = np.random.default_rng(batch * 31 + page)
+    p = Pool(rng, max_rows, max_pages, num_pages, page)
+    d = upload(p)
+    for step in range(6):
+        rows = rng.permutation(max_rows)[:batch]
+        new = rng.integers(-1, hi + 1, batch)
+        tokens = int(np.maximum(new, 0).sum()) + int(rng.integers(-3, 9))
+        tokens = max(tokens, 0)
+        plan = ops.reserve_pages(*d, ints(new), page, rows=ints(rows), tokens=tokens)
+        same_plan(plan, p.reserve(rows, new, tokens))
+        same_pool(p, d)
+        rows = rng.permutation(max_rows)[:batch]
+        new = np.where(rng.random(batch) < 0.3, 0, p.lens[rows] - rng.integers(-2, hi // 2 + 2, batch))
+        ops.trim_pages(*d, ints(new), page, rows=ints(rows))
+        p.trim(rows, new)
+        same_pool(p, d)
+
+
+def test_pages_refuse_rows_out_of_range_and_named_twice():
+    rng = np.random.default_rng(1)
+    p = Pool(rng, 6, 8, 30, 4)
+    d = upload(p)
+    rows, new = [3, -1, 3, 6, 0, 2 ** 31 - 1, 5], [5, 2, 9, 1, 4, 1, 0]
+    plan = ops.reserve_pages(*d, ints(new), 4, rows=ints(rows), tokens=22)
+    same_plan(plan, p.reserve(rows, new, 22))
+    assert plan.granted.tolist() == [1, 0, 0, 0, 1, 0, 1]
+    ops.trim_pages(*d, ints([2, 0, 0, 0, 3, 0, 0]), 4, rows=ints(rows))
+    p.trim(rows, [2, 0, 0, 0, 3, 0, 0])
+    same_pool(p, d)
+
+
+def test_pages_empty_steps():
+    rng = np.random.default_rng(2)
+    p = Pool(rng, 4, 8, 8, 16)
+    d = upload(p)
+    plan = ops.reserve_pages(*d, ints([]), 16, tokens=3)
+    assert plan.start.tolist() == [0] and plan.slots.tolist() == [-1] * 3 and plan.ctx_len.tolist() == [0] * 3
+    plan = ops.reserve_pages(*d, ints([0, 0]), 16, tokens=0)
+    assert plan.granted.tolist() == [1, 1] and plan.start.tolist() == [0, 0, 0]
+    ops.trim_pages(*d, ints([]), 16)
+    same_pool(p, d)
+
+
+def test_pages_taken_back_leave_the_stack_as_it_was():
+    rng = np.random.default_rng(3)
+    p = Pool(rng, 40, 30, 700, 16)
+    d = upload(p)
+    ops.reserve_pages(*d, ints(rng.integers(1, 60, 40)), 16, tokens=3000)
+    before = [t.clone() for t in d]
+    ops.reserve_pages(*d, ints(rng.integers(0, 200, 40)), 16, tokens=9000)
+    ops.trim_pages(*d, before[1], 16)
+    for a, b in zip(before, d):
+        assert torch.equal(a, b)
+
+
+def test_pages_slots_pass_32_bits():
+    """A pool of few pages that are very long: the slot is page * page_size in 64 bits."""
+    page = 1 << 30
+    table, lens = torch.full((1, 2), -1, dtype=torch.int32, device="cuda"), ints([0])
+    free, count = ints([6, 7]), ints([2])
+    plan = ops.reserve_pages(table, lens, free, count, ints([2]), page, tokens=2)
+    assert plan.slots.tolist() == [7 * page, 7 * page + 1]
+
+
+def test_pages_in_a_captured_graph_and_on_a_side_stream():
+    rng = np.random.default_rng(4)
+    p = Pool(rng, 16, 64, 1024, 16)
+    d = upload(p)
+    new, out = ints([3] * 16), ops.PagePlan.empty(16, 48)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        ops.reserve_pages(*d, new, 16, out=out)
+    torch.cuda.current_stream().wait_stream(s)
+    p.reserve(range(16), [3] * 16, 48)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.reserve_pages(*d, new, 16, out=out)
+    for _ in range(5):
+        g.replay()
+        want = p.reserve(range(16), [3] * 16, 48)
+        same_plan(out, want)
+    same_pool(p, d)
+
+
+# ---------------------------------------------------------------------------------------------------------
+# paged append
+# ---------------------------------------------------------------------------------------------------------
+
+
+def key_bounds(k):
+    """k [..., tokens, hd] as stored -> (codes [..., 2, hd], scales [...]), from the definition in 64 bits."""
+    k = k.astype(np.float64)
+    lo, hi = k.min(-2), k.max(-2)
+    s = (np.maximum(np.abs(lo), np.abs(hi)).max(-1) / 127).astype(np.float32)
+    d = np.where(s > 0, s, 1).astype(np.float64)[..., None]
+    c = np.stack([np.floor(lo / d), np.ceil(hi / d)], -2)
+    return np.clip(c, -127, 127).astype(np.int8), s
+
+
+@pytest.mark.parametrize("head_major", [True, False])
+@pytest.mark.parametrize("src,dst", [("float32", "float16"), ("float16", "float16"), ("float32", "float32"),
+                                     ("float16", "float32")])
+@pytest.mark.parametrize("hkv,hd,page,lens", [
+    (2, 128, 16, [(0, 1), (5, 1), (15, 1), (16, 1), (47, 1)]), (3, 64, 16, [(0, 40), (7, 33), (31, 2), (12, 0)]),
+    (1, 256, 8, [(3, 50)]), (5, 32, 5, [(4, 19), (0, 5), (9, 1)]), (8, 128, 64, [(10, 200), (64, 64), (1, 62)]),
+    (12, 64, 16, [(3, 900)])])
+def test_append_stores_rows_and_bounds(hkv, hd, page, lens, src, dst, head_major):
+    rng = np.random.default_rng(hkv * hd + page)
+    per = max(-(-(a + b) // page) for a, b in lens)
+    pages = len(lens) * per + 2
+    table = rng.permutation(pages)
+    pool = [rng.standard_normal((pages, hkv, page, hd)).astype(dst) for _ in range(2)]
+    slots, last = [], {}
+    for b, (old, new) in enumerate(lens):
+        for p in range(old, old + new):
+            slots.append(table[b * per + p // page] * page + p % page)
+            last[slots[-1] // page] = p % page + 1
+        slots.append(-1)  # padding between the sequences
+    slots += [pages * page, 1 << 40]
+    rows = [rng.standard_normal((len(slots), hkv, hd)).astype(src) for _ in range(2)]
+    # a wider activation row than the heads fill, as a slice of fused q | k | v
+    wide = torch.zeros((len(slots), 2 * hkv * hd + 8), dtype=getattr(torch, src), device="cuda")
+    k, v = (wide[:, i * hkv * hd:(i + 1) * hkv * hd].view(-1, hkv, hd) for i in range(2))
+    k.copy_(dev(rows[0]))
+    v.copy_(dev(rows[1]))
+
+    def up(x):
+        return dev(x) if head_major else dev(x.transpose(0, 2, 1, 3)).transpose(1, 2)
+
+    kp, vp = up(pool[0]), up(pool[1])
+    bounds = torch.full((pages, hkv, 2, hd), 99, dtype=torch.int8, device="cuda")
+    scales = torch.full((pages, hkv), -7.0, device="cuda")
+    ops.append_kv(k, v, dev(np.array(slots, np.int64)), kp, vp, bounds, scales)
+    for t, s in enumerate(slots):
+        if 0 <= s < pages * page:
+            pool[0][s // page, :, s % page] = rows[0][t].astype(dst)
+            pool[1][s // page, :, s % page] = rows[1][t].astype(dst)
+    np.testing.assert_array_equal(kp.cpu().numpy(), pool[0])
+    np.testing.assert_array_equal(vp.cpu().numpy(), pool[1])
+    got_b, got_s = bounds.cpu().numpy(), scales.cpu().numpy()
+    for p in range(pages):
+        if p in last:
+            want_b, want_s = key_bounds(pool[0][p, :, :last[p]])
+            np.testing.assert_array_equal(got_s[p], want_s)
+            np.testing.assert_array_equal(got_b[p], want_b)
+        else:  # a page that nothing was written to keeps its bounds
+            assert (got_b[p] == 99).all() and (got_s[p] == -7).all()
+
+
+def test_append_bounds_hold_the_keys_and_odd_values_stay_finite():
+    """lo * s <= k <= hi * s up to the ulp of the largest key, for zeros, subnormals and powers of two; a page with an
+    infinite key has zero codes."""
+    k = torch.zeros((6, 1, 64), device="cuda")
+    k[1] = 2.0 ** -24
+    k[2] = torch.linspace(-1, 1, 64, device="cuda")
+    k[3] = 2.0 ** torch.arange(-32, 32, device="cuda").float()
+    k[4, 0, 3] = float("inf")
+    k[5] = torch.randn(64, device="cuda") * 1e-42
+    pools = [torch.zeros((6, 1, 16, 64), device="cuda") for _ in range(2)]
+    bounds, scales = torch.zeros((6, 1, 2, 64), dtype=torch.int8, device="cuda"), torch.zeros((6, 1), device="cuda")
+    ops.append_kv(k, k, torch.arange(6, device="cuda") * 16, *pools, bounds, scales)
+    b, s = bounds.double().cpu()[:, 0], scales.double().cpu()[:, 0, None]
+    kk = k[:, 0].double().cpu()
+    for p in (0, 1, 2, 3):
+        slack = kk[p].abs().max() * 2.0 ** -23
+        assert (b[p, 0] * s[p] <= kk[p] + slack).all() and (b[p, 1] * s[p] >= kk[p] - slack).all(), p
+        assert (b[p].abs() <= 127).all()
+    assert (b[4] == 0).all() and torch.isinf(s[4]).all()
+    assert (b[5].abs() <= 127).all()
+    assert (pools[0][4, 0, 0] == k[4, 0]).all()
+
+
+def test_append_without_bounds_and_of_nothing():
+    k = torch.randn((3, 2, 128), device="cuda")
+    pools = [torch.zeros((4, 2, 16, 128), device="cuda", dtype=torch.float16) for _ in range(2)]
+    ops.append_kv(k, k, torch.tensor([0, 1, 63], device="cuda"), *pools)
+    assert torch.equal(pools[0][3, :, 15], k[2].half()) and torch.equal(pools[1][0, :, 1], k[1].half())
+    ops.append_kv(k[:0], k[:0], torch.empty(0, dtype=torch.int64, device="cuda"), *pools)
+    with pytest.raises(ZcError):
+        ops.append_kv(k, k, torch.tensor([0, 1], device="cuda"), *pools)
+    with pytest.raises(ZcError):
+        ops.append_kv(k.double(), k.double(), torch.tensor([0, 1, 2], device="cuda"), *pools)
+
+
+# ---------------------------------------------------------------------------------------------------------
+# logits rules
+# ---------------------------------------------------------------------------------------------------------
+
+
+def plain_logits(x, past, past_len, prompt_len, past_rows, rep, freq, pres, bias, mask, mask_rows):
+    """(values, magnitude of what was added up) in 64 bits; bias: a list of (ids, values) per row."""
+    v, big = x.astype(np.float64), np.abs(x.astype(np.float64))
+    rows, vocab = x.shape
+    for r in range(rows):
+        if past is not None and 0 <= past_rows[r] < len(past):
+            h = past[past_rows[r]][:past_len[past_rows[r]]]
+            gen = h[prompt_len[past_rows[r]]:]
+            ok = h[(h >= 0) & (h < vocab)]
+            for t in np.unique(ok):
+                v[r, t] = v[r, t] / rep[r] if v[r, t] > 0 else v[r, t] * rep[r]
+                c = int((gen == t).sum())
+                big[r, t] = max(abs(x[r, t]), abs(v[r, t])) + abs(freq[r]) * c + abs(pres[r])
+                if c:
+                    v[r, t] -= float(freq[r]) * c + float(pres[r])
+        if bias is not None:
+            for t, b in zip(*bias[r]):
+                if 0 <= t < vocab:
+                    v[r, t] += float(b)
+                    big[r, t] += abs(float(b))
+        if mask is not None and 0 <= mask_rows[r] < len(mask):
+            bits = np.unpackbits(mask[mask_rows[r]].view(np.uint8), bitorder="little")[:vocab]
+            v[r, bits == 0] = -np.inf
+    return v, big
+
+
+def rules(rng, rows, vocab, cap, n_bias, masks, dup=True):
+    past = rng.integers(-2, vocab + 2, (rows + 1, cap)).astype(np.int32)
+    past[:, cap // 2:] = past[:, :cap - cap // 2]  # repeats, across the prompt's end
+    past_len = rng.integers(0, cap + 1, rows + 1).astype(np.int32)
+    past_len[0] = cap
+    prompt_len = (past_len * rng.random(rows + 1)).astype(np.int32)
+    past_rows = rng.permutation(rows + 1)[:rows].astype(np.int32)
+    if rows > 2:
+        past_rows[1] = -1
+    rep, freq, pres = (rng.random(rows).astype(np.float32) * k + o for k, o in ((0.8, 0.9), (1.0, -0.3), (1.0, -0.2)))
+    if rows > 3:
+        rep[2], freq[2], pres[2] = 1, 0, 0
+    bias = None
+    if n_bias:
+        bias = []
+        for r in range(rows):
+            n = 0 if r == rows - 1 and rows > 1 else n_bias
+            ids = rng.integers(-1, vocab + 1, n).astype(np.int32)
+            if dup and n > 2:
+                ids[-1] = ids[0]
+                ids[n // 2] = ids[0]
+            bias.append((ids, rng.standard_normal(n).astype(np.float32) * 3))
+    mask = mask_rows = None
+    if masks:
+        mask = rng.integers(-2 ** 31, 2 ** 31, (masks, (vocab + 31) // 32 + 1)).astype(np.int32)
+        mask[0] = 0  # a state that allows nothing
+        mask_rows = rng.integers(-1, masks + 1, rows).astype(np.int32)
+        mask_rows[0] = 0 if rows > 1 else masks - 1
+    return past, past_len, prompt_len, past_rows, rep, freq, pres, bias, mask, mask_rows
+
+
+@pytest.mark.parametrize("x_type", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("rows,vocab,cap,n_bias,masks", [
+    (1, 1, 1, 1, 1), (1, 32000, 700, 0, 2), (2, 31, 5, 3, 2), (5, 1000, 64, 0, 0), (4, 1003, 300, 40, 3),
+    (9, 8193, 17, 5, 4), (3, 100003, 4000, 300, 2), (6, 131072, 333, 1, 0)])
+def test_logits_rules(rows, vocab, cap, n_bias, masks, x_type):
+    """Tolerance: at most 8 fp32 roundings (quotient or product, frequency times count, three sums, the bias sum's two
+    more), each half an ulp (2^-24) of no more than the magnitudes added up."""
+    rng = np.random.default_rng(rows * 7 + vocab)
+    t = getattr(torch, x_type)
+    x = (torch.from_numpy(rng.standard_normal((rows, vocab)).astype(np.float32)) * 4).to(t)
+    x[0, 0] = float("nan")
+    x[rows - 1, vocab // 2] = -float("inf")
+    a = rules(rng, rows, vocab, cap, n_bias, masks)
+    past, past_len, prompt_len, past_rows, rep, freq, pres, bias, mask, mask_rows = a
+    with np.errstate(invalid="ignore"):
+        want, big = plain_logits(x.double().numpy(), *a)
+    kw = dict(past=dev(past), past_len=dev(past_len), prompt_len=dev(prompt_len), past_rows=dev(past_rows),
+              repetition=dev(rep), frequency=dev(freq), presence=dev(pres))
+    if bias:
+        kw.update(bias_start=ints(np.cumsum([0] + [len(b[0]) for b in bias])),
+                  bias_ids=dev(np.concatenate([b[0] for b in bias])), bias=dev(np.concatenate([b[1] for b in bias])))
+    if masks:
+        kw.update(mask=dev(mask), mask_rows=dev(mask_rows))
+    tol = 8 * 2.0 ** -24 * np.where(np.isfinite(big), big, 0)
+
+    def near(got):
+        got = got.cpu().numpy().astype(np.float64)
+        np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+        fine = np.isfinite(want)
+        np.testing.assert_array_equal(got[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)])
+        assert (np.abs(got - want)[fine] <= tol[fine]).all()
+
+    first = ops.process_logits(x.cuda(), **kw)
+    near(first)
+    # a strided input into a strided, misaligned output
+    wide = torch.full((rows, 2 * vocab + 3), 5.0, dtype=t, device="cuda")
+    wide[:, 1:1 + vocab] = x.cuda()
+    out = torch.full((rows, vocab + 3), -1.0, device="cuda")
+    ops.process_logits(wide[:, 1:1 + vocab], out=out[:, 2:2 + vocab], **kw)
+    assert torch.equal(out[:, 2:2 + vocab].nan_to_num(), first.nan_to_num())
+    assert (out[:, :2] == -1).all() and (out[:, 2 + vocab:] == -1).all()
+    if t is torch.float32:  # in place
+        y = x.cuda()
+        assert ops.process_logits(y, **kw) is y
+        assert torch.equal(y.nan_to_num(), first.nan_to_num())
+
+
+def test_logits_without_rules_are_a_copy():
+    x = torch.randn((3, 777), device="cuda", dtype=torch.bfloat16)
+    assert torch.equal(ops.process_logits(x), x.float())
+    y = x.float()
+    assert torch.equal(ops.process_logits(y, past=torch.empty((3, 0), dtype=torch.int32, device="cuda"),
+                                          past_len=ints([0, 0, 0]), repetition=torch.full((3,), 2.0, device="cuda")),
+                       x.float())
+    assert ops.process_logits(x[:0]).shape == (0, 777)
+
+
+def test_logits_refuse():
+    x = torch.randn((3, 64), device="cuda")
+    with pytest.raises(ZcError):
+        ops.process_logits(x, past=ints([[1]]), past_len=ints([1]))  # one history for three rows
+    with pytest.raises(ZcError):
+        ops.process_logits(x, bias=torch.ones(1, device="cuda"))
+    with pytest.raises(ZcError):
+        ops.process_logits(x, mask=ints([[1], [1], [1]]))  # 64 tokens need two words
+    with pytest.raises(ZcError):
+        ops.process_logits(x.double())
+    with pytest.raises(ZcError):
+        ops.process_logits(x.t())

@@ -1,0 +1,86 @@
+"""The mixed-serving-batch operators refuse on the host, before any device work, what they do not cover (no GPU)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from zeroplatform_b200 import _lib
+
+BUF = np.zeros(4096 + 4, np.float64)  # never dereferenced: every call below is refused first
+P = (BUF.ctypes.data + 15) // 16 * 16
+
+
+def reserve(table=P, lens=P, free=P, count=P, max_rows=4, max_pages=8, num_pages=16, page=16, rows=None, new=P,
+            batch=2, tokens=8, start=P, slots=P, pos=P, trow=P, ctx=P, granted=P):
+    return _lib.lib().zcu_pages_reserve(table, lens, free, count, max_rows, max_pages, num_pages, page, rows, new,
+                                        batch, tokens, start, slots, pos, trow, ctx, granted, None)
+
+
+@pytest.mark.parametrize("bad", [dict(table=None), dict(lens=None), dict(free=None), dict(count=None), dict(new=None),
+                                 dict(start=None), dict(slots=None), dict(pos=None), dict(trow=None), dict(ctx=None),
+                                 dict(granted=None), dict(max_rows=0), dict(max_pages=0), dict(num_pages=0),
+                                 dict(page=0), dict(page=-16), dict(batch=-1), dict(tokens=-1), dict(batch=5)])
+def test_reserve_refuses(bad):
+    assert reserve(**bad) == -2
+    assert b"zcu_pages_reserve" in _lib.lib().zc_cuda_last_error()
+
+
+def test_reserve_refuses_more_than_one_cta_holds():
+    assert reserve(batch=20000, max_rows=20000) == -6
+    assert reserve(batch=4, max_rows=60000, rows=P) == -6
+
+
+def trim(table=P, lens=P, free=P, count=P, max_rows=4, max_pages=8, num_pages=16, page=16, rows=None, new=P, batch=2):
+    return _lib.lib().zcu_pages_trim(table, lens, free, count, max_rows, max_pages, num_pages, page, rows, new, batch,
+                                     None)
+
+
+@pytest.mark.parametrize("bad", [dict(table=None), dict(lens=None), dict(free=None), dict(count=None), dict(new=None),
+                                 dict(max_rows=0), dict(page=0), dict(batch=-1), dict(batch=5)])
+def test_trim_refuses(bad):
+    assert trim(**bad) == -2
+
+
+def test_trim_of_nothing_is_nothing():
+    assert trim(batch=0) == 0
+
+
+def append(k=P, v=P, in_dtype=0, ks=256, vs=256, slots=P, tokens=2, kp=P, vp=P, kv_dtype=1, hkv=2, hd=128, page=16,
+           pages=4, sp=4096, ss=128, sh=2048, bounds=P, scales=P):
+    return _lib.lib().zcu_append_kv(k, v, in_dtype, ks, vs, slots, tokens, kp, vp, kv_dtype, hkv, hd, page, pages, sp,
+                                    ss, sh, bounds, scales, None)
+
+
+@pytest.mark.parametrize("bad", [dict(k=None), dict(v=None), dict(slots=None), dict(kp=None), dict(vp=None),
+                                 dict(bounds=None), dict(scales=None), dict(in_dtype=2), dict(kv_dtype=-1),
+                                 dict(hkv=0), dict(hd=0), dict(page=0), dict(pages=0), dict(tokens=-1), dict(ks=258),
+                                 dict(ss=130), dict(k=P + 4), dict(kp=P + 4), dict(bounds=P + 1)])
+def test_append_refuses(bad):
+    assert append(**bad) == -2
+
+
+def test_append_covers_four_head_sizes():
+    assert append(hd=96) == -4 and append(hd=512) == -4 and append(hd=16) == -4
+    assert append(tokens=0, k=None, v=None, slots=None) == 0
+
+
+def logits(x=P, dtype=0, xs=64, out=P + 1024, os=64, rows=2, vocab=64, **rules):
+    r = _lib.LogitsRules(**rules)
+    return _lib.lib().zcu_process_logits(x, dtype, xs, out, os, rows, vocab, C.byref(r), None)
+
+
+@pytest.mark.parametrize("bad", [dict(x=None), dict(out=None), dict(dtype=3), dict(dtype=-1), dict(rows=-1),
+                                 dict(vocab=0), dict(xs=63), dict(os=63), dict(past=P, past_cap=4, past_count=2),
+                                 dict(past=P, past_len=P, past_cap=-1, past_count=2),
+                                 dict(past=P, past_len=P, past_cap=4, past_count=0),
+                                 dict(bias_start=P, n_bias=3), dict(bias_start=P, n_bias=-1),
+                                 dict(mask=P, masks=2, mask_stride=1), dict(mask=P, masks=0, mask_stride=2),
+                                 dict(mask=P, masks=1, mask_stride=2), dict(out=P, dtype=1), dict(out=P, os=128)])
+def test_logits_refuses(bad):
+    assert logits(**bad) == -2
+
+
+def test_logits_refuses_a_vocabulary_that_no_cluster_holds():
+    assert logits(vocab=409601, xs=409632, os=409632) == -6
+    assert logits(rows=0) == 0
+    assert _lib.lib().zcu_process_logits(P, 0, 64, P, 64, 1, 64, None, None) == -2

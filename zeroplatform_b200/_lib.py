@@ -148,6 +148,24 @@ SIGNATURES.update({
 })
 
 
+class LogitsRules(C.Structure):
+    """zcu_logits_rules (include/zero_tensor_cuda.h)."""
+
+    _fields_ = [("past", vp), ("past_len", vp), ("prompt_len", vp), ("past_rows", vp), ("past_cap", i32),
+                ("past_count", i32), ("repetition", vp), ("frequency", vp), ("presence", vp), ("bias_start", vp),
+                ("bias_ids", vp), ("bias", vp), ("n_bias", i32), ("masks", i32), ("mask", vp), ("mask_rows", vp),
+                ("mask_stride", i64)]
+
+
+SIGNATURES.update({
+    "zcu_pages_reserve": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, vp, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp]),
+    "zcu_pages_trim": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, vp, vp, i32, vp]),
+    "zcu_append_kv": (i32, [vp, vp, i32, i64, i64, vp, i32, vp, vp, i32, i32, i32, i32, i32, i64, i64, i64, vp, vp,
+                            vp]),
+    "zcu_process_logits": (i32, [vp, i32, i64, vp, i64, i32, i32, C.POINTER(LogitsRules), vp]),
+})
+
+
 class ZcError(RuntimeError):
     pass
 

@@ -1,0 +1,289 @@
+// pages.cu -- block tables and slot maps from request lengths, on the device.
+//
+// The engine's PagedKvCache bookkeeping (PagedKvCache.cs:105-271: a page stack, a table row per sequence) for callers
+// whose lengths live on the GPU: a step that decides on the device how many tokens each request adds (speculative
+// drafts, sampled stops, padded graphs) gets its pages, slots and positions without a host round trip.
+//
+//   reserve  request b on table row r: old = len[r], n = max(n_new, 0); more = ceil((old + n) / P) - ceil(old / P)
+//            pages, the j-th of them free[count - 1 - (pages of the requests before it) - j]; token t of the step
+//            belongs to the request whose [start[b], start[b + 1]) holds it.
+//   trim     pages past ceil(min(new, old) / P) go back to the stack, the last request's last page first, so that a
+//            reserve taken back leaves the stack as it was.
+//
+// Both are chains of a few dependent loads (row -> length -> scan -> stack -> store): latency bound at every size that
+// a step has, so each is one launch.  A cluster of up to 8 CTAs shares the tokens; every CTA does the whole scan
+// (2 loads per request), and the cluster barrier separates these reads from the new lengths and count, which only the
+// first CTA writes.  No atomics on global memory: the result does not depend on the order of anything.
+
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <utility>
+
+#include "batch_ops.h"
+#include "common.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace zc {
+
+namespace {
+
+constexpr int PG_THREADS = 1024;
+constexpr size_t PG_SMEM_MAX = 220 * 1024;
+
+// Exclusive prefix of v over the block's threads (red: 33 words); *total gets the sum.
+__device__ __forceinline__ long long block_prefix(long long v, long long* red, long long* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += u;
+  }
+  if (lane == 31) red[warp] = inc;
+  __syncthreads();
+  if (warp == 0) {
+    long long w = red[lane];  // PG_THREADS / 32 == 32 warps
+    long long wi = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, wi, o);
+      if (lane >= o) wi += u;
+    }
+    red[lane] = wi - w;
+    if (lane == 31) red[32] = wi;
+  }
+  __syncthreads();
+  const long long r = red[warp] + inc - v;
+  *total = red[32];
+  __syncthreads();
+  return r;
+}
+
+__device__ __forceinline__ int pages_of(long long tokens, int page) { return (int)((tokens + page - 1) / page); }
+
+// What both kernels keep per request in shared memory.
+struct Req {
+  int* row;    // table row, -1: not usable (out of range, or a row that an earlier request of the call names)
+  int* old;    // tokens stored
+  int* first;  // pages stored (reserve) or kept (trim)
+  int* poff;   // [batch + 1] pages moved by the requests before it (trim: behind it)
+  int* start;  // [batch + 1] first token (reserve only)
+};
+
+// Table rows of the requests; a row named twice belongs to the first request that names it.
+__device__ void load_rows(const PagePool& p, const int32_t* rows, int batch, const Req& q, int* owner) {
+  if (!rows) {
+    for (int b = threadIdx.x; b < batch; b += PG_THREADS) q.row[b] = b;  // batch <= max_rows
+    __syncthreads();
+    return;
+  }
+  for (int b = threadIdx.x; b < batch; b += PG_THREADS) {
+    const int r = rows[b];
+    q.row[b] = (unsigned)r < (unsigned)p.max_rows ? r : -1;
+    if (q.row[b] >= 0) owner[r] = 0x7fffffff;
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < batch; b += PG_THREADS)
+    if (q.row[b] >= 0) atomicMin(&owner[q.row[b]], b);
+  __syncthreads();
+  for (int b = threadIdx.x; b < batch; b += PG_THREADS)
+    if (q.row[b] >= 0 && owner[q.row[b]] != b) q.row[b] = -1;
+  __syncthreads();
+}
+
+// The last i in [0, n) with at[i] <= v (at ascending, at[0] <= v).
+__device__ __forceinline__ int find(const int* at, int n, int v) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (at[mid] <= v)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(PG_THREADS) reserve_kernel(PagePool p, const int32_t* __restrict__ rows,
+                                                               const int32_t* __restrict__ n_new, int batch,
+                                                               int tokens, PagePlanOut o) {
+  extern __shared__ int sm[];
+  __shared__ long long red[33];
+  pdl_trigger();
+  pdl_wait();
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = cluster.block_rank(), ranks = cluster.num_blocks();
+  const int P = p.page_size;
+  const Req q{sm, sm + batch, sm + 2 * batch, sm + 3 * batch, sm + 4 * batch + 1};
+  load_rows(p, rows, batch, q, sm + 5 * batch + 2);
+  const int count = min(max(*p.free_count, 0), p.num_pages);
+
+  // each thread owns `per` consecutive requests
+  const int per = (batch + PG_THREADS - 1) / PG_THREADS;
+  const int b0 = min(batch, (int)threadIdx.x * per), b1 = min(batch, b0 + per);
+  long long sum = 0, total;
+  for (int b = b0; b < b1; ++b) sum += max(n_new[b], 0);
+  long long at = block_prefix(sum, red, &total);
+  const long long whole = total;
+  long long more = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int n = max(n_new[b], 0), r = q.row[b];
+    const int old = r >= 0 ? max(p.len[r], 0) : 0;
+    q.start[b] = (int)min(at, (long long)0x7fffffff);
+    at += n;
+    const bool fits = r >= 0 && (long long)old + n <= (long long)p.max_pages * P && at <= tokens;
+    const int have = pages_of(old, P);
+    q.old[b] = old;
+    q.first[b] = fits ? have : -1;
+    if (fits) more += pages_of((long long)old + n, P) - have;
+  }
+  if (threadIdx.x == 0) q.start[batch] = (int)min(whole, (long long)0x7fffffff);
+  long long off = block_prefix(more, red, &total);
+  long long taken = 0;
+  for (int b = b0; b < b1; ++b) {
+    q.poff[b] = (int)min(off, (long long)count);
+    if (q.first[b] < 0) continue;
+    const int n = max(n_new[b], 0), m = pages_of((long long)q.old[b] + n, P) - q.first[b];
+    off += m;
+    if (off > count)
+      q.first[b] = -1;  // refused, as every later request that needs a page
+    else
+      taken += m;
+  }
+  block_prefix(taken, red, &total);
+  const int used = (int)total;  // the granted requests' pages: the first `used` of the prefix
+  if (threadIdx.x == 0) q.poff[batch] = used;
+  cluster.sync();  // every CTA has read the lengths and the count (and, as a block barrier, filled its shared memory)
+
+  if (rank == 0) {
+    if (threadIdx.x == 0) *p.free_count = count - used;
+    for (int b = threadIdx.x; b < batch; b += PG_THREADS) {
+      const bool ok = q.first[b] >= 0;
+      o.granted[b] = ok;
+      o.start[b] = q.start[b];
+      if (ok) p.len[q.row[b]] = q.old[b] + max(n_new[b], 0);
+    }
+    if (threadIdx.x == 0) o.start[batch] = q.start[batch];
+  }
+  const int tid = rank * PG_THREADS + threadIdx.x, step = ranks * PG_THREADS;
+  // new pages into the tables: the i-th page popped belongs to the last request whose poff is <= i.  A refused
+  // request's poff is at least `used`, a request without new pages is followed by one with the same poff.
+  for (int i = tid; i < used; i += step) {
+    const int b = find(q.poff, batch, i);
+    p.table[(size_t)q.row[b] * p.max_pages + q.first[b] + (i - q.poff[b])] = p.free_list[count - 1 - i];
+  }
+  for (int t = tid; t < tokens; t += step) {
+    int64_t slot = -1;
+    int pos = 0, row = -1, ctx = 0;
+    if (t < q.start[batch]) {
+      const int b = find(q.start, batch, t);
+      if (q.first[b] >= 0) {
+        pos = q.old[b] + (t - q.start[b]);
+        row = q.row[b];
+        ctx = pos + 1;
+        const int col = pos / P, fresh = col - q.first[b];
+        const int page = fresh < 0 ? p.table[(size_t)row * p.max_pages + col]
+                                   : p.free_list[count - 1 - (q.poff[b] + fresh)];
+        slot = (int64_t)page * P + (pos - col * P);
+      }
+    }
+    o.slots[t] = slot;
+    o.positions[t] = pos;
+    o.token_rows[t] = row;
+    o.ctx_len[t] = ctx;
+  }
+}
+
+__global__ void __launch_bounds__(PG_THREADS) trim_kernel(PagePool p, const int32_t* __restrict__ rows,
+                                                            const int32_t* __restrict__ new_len, int batch) {
+  extern __shared__ int sm[];
+  __shared__ long long red[33];
+  pdl_trigger();
+  pdl_wait();
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = cluster.block_rank(), ranks = cluster.num_blocks();
+  const int P = p.page_size;
+  const Req q{sm, sm + batch, sm + 2 * batch, sm + 3 * batch, nullptr};
+  load_rows(p, rows, batch, q, sm + 4 * batch + 1);
+  const int count = min(max(*p.free_count, 0), p.num_pages);
+  const int per = (batch + PG_THREADS - 1) / PG_THREADS;
+  // requests in reverse order: index i is request batch - 1 - i
+  const int i0 = min(batch, (int)threadIdx.x * per), i1 = min(batch, i0 + per);
+  long long gone = 0, total;
+  for (int i = i0; i < i1; ++i) {
+    const int b = batch - 1 - i, r = q.row[b];
+    const int old = r >= 0 ? min(max(p.len[r], 0), (int)min((long long)p.max_pages * P, 0x7fffffffLL)) : 0;
+    const int keep = min(max(new_len[b], 0), old);
+    q.old[b] = pages_of(old, P);
+    q.first[b] = pages_of(keep, P);
+    gone += q.old[b] - q.first[b];
+  }
+  long long off = block_prefix(gone, red, &total);
+  for (int i = i0; i < i1; ++i) {
+    const int b = batch - 1 - i;
+    q.poff[i] = (int)min(off, 0x7fffffffLL);  // by reverse index: ascending
+    off += q.old[b] - q.first[b];
+  }
+  // a stack never grows past the pool: what a broken table names beyond it is dropped
+  const int back = (int)min(total, (long long)(p.num_pages - count));
+  cluster.sync();
+  if (rank == 0) {
+    if (threadIdx.x == 0) *p.free_count = count + back;
+    for (int b = threadIdx.x; b < batch; b += PG_THREADS)
+      if (q.row[b] >= 0) {
+        const int r = q.row[b], old = p.len[r];
+        p.len[r] = max(min(max(new_len[b], 0), old), 0);
+      }
+  }
+  const int tid = rank * PG_THREADS + threadIdx.x, step = ranks * PG_THREADS;
+  const int moved = (int)min(total, 0x7fffffffLL);
+  for (int j = tid; j < moved; j += step) {
+    const int i = find(q.poff, batch, j), b = batch - 1 - i;
+    int32_t* e = p.table + (size_t)q.row[b] * p.max_pages + (q.old[b] - 1 - (j - q.poff[i]));
+    if (j < back) p.free_list[count + j] = *e;
+    *e = -1;
+  }
+}
+
+int check(const PagePool& p, int batch) {
+  if (!p.table || !p.len || !p.free_list || !p.free_count || batch < 0) return kBadArgument;
+  if (p.max_rows <= 0 || p.max_pages <= 0 || p.num_pages <= 0 || p.page_size <= 0) return kBadArgument;
+  return kOk;
+}
+
+int cluster_for(long long items) { return items <= 2 * PG_THREADS ? 1 : items <= 8 * PG_THREADS ? 4 : 8; }
+
+}  // namespace
+
+int pages_reserve(const PagePool& p, const int32_t* rows, const int32_t* n_new, int batch, int tokens,
+                  const PagePlanOut& o, cudaStream_t s) {
+  if (const int rc = check(p, batch)) return rc;
+  if (tokens < 0 || !o.start || (batch > 0 && (!n_new || !o.granted))) return kBadArgument;
+  if (tokens > 0 && (!o.slots || !o.positions || !o.token_rows || !o.ctx_len)) return kBadArgument;
+  if (!rows && batch > p.max_rows) return kBadArgument;
+  const size_t smem = ((size_t)5 * batch + 2 + (rows ? p.max_rows : 0)) * sizeof(int);
+  if (smem > PG_SMEM_MAX) return kTooLarge;
+  if (allow_smem(reserve_kernel, smem)) return kCudaError;
+  const int c = cluster_for(tokens);
+  return launch_cluster_pdl(reserve_kernel, dim3(c), dim3(PG_THREADS), c, smem, s, p, rows, n_new, batch, tokens, o) ==
+                 cudaSuccess
+             ? kOk
+             : kCudaError;
+}
+
+int pages_trim(const PagePool& p, const int32_t* rows, const int32_t* new_len, int batch, cudaStream_t s) {
+  if (const int rc = check(p, batch)) return rc;
+  if (batch == 0) return kOk;
+  if (!new_len || (!rows && batch > p.max_rows)) return kBadArgument;
+  const size_t smem = ((size_t)4 * batch + 1 + (rows ? p.max_rows : 0)) * sizeof(int);
+  if (smem > PG_SMEM_MAX) return kTooLarge;
+  if (allow_smem(trim_kernel, smem)) return kCudaError;
+  const int c = cluster_for((long long)batch * 16);  // the host does not know how many pages go back
+  return launch_cluster_pdl(trim_kernel, dim3(c), dim3(PG_THREADS), c, smem, s, p, rows, new_len, batch) == cudaSuccess
+             ? kOk
+             : kCudaError;
+}
+
+}  // namespace zc

@@ -7,6 +7,9 @@ Names and argument meaning follow the reference (kzxl/ZeroPlatform):
 * ``TensorBlas.gemv_q8_0 / gemv_q4_0`` -- ZeroTensor/src/ZeroTensor.Core/TensorBlas.Quantized.cs:447-485
   (host arrays in, host array out; goes through the reference bridge ABI ``zc_gemv_*``)
 * ``TensorOps.paged_attention`` -- ZeroTensor/src/ZeroTensor.Core/TensorOps.Neural.cs:2372-2476
+* ``reserve_pages``, ``trim_pages``, ``append_kv``, ``process_logits`` --
+  one step of a mixed serving batch, its state on the device (no counterpart in the reference, whose page tables,
+  histories and sampling rules are per call on the host)
 * ``QuantizedWeight`` -- a weight uploaded once and kept in the device layout (the repack of the
   reference's BlockQ8_0 / BlockQ4_0 arrays, BlockQ8_0.cs:10-17, BlockQ4_0.cs:10-17).
 
@@ -16,12 +19,14 @@ managed code on a non-zero status).
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import numpy as np
 import torch
 
 import ctypes as C
 
-from ._lib import ZcError, check, lib
+from ._lib import LogitsRules, ZcError, check, lib
 
 QK = 32
 Q8_BYTES = 34
@@ -222,3 +227,176 @@ class LlmSampler:
         check(lib().zcu_sample(lg.data_ptr(), rows, vocab, _ptr(past_t), _ptr(plen_t), pcap, C.byref(cfg), _ptr(u_t),
                                out.data_ptr(), None, None, None, 0, _stream(stream)), "sample")
         return out
+
+
+# ---- one step of a mixed serving batch (zcu_pages_*, zcu_append_kv, zcu_process_logits) ----
+
+_FLOAT_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _call(fn, what: str, device: torch.device, stream, *args):
+    """fn(*args, stream) on `device`, whichever device is current; the stream defaults to that device's current one."""
+    if device.index == torch.cuda.current_device():
+        s = torch._C._cuda_getCurrentRawStream(device.index) if stream is None else stream.cuda_stream
+        rc = fn(*args, s)
+    else:
+        with torch.cuda.device(device):
+            s = torch.cuda.current_stream() if stream is None else stream
+            rc = fn(*args, s.cuda_stream)
+    if rc:
+        check(rc, what)
+
+
+def _arg(what: str, t, dtype, device, shape=None):
+    """The address of a contiguous CUDA tensor of that type (None: NULL) and, if given, shape."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.device != device or not t.is_contiguous() or (shape is not None and t.shape != shape):
+        raise ZcError(f"{what} must be a contiguous {dtype} tensor on {device}"
+                      f"{'' if shape is None else f' of shape {tuple(shape)}'}, got {t.dtype} {tuple(t.shape)} "
+                      f"on {t.device}")
+    return t.data_ptr()
+
+
+def _cuda(what: str, t) -> torch.device:
+    if not (torch.is_tensor(t) and t.is_cuda):
+        raise ZcError(f"{what} must be a CUDA tensor")
+    return t.device
+
+
+def _pool_args(page_table, seq_len, free_pages, free_count, page_size):
+    dev = _cuda("page_table", page_table)
+    if page_table.dim() != 2 or free_pages.dim() != 1:
+        raise ZcError("page_table must be [max_rows, max_pages] and free_pages [num_pages]")
+    rows, cols = page_table.shape
+    i = torch.int32
+    return dev, (_arg("page_table", page_table, i, dev), _arg("seq_len", seq_len, i, dev, (rows,)),
+                 _arg("free_pages", free_pages, i, dev), _arg("free_count", free_count, i, dev, (1,)), rows, cols,
+                 free_pages.shape[0], page_size)
+
+
+class PagePlan(NamedTuple):
+    """What reserve_pages says of a step's tokens: start [batch + 1], slots int64 [tokens], positions, token_rows and
+    ctx_len [tokens], granted [batch] (int32)."""
+
+    start: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+    token_rows: torch.Tensor
+    ctx_len: torch.Tensor
+    granted: torch.Tensor
+
+    @staticmethod
+    def empty(batch: int, tokens: int, device="cuda") -> "PagePlan":
+        e = lambda n, t=torch.int32: torch.empty(n, dtype=t, device=device)  # noqa: E731
+        return PagePlan(e(batch + 1), e(tokens, torch.int64), e(tokens), e(tokens), e(tokens), e(batch))
+
+
+def reserve_pages(page_table, seq_len, free_pages, free_count, n_new, page_size: int, rows=None, tokens=None, out=None,
+                  stream=None) -> PagePlan:
+    """Block tables and slot maps from request lengths, on the device (zcu_pages_reserve): request b adds n_new[b]
+    tokens to table row rows[b] (None: row b) of the pool (page_table [max_rows, max_pages], seq_len [max_rows], the
+    stack free_pages [num_pages] of *free_count ids; int32, updated in place).  `tokens` is the length of the step's
+    token arrays (room behind the last token is padding), taken from `out` (a PagePlan to write to) when that is
+    given."""
+    dev, pool = _pool_args(page_table, seq_len, free_pages, free_count, page_size)
+    batch = n_new.shape[0]
+    if out is None:
+        if tokens is None:
+            raise ZcError("reserve_pages needs tokens, the length of the step's token arrays, or out")
+        out = PagePlan.empty(batch, tokens, dev)
+    start, slots, positions, token_rows, ctx_len, granted = out
+    n = slots.shape[0]
+    if tokens is not None and tokens != n:
+        raise ZcError(f"out has room for {n} tokens, not {tokens}")
+    i, at = torch.int32, (n,)
+    _call(lib().zcu_pages_reserve, "reserve_pages", dev, stream, *pool, _arg("rows", rows, i, dev, (batch,)),
+          _arg("n_new", n_new, i, dev, (batch,)), batch, n, _arg("start", start, i, dev, (batch + 1,)),
+          _arg("slots", slots, torch.int64, dev, at), _arg("positions", positions, i, dev, at),
+          _arg("token_rows", token_rows, i, dev, at), _arg("ctx_len", ctx_len, i, dev, at),
+          _arg("granted", granted, i, dev, (batch,)))
+    return out if isinstance(out, PagePlan) else PagePlan(*out)
+
+
+def trim_pages(page_table, seq_len, free_pages, free_count, new_len, page_size: int, rows=None, stream=None) -> None:
+    """Row rows[b] (None: row b) keeps min(new_len[b], its length) tokens; the pages behind them go back to the stack
+    (zcu_pages_trim).  new_len 0 frees a sequence; a shorter one takes rejected drafts back."""
+    dev, pool = _pool_args(page_table, seq_len, free_pages, free_count, page_size)
+    batch = new_len.shape[0]
+    _call(lib().zcu_pages_trim, "trim_pages", dev, stream, *pool, _arg("rows", rows, torch.int32, dev, (batch,)),
+          _arg("new_len", new_len, torch.int32, dev, (batch,)), batch)
+
+
+def _kv_pools(k_pool, v_pool, dev):
+    """(dtype code, pages, hkv, page size, hd, page / slot / head stride) of pools [pages, hkv, page size, hd], any
+    strides with contiguous heads; a [pages, page size, hkv, hd] pool is passed as pool.transpose(1, 2)."""
+    if k_pool.dim() != 4 or k_pool.shape != v_pool.shape or k_pool.stride() != v_pool.stride():
+        raise ZcError("k_pool and v_pool must be [pages, kv heads, page size, head size] with the same strides")
+    if k_pool.dtype not in (torch.float32, torch.float16) or v_pool.dtype != k_pool.dtype:
+        raise ZcError("k_pool and v_pool must be fp32 or fp16")
+    if k_pool.device != dev or v_pool.device != dev or k_pool.stride(3) != 1:
+        raise ZcError(f"k_pool and v_pool must be on {dev} with contiguous heads")
+    n, hkv, page, hd = k_pool.shape
+    sp, sh, ss, _ = k_pool.stride()
+    return _FLOAT_CODE[k_pool.dtype], n, hkv, page, hd, sp, ss, sh
+
+
+def append_kv(k, v, slots, k_pool, v_pool, bounds=None, scales=None, stream=None) -> None:
+    """Keys and values [tokens, hkv, hd] (fp32 or fp16; any token stride) into paged pools [pages, hkv, page size, hd]
+    at slots [tokens] (int64; reserve_pages' slots, negative ones skipped).  bounds int8 [pages, hkv, 2, hd] and
+    scales fp32 [pages, hkv] receive the 8-bit key bounds of the pages written, which sparse_paged_attention scores
+    pages by (zcu_append_kv)."""
+    dev = _cuda("k", k)
+    code, pages, hkv, page, hd, sp, ss, sh = _kv_pools(k_pool, v_pool, dev)
+    if k.shape != v.shape or k.dim() != 3 or k.shape[1:] != (hkv, hd) or k.dtype != v.dtype or v.device != dev:
+        raise ZcError(f"k and v must both be [tokens, {hkv}, {hd}] of one type on one device")
+    if k.dtype not in (torch.float32, torch.float16):
+        raise ZcError("k and v must be fp32 or fp16")
+    tokens = k.shape[0]
+    for name, t in (("k", k), ("v", v)):
+        if t.stride(2) != 1 or (hkv > 1 and t.stride(1) != hd):
+            raise ZcError(f"{name}'s heads must be contiguous")
+    _call(lib().zcu_append_kv, "append_kv", dev, stream, k.data_ptr(), v.data_ptr(), _FLOAT_CODE[k.dtype], k.stride(0),
+          v.stride(0), _arg("slots", slots, torch.int64, dev, (tokens,)), tokens, k_pool.data_ptr(),
+          v_pool.data_ptr(), code, hkv, hd, page, pages, sp, ss, sh,
+          _arg("bounds", bounds, torch.int8, dev, (pages, hkv, 2, hd)),
+          _arg("scales", scales, torch.float32, dev, (pages, hkv)))
+
+
+def process_logits(logits, out=None, past=None, past_len=None, prompt_len=None, past_rows=None, repetition=None,
+                   frequency=None, presence=None, bias_start=None, bias_ids=None, bias=None, mask=None, mask_rows=None,
+                   stream=None):
+    """Per-request rules on logits [rows, vocab] (fp32, fp16 or bf16; any row stride) before LlmSampler.sample: penalties
+    for the tokens of a history, biases, grammar masks (zcu_process_logits).  Writes fp32 to `out`, by default the
+    logits themselves when these are fp32 and a new tensor otherwise, and returns it.
+
+    past [n, cap], past_len [n], prompt_len [n]: histories, row past_rows[r] (None: r) for row r; repetition divides
+    positive logits (multiplies others) of every token seen, frequency and presence are subtracted for the ones behind
+    the prompt, each [rows] fp32.  bias_start [rows + 1], bias_ids, bias: each row's biased tokens.  mask [m, words]
+    int32: bit t % 32 of word t / 32 allows token t; row r uses mask_rows[r] (None: r; outside: unmasked)."""
+    dev = _cuda("logits", logits)
+    if logits.dim() != 2 or logits.dtype not in _FLOAT_CODE or (logits.numel() and logits.stride(1) != 1):
+        raise ZcError("logits must be [rows, vocab] fp32, fp16 or bf16 with contiguous rows")
+    rows, vocab = logits.shape
+    if out is None:
+        out = logits if logits.dtype is torch.float32 else torch.empty((rows, vocab), dtype=torch.float32, device=dev)
+    if out.shape != logits.shape or out.dtype is not torch.float32 or out.device != dev or \
+            (out.numel() and out.stride(1) != 1):
+        raise ZcError(f"out must be [{rows}, {vocab}] fp32 on {dev} with contiguous rows")
+    i, f, at = torch.int32, torch.float32, (rows,)
+    n, cap = (0, 0) if past is None else past.shape
+    masks, words = (0, 0) if mask is None else mask.shape
+    n_bias = 0 if bias is None else bias.shape[0]
+    if past is not None and past_rows is None and n < rows:
+        raise ZcError(f"past has {n} rows for {rows} rows of logits and no past_rows")
+    if (bias_start is None) != (bias is None) or (bias_ids is None) != (bias is None):
+        raise ZcError("bias_start, bias_ids and bias go together")
+    r = LogitsRules(_arg("past", past, i, dev), _arg("past_len", past_len, i, dev, (n,)),
+                    _arg("prompt_len", prompt_len, i, dev, (n,)), _arg("past_rows", past_rows, i, dev, at), cap, n,
+                    _arg("repetition", repetition, f, dev, at), _arg("frequency", frequency, f, dev, at),
+                    _arg("presence", presence, f, dev, at), _arg("bias_start", bias_start, i, dev, (rows + 1,)),
+                    _arg("bias_ids", bias_ids, i, dev, (n_bias,)), _arg("bias", bias, f, dev), n_bias, masks,
+                    _arg("mask", mask, i, dev), _arg("mask_rows", mask_rows, i, dev, at), words)
+    _call(lib().zcu_process_logits, "process_logits", dev, stream, logits.data_ptr(), _FLOAT_CODE[logits.dtype],
+          logits.stride(0), out.data_ptr(), out.stride(0), rows, vocab, C.byref(r))
+    return out
