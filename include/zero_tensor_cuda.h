@@ -387,6 +387,30 @@ ZC_API int32_t zcu_append_kv(const void* k, const void* v, int32_t in_dtype, int
                              int32_t hkv, int32_t hd, int32_t page_size, int32_t num_pages, int64_t page_stride,
                              int64_t slot_stride, int64_t head_stride, int8_t* bounds, float* scales, void* stream);
 
+/* Decode attention over a part of a long cache: for every query row and KV head the `budget` pages that an 8-bit upper
+ * bound of q.k scores highest, the first `sink` and the last `recent` pages always among them (sink + recent <=
+ * budget), and paged attention (as zcu_paged_attention) over the tokens of these pages.
+ *   q [batch][hq][hd] fp32, q_stride elements between rows; out [batch][hq][hd]
+ *   pools as in zcu_paged_attention (kv_dtype 0 = fp32, 1 = fp16; 16-byte aligned pieces); bounds and scales as
+ *   zcu_append_kv keeps them, 16-byte aligned
+ *   page_table [table_rows][max_pages]; query b reads row rows[b] (NULL: b) and attends to ctx_len[b] tokens of it; a
+ *   row outside the table or a ctx_len of 0 yields zeros.  max_ctx: an upper bound of ctx_len; longer ones are cut to
+ *   it.  Page ids outside [0, num_pages) rank last and are never read.
+ *   sel int32 [batch][hkv][budget] receives the chosen pages (indices into the table row, ascending), -1 behind them.
+ * score(page) = scale_page * max over the KV head's query heads of s_q * sum_d max(qi_d lo_d, qi_d hi_d), with
+ * s_q = max|q| / 32512 and qi = rint(q / s_q): whole numbers summed exactly and two fp32 products, so the choice
+ * does not depend on the launch; the lower page wins among equal scores.
+ * hd 64, 128 or 256, page_size a multiple of 8 (else -4); -6 when 8 CTAs' shared memory does not hold the scores of
+ * max_ctx tokens (about 300,000 pages). */
+ZC_API int32_t zcu_sparse_paged_attention(const float* q, int64_t q_stride, const void* k_pool, const void* v_pool,
+                                          int32_t kv_dtype, const int8_t* bounds, const float* scales,
+                                          const int32_t* page_table, int32_t table_rows, const int32_t* rows,
+                                          const int32_t* ctx_len, float* out, int32_t* sel, int32_t batch, int32_t hq,
+                                          int32_t hkv, int32_t hd, int32_t page_size, int32_t max_pages,
+                                          int32_t num_pages, int64_t page_stride, int64_t slot_stride,
+                                          int64_t head_stride, float scale, int32_t max_ctx, int32_t budget,
+                                          int32_t sink, int32_t recent, void* stream);
+
 /* Per-request rules on logits [rows][vocab] (dtype 0 = fp32, 1 = fp16, 2 = bf16; strides in elements) before zcu_sample,
  * written as fp32 to out (which may be the logits themselves when these are fp32; no other overlap).  For token t of
  * row r, with `seen` whether t stands in the row's history and c how often it stands behind the prompt:

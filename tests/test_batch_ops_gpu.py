@@ -288,6 +288,203 @@ def test_append_without_bounds_and_of_nothing():
 
 
 # ---------------------------------------------------------------------------------------------------------
+# page-sparse attention
+# ---------------------------------------------------------------------------------------------------------
+
+
+def plain_select(q, codes, scales, n, budget, sink, recent):
+    """q [group, hd] fp32; codes [n, 2, hd]; scales [n] (None entries: no such page) -> ascending page list."""
+    if n <= budget:
+        return list(range(n))
+    top = np.abs(q).max(-1)
+    s_q = (top.astype(np.float64) / 32512).astype(np.float32)
+    d = np.where(s_q > 0, s_q, 1)[:, None].astype(np.float64)
+    qi = np.rint((q / d).astype(np.float32)).astype(np.int64)
+    isum = np.maximum(qi[:, None] * codes[None, :, 0].astype(np.int64),
+                      qi[:, None] * codes[None, :, 1].astype(np.int64)).sum(-1)
+    score = (isum.astype(np.float32) * s_q[:, None]).max(0) * scales
+    order = [(-np.inf if p < sink or p >= n - recent else (np.inf if np.isnan(scales[p]) else -score[p]), p)
+             for p in range(n)]
+    return sorted(p for _, p in sorted(order)[:budget])
+
+
+def plain_attention(q, k, v, scale):
+    """One head group over gathered tokens in 64 bits; also the size of the score terms, for the tolerance."""
+    z = q.astype(np.float64) @ k.T.astype(np.float64) * scale
+    mag = (np.abs(q).astype(np.float64) @ np.abs(k.T).astype(np.float64)).max() * abs(scale) if len(k) else 0.0
+    z = np.exp(z - z.max(-1, keepdims=True))
+    return z @ v.astype(np.float64) / z.sum(-1, keepdims=True), mag
+
+
+def sparse_case(rng, ctx, hq, hkv, hd, page, half, head_major=True, per=None, bad_pages=False):
+    batch = len(ctx)
+    per = per or max(1, max(-(-x // page) for x in ctx))
+    pages = batch * per + 3
+    table = rng.permutation(pages)[:batch * per].reshape(batch, per).astype(np.int32)
+    if bad_pages:
+        table[rng.random(table.shape) < 0.2] = rng.choice([-1, pages, 2 ** 31 - 1])
+    dt = np.float16 if half else np.float32
+    k = (rng.standard_normal((pages, hkv, page, hd)) + 1.5 * rng.standard_normal((pages, hkv, 1, hd))).astype(dt)
+    v = rng.standard_normal((pages, hkv, page, hd)).astype(dt)
+    codes, scales = key_bounds(k)
+    # slots behind a sequence's last token hold anything
+    for b, x in enumerate(ctx):
+        p = table[b, x // page] if x % page else -1
+        if 0 <= p < pages:
+            codes[p], scales[p] = key_bounds(k[p, :, :x % page])
+            k[p, :, x % page:], v[p, :, x % page:] = np.nan, np.inf
+    q = rng.standard_normal((batch, hq, hd)).astype(np.float32)
+
+    def up(x):
+        return dev(x) if head_major else dev(x.transpose(0, 2, 1, 3)).transpose(1, 2)
+
+    return q, k, v, codes, scales, table, (up(k), up(v), dev(codes), dev(scales), dev(table))
+
+
+def check_sparse(q, k, v, codes, scales, table, ctx, budget, sink, recent, out, sel, rows=None):
+    """Selection exactly.  Output tolerance, relative to the largest value attended: a score is off by at most hd
+    roundings of 2^-23 of the terms it adds (products of hi + lo pairs hold 2^-22), which moves a weight by as much
+    relatively, on both sides of the quotient; sums over T tokens add T / 8 accumulator roundings and a constant."""
+    batch, hq, hd = q.shape
+    pages, hkv, page, _ = k.shape
+    group = hq // hkv
+    scale = 1 / np.sqrt(hd)
+    out, sel = out.cpu().numpy(), sel.cpu().numpy()
+    for b in range(batch):
+        r = b if rows is None else rows[b]
+        n = -(-int(ctx[b]) // page) if 0 <= r < len(table) else 0
+        for h in range(hkv):
+            hs = slice(h * group, (h + 1) * group)
+            t = table[r, :n] if n else table[0, :0]
+            ok = (t >= 0) & (t < pages)
+            at = np.where(ok, t, 0)
+            sc = np.where(ok, scales[at, h], np.nan).astype(np.float32)
+            want = plain_select(q[b, hs], codes[at, h], sc, n, budget, sink, recent)
+            assert sel[b, h].tolist() == want + [-1] * (budget - len(want)), (b, h)
+            keep = [(p, j) for p in want if ok[p] for j in range(page) if p * page + j < ctx[b]]
+            if not keep:
+                assert (out[b, hs] == 0).all()
+                continue
+            kk = np.stack([k[t[p], h, j] for p, j in keep])
+            vv = np.stack([v[t[p], h, j] for p, j in keep])
+            ref, mag = plain_attention(q[b, hs], kk, vv, scale)
+            tol = np.abs(vv.astype(np.float64)).max() * (2 * hd * 2.0 ** -23 * mag + (len(keep) / 8 + 64) * 2.0 ** -23)
+            assert np.abs(out[b, hs] - ref).max() <= tol, (b, h, np.abs(out[b, hs] - ref).max(), tol)
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("hq,hkv,hd,page,ctx,budget,sink,recent", [
+    (8, 2, 128, 16, [1, 15, 16, 17, 0, 300], 4, 1, 1), (4, 4, 64, 16, [129, 1000, 64], 8, 0, 1),
+    (32, 8, 128, 16, [2049], 16, 1, 2), (7, 1, 64, 8, [777, 63], 12, 2, 3), (6, 2, 256, 32, [1500, 31], 9, 1, 1),
+    (16, 1, 128, 16, [700, 1200], 20, 1, 4), (24, 2, 64, 24, [1000], 11, 0, 0), (12, 12, 64, 16, [640], 40, 1, 1),
+    (40, 2, 128, 64, [5000, 4999], 30, 1, 1), (8, 8, 128, 16, [333] * 40, 6, 1, 2), (2, 1, 128, 16, [9000], 1, 0, 1)])
+def test_sparse_attention(hq, hkv, hd, page, ctx, budget, sink, recent, half):
+    rng = np.random.default_rng(hq * 100 + hd + page)
+    q, k, v, codes, scales, table, d = sparse_case(rng, ctx, hq, hkv, hd, page, half, head_major=hd != 64)
+    out, sel = ops.sparse_paged_attention(dev(q), *d, ints(ctx), budget, sink=sink, recent=recent)
+    check_sparse(q, k, v, codes, scales, table, ctx, budget, sink, recent, out, sel)
+
+
+@pytest.mark.parametrize("half", [True, False])
+def test_sparse_attention_rows_strides_and_bad_pages(half):
+    """Queries that share table rows, rows without a sequence, a strided q, table entries outside the pool, and a
+    max_ctx below a length."""
+    rng = np.random.default_rng(9)
+    lens = [500, 37, 900]
+    q, k, v, codes, scales, table, d = sparse_case(rng, lens, 8, 2, 128, 16, half, bad_pages=True)
+    rows = [2, 0, 0, -1, 1, 3, 2, 2 ** 31 - 1]
+    ctx = [899, 500, 499, 12, 37, 5, 16, 3]
+    q = rng.standard_normal((8, 8, 128)).astype(np.float32)
+    wide = torch.zeros((8, 12 * 128), device="cuda")
+    wide[:, 128:9 * 128] = dev(q.reshape(8, -1))
+    view = wide[:, 128:9 * 128].view(8, 8, 128)
+    # token 499 of row 0 and 898 of row 2 are the last ones with keys: shorter rows see only stored tokens
+    out, sel = ops.sparse_paged_attention(view, *d, ints(ctx), 10, rows=ints(rows), recent=2)
+    check_sparse(q, k, v, codes, scales, table, ctx, 10, 1, 2, out, sel, rows)
+    cut, sel_cut = ops.sparse_paged_attention(view, *d, ints(ctx), 10, rows=ints(rows), recent=2, max_ctx=320)
+    check_sparse(q, k, v, codes, scales, table, [min(x, 320) for x in ctx], 10, 1, 2, cut, sel_cut, rows)
+
+
+def test_sparse_attention_whole_budget_is_paged_attention():
+    """With a budget that holds every page the result is that of paged_attention_batched (both hold fp32 to 1e-5)."""
+    rng = np.random.default_rng(10)
+    ctx = [1, 200, 640, 0]
+    q, k, v, codes, scales, table, d = sparse_case(rng, ctx, 12, 4, 128, 16, True)
+    out, _ = ops.sparse_paged_attention(dev(q), *d, ints(ctx), 40)
+    pools = [torch.nan_to_num(x, nan=0.0, posinf=0.0) for x in d[:2]]
+    sp, sh, ss, _ = pools[0].stride()
+    ref = ops.paged_attention_batched(dev(q), *pools, d[4], ints(ctx), 4, 16, pools[0].shape[0], sp, ss, sh,
+                                      1 / np.sqrt(128), 640)
+    assert (out - ref).abs().max() <= 1e-5 * ref.abs().max()
+
+
+def test_sparse_attention_extreme_queries():
+    """Queries far outside fp16's range, all zero, and with one element that dwarfs the rest."""
+    rng = np.random.default_rng(11)
+    ctx = [400, 400, 400, 400]
+    q, k, v, codes, scales, table, d = sparse_case(rng, ctx, 4, 2, 64, 16, True)
+    q[0] *= np.float32(1e6)
+    q[1] *= np.float32(1e-20)
+    q[2] = 0
+    q[3, :, 5] = 3e5
+    out, sel = ops.sparse_paged_attention(dev(q), *d, ints(ctx), 7, sink=0)
+    check_sparse(q, k, v, codes, scales, table, ctx, 7, 0, 1, out, sel)
+    q[1, 0, 0] = np.nan
+    out, _ = ops.sparse_paged_attention(dev(q), *d, ints(ctx), 7)
+    assert torch.isnan(out[1, 0]).all() and torch.isfinite(out[0]).all() and torch.isfinite(out[2:]).all()
+
+
+def test_sparse_attention_equal_pages_go_to_the_lower_one():
+    page, hd = 16, 64
+    k = torch.ones((40, 1, page, hd), dtype=torch.float16, device="cuda")
+    k[20:] = 2
+    codes, scales = (dev(x) for x in key_bounds(k.cpu().numpy()))
+    table = torch.arange(40, dtype=torch.int32, device="cuda")[None]
+    q = torch.ones((1, 1, hd), device="cuda")
+    for budget in (3, 20, 25, 39):
+        _, sel = ops.sparse_paged_attention(q, k, k, codes, scales, table, ints([640]), budget, sink=0, recent=0)
+        high = list(range(20, min(40, 20 + budget)))
+        assert sel[0, 0].tolist() == sorted(high + list(range(budget - len(high))))
+
+
+def test_sparse_attention_long_sequence_many_pages():
+    """More pages than one CTA scores, in a pool whose far pages lie beyond 32-bit element offsets."""
+    rng = np.random.default_rng(12)
+    page, hd, n = 8, 64, 20000
+    pages = (1 << 31) // (page * hd) + 64  # elements of the pool: just past 2^31
+    k = torch.zeros((pages, 1, page, hd), dtype=torch.float16, device="cuda")
+    v = torch.zeros_like(k)
+    table = torch.randperm(pages - 1, device="cuda")[:n].int()[None]
+    table[0, -1] = pages - 1
+    q = rng.standard_normal((1, 3, hd)).astype(np.float32)
+    ks = rng.standard_normal((n, 1, page, hd)).astype(np.float16)
+    vs = rng.standard_normal((n, 1, page, hd)).astype(np.float16)
+    at = table[0].long()
+    k[at], v[at] = dev(ks), dev(vs)
+    codes, scales = key_bounds(ks)
+    bounds = torch.zeros((pages, 1, 2, hd), dtype=torch.int8, device="cuda")
+    sc = torch.zeros((pages, 1), device="cuda")
+    bounds[at], sc[at] = dev(codes), dev(scales)
+    ctx = n * page - 3
+    out, sel = ops.sparse_paged_attention(dev(q), k, v, bounds, sc, table, ints([ctx]), 50)
+    check_sparse(q, ks, vs, codes, scales, np.arange(n, dtype=np.int32)[None], [ctx], 50, 1, 1, out, sel)
+
+
+def test_sparse_attention_in_a_captured_graph():
+    rng = np.random.default_rng(13)
+    ctx = [600, 350]
+    q, k, v, codes, scales, table, d = sparse_case(rng, ctx, 8, 2, 128, 16, True)
+    qd, cd = dev(q), ints([100, 350])
+    out, sel = torch.zeros((2, 8, 128), device="cuda"), torch.zeros((2, 2, 9), dtype=torch.int32, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.sparse_paged_attention(qd, *d, cd, 9, out=out, sel=sel)
+    cd.copy_(ints(ctx))
+    g.replay()
+    check_sparse(q, k, v, codes, scales, table, ctx, 9, 1, 1, out, sel)
+
+
+# ---------------------------------------------------------------------------------------------------------
 # logits rules
 # ---------------------------------------------------------------------------------------------------------
 

@@ -64,6 +64,32 @@ def test_append_covers_four_head_sizes():
     assert append(tokens=0, k=None, v=None, slots=None) == 0
 
 
+def sparse(q=P, qs=1024, kp=P, vp=P, kv_dtype=1, bounds=P, scales=P, table=P, table_rows=2, rows=None, ctx=P, out=P,
+           sel=P, batch=2, hq=8, hkv=2, hd=128, page=16, max_pages=64, pages=128, sp=4096, ss=128, sh=2048,
+           max_ctx=1024, budget=8, sink=1, recent=1):
+    return _lib.lib().zcu_sparse_paged_attention(q, qs, kp, vp, kv_dtype, bounds, scales, table, table_rows, rows, ctx,
+                                                 out, sel, batch, hq, hkv, hd, page, max_pages, pages, sp, ss, sh,
+                                                 0.125, max_ctx, budget, sink, recent, None)
+
+
+@pytest.mark.parametrize("bad", [dict(q=None), dict(kp=None), dict(vp=None), dict(bounds=None), dict(scales=None),
+                                 dict(table=None), dict(ctx=None), dict(out=None), dict(sel=None), dict(kv_dtype=2),
+                                 dict(batch=-1), dict(hq=0), dict(hkv=0), dict(hq=7), dict(hd=0), dict(page=0),
+                                 dict(max_pages=0), dict(pages=0), dict(table_rows=0), dict(table_rows=1),
+                                 dict(max_ctx=-1), dict(budget=0), dict(sink=-1), dict(recent=-1),
+                                 dict(sink=5, recent=4), dict(ss=132), dict(kp=P + 8), dict(bounds=P + 8),
+                                 dict(sink=2 ** 31 - 1, recent=2 ** 31 - 1)])
+def test_sparse_attention_refuses(bad):
+    assert sparse(**bad) == -2
+
+
+def test_sparse_attention_covers_three_head_sizes_and_pages_of_eights():
+    assert sparse(hd=96, ss=96) == -4 and sparse(hd=32) == -4 and sparse(hd=512, ss=512) == -4
+    assert sparse(page=20) == -4 and sparse(page=4) == -4
+    assert sparse(max_pages=1 << 20, max_ctx=1 << 24) == -6
+    assert sparse(batch=0) == 0
+
+
 def logits(x=P, dtype=0, xs=64, out=P + 1024, os=64, rows=2, vocab=64, **rules):
     r = _lib.LogitsRules(**rules)
     return _lib.lib().zcu_process_logits(x, dtype, xs, out, os, rows, vocab, C.byref(r), None)

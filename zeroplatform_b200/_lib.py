@@ -162,6 +162,8 @@ SIGNATURES.update({
     "zcu_pages_trim": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, vp, vp, i32, vp]),
     "zcu_append_kv": (i32, [vp, vp, i32, i64, i64, vp, i32, vp, vp, i32, i32, i32, i32, i32, i64, i64, i64, vp, vp,
                             vp]),
+    "zcu_sparse_paged_attention": (i32, [vp, i64, vp, vp, i32, vp, vp, vp, i32, vp, vp, vp, vp] + [i32] * 7 +
+                                   [i64, i64, i64, f32, i32, i32, i32, i32, vp]),
     "zcu_process_logits": (i32, [vp, i32, i64, vp, i64, i32, i32, C.POINTER(LogitsRules), vp]),
 })
 

@@ -90,6 +90,46 @@ int32_t zcu_append_kv(const void* k, const void* v, int32_t in_dtype, int64_t k_
   return done(kv_append(a, as_stream(stream)), "zcu_append_kv");
 }
 
+int32_t zcu_sparse_paged_attention(const float* q, int64_t q_stride, const void* k_pool, const void* v_pool,
+                                   int32_t kv_dtype, const int8_t* bounds, const float* scales,
+                                   const int32_t* page_table, int32_t table_rows, const int32_t* rows,
+                                   const int32_t* ctx_len, float* out, int32_t* sel, int32_t batch, int32_t hq,
+                                   int32_t hkv, int32_t hd, int32_t page_size, int32_t max_pages, int32_t num_pages,
+                                   int64_t page_stride, int64_t slot_stride, int64_t head_stride, float scale,
+                                   int32_t max_ctx, int32_t budget, int32_t sink, int32_t recent, void* stream) {
+  if (kv_dtype & ~1) return done(kBadArgument, "zcu_sparse_paged_attention");
+  SparseAttnArgs a{};
+  a.q = q;
+  a.q_stride = q_stride;
+  a.k_pool = k_pool;
+  a.v_pool = v_pool;
+  a.kv_half = kv_dtype;
+  a.page_stride = page_stride;
+  a.slot_stride = slot_stride;
+  a.head_stride = head_stride;
+  a.bounds = bounds;
+  a.scales = scales;
+  a.page_table = page_table;
+  a.table_rows = table_rows;
+  a.rows = rows;
+  a.ctx_len = ctx_len;
+  a.out = out;
+  a.sel = sel;
+  a.batch = batch;
+  a.hq = hq;
+  a.hkv = hkv;
+  a.hd = hd;
+  a.page_size = page_size;
+  a.max_pages = max_pages;
+  a.num_pages = num_pages;
+  a.scale = scale;
+  a.max_ctx = max_ctx;
+  a.budget = budget;
+  a.sink = sink;
+  a.recent = recent;
+  return done(sparse_attention(a, as_stream(stream)), "zcu_sparse_paged_attention");
+}
+
 int32_t zcu_process_logits(const void* logits, int32_t dtype, int64_t logits_stride, float* out, int64_t out_stride,
                            int32_t rows, int32_t vocab, const zcu_logits_rules* r, void* stream) {
   if (!r) return done(kBadArgument, "zcu_process_logits");

@@ -7,7 +7,7 @@ Names and argument meaning follow the reference (kzxl/ZeroPlatform):
 * ``TensorBlas.gemv_q8_0 / gemv_q4_0`` -- ZeroTensor/src/ZeroTensor.Core/TensorBlas.Quantized.cs:447-485
   (host arrays in, host array out; goes through the reference bridge ABI ``zc_gemv_*``)
 * ``TensorOps.paged_attention`` -- ZeroTensor/src/ZeroTensor.Core/TensorOps.Neural.cs:2372-2476
-* ``reserve_pages``, ``trim_pages``, ``append_kv``, ``process_logits`` --
+* ``reserve_pages``, ``trim_pages``, ``append_kv``, ``sparse_paged_attention``, ``process_logits`` --
   one step of a mixed serving batch, its state on the device (no counterpart in the reference, whose page tables,
   histories and sampling rules are per call on the host)
 * ``QuantizedWeight`` -- a weight uploaded once and kept in the device layout (the repack of the
@@ -19,6 +19,7 @@ managed code on a non-zero status).
 """
 from __future__ import annotations
 
+import math
 from typing import NamedTuple
 
 import numpy as np
@@ -361,6 +362,43 @@ def append_kv(k, v, slots, k_pool, v_pool, bounds=None, scales=None, stream=None
           v_pool.data_ptr(), code, hkv, hd, page, pages, sp, ss, sh,
           _arg("bounds", bounds, torch.int8, dev, (pages, hkv, 2, hd)),
           _arg("scales", scales, torch.float32, dev, (pages, hkv)))
+
+
+def sparse_paged_attention(q, k_pool, v_pool, bounds, scales, page_table, ctx_len, budget: int, rows=None, sink: int = 1,
+                           recent: int = 1, scale=None, max_ctx=None, out=None, sel=None, stream=None):
+    """Decode attention of q [batch, hq, hd] fp32 (any row stride) over the `budget` pages per query and KV head that
+    the key bounds score highest, the first `sink` and last `recent` pages always among them
+    (zcu_sparse_paged_attention).
+
+    Pools [pages, hkv, page size, hd] and bounds / scales as append_kv keeps them; page_table [rows, max_pages] and
+    ctx_len [batch] int32; query b reads table row rows[b] (None: b; reserve_pages' token_rows), so several queries of
+    one sequence may share a row.  max_ctx bounds ctx_len (default: what the table holds).  Returns (out [batch, hq,
+    hd], sel [batch, hkv, budget]: the chosen pages as indices into the table row, ascending, -1 behind them)."""
+    dev = _cuda("q", q)
+    code, pages, hkv, page, hd, sp, ss, sh = _kv_pools(k_pool, v_pool, dev)
+    if q.dim() != 3 or q.dtype is not torch.float32 or q.shape[2] != hd or \
+            (q.numel() and (q.stride(2) != 1 or (q.shape[1] > 1 and q.stride(1) != hd))):
+        raise ZcError(f"q must be [batch, hq, {hd}] fp32 with contiguous heads")
+    batch, hq, _ = q.shape
+    if page_table.dim() != 2:
+        raise ZcError("page_table must be [rows, max_pages]")
+    table_rows, max_pages = page_table.shape
+    if scale is None:
+        scale = 1.0 / math.sqrt(hd)
+    if max_ctx is None:
+        max_ctx = min(max_pages * page, 0x7fffffff)
+    i, f = torch.int32, torch.float32
+    if out is None:
+        out = torch.empty((batch, hq, hd), dtype=f, device=dev)
+    if sel is None:
+        sel = torch.empty((batch, hkv, budget), dtype=i, device=dev)
+    _call(lib().zcu_sparse_paged_attention, "sparse_paged_attention", dev, stream, q.data_ptr(), q.stride(0),
+          k_pool.data_ptr(), v_pool.data_ptr(), code, _arg("bounds", bounds, torch.int8, dev, (pages, hkv, 2, hd)),
+          _arg("scales", scales, f, dev, (pages, hkv)), _arg("page_table", page_table, i, dev), table_rows,
+          _arg("rows", rows, i, dev, (batch,)), _arg("ctx_len", ctx_len, i, dev, (batch,)),
+          _arg("out", out, f, dev, (batch, hq, hd)), _arg("sel", sel, i, dev, (batch, hkv, budget)), batch, hq, hkv,
+          hd, page, max_pages, pages, sp, ss, sh, scale, max_ctx, budget, sink, recent)
+    return out, sel
 
 
 def process_logits(logits, out=None, past=None, past_len=None, prompt_len=None, past_rows=None, repetition=None,
