@@ -400,8 +400,8 @@ ZC_API int32_t zcu_append_kv(const void* k, const void* v, int32_t in_dtype, int
  * score(page) = scale_page * max over the KV head's query heads of s_q * sum_d max(qi_d lo_d, qi_d hi_d), with
  * s_q = max|q| / 32512 and qi = rint(q / s_q): whole numbers summed exactly and two fp32 products, so the choice
  * does not depend on the launch; the lower page wins among equal scores.
- * hd 64, 128 or 256, page_size a multiple of 8 (else -4); -6 when 8 CTAs' shared memory does not hold the scores of
- * max_ctx tokens (about 300,000 pages). */
+ * hd 64, 128 or 256, page_size a multiple of 8 (else -4); -6 when a CTA's shared memory does not hold the scores of
+ * max_ctx tokens (about 50,000 pages). */
 ZC_API int32_t zcu_sparse_paged_attention(const float* q, int64_t q_stride, const void* k_pool, const void* v_pool,
                                           int32_t kv_dtype, const int8_t* bounds, const float* scales,
                                           const int32_t* page_table, int32_t table_rows, const int32_t* rows,

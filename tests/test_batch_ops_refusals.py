@@ -86,7 +86,7 @@ def test_sparse_attention_refuses(bad):
 def test_sparse_attention_covers_three_head_sizes_and_pages_of_eights():
     assert sparse(hd=96, ss=96) == -4 and sparse(hd=32) == -4 and sparse(hd=512, ss=512) == -4
     assert sparse(page=20) == -4 and sparse(page=4) == -4
-    assert sparse(max_pages=1 << 20, max_ctx=1 << 24) == -6
+    assert sparse(max_pages=1 << 20, max_ctx=1 << 20) == -6
     assert sparse(batch=0) == 0
 
 

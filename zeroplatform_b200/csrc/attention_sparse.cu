@@ -13,8 +13,8 @@
 //           is one product of 2 hd signed bytes: mma m16n8k32.s8, eight heads' high bytes of qi in rows 0-7 and their
 //           low bytes in rows 8-15, eight pages as columns.  A page's record goes straight from memory into the
 //           operand registers (16 bytes a lane; the contraction index is permuted alike on both sides).
-//   select  radix select on the order-preserving bits of the scores, 8 bits a pass, histograms summed over the
-//           cluster through distributed shared memory; the chosen pages are handed out in page order.
+//   select  the CTAs exchange their scores through distributed shared memory; each finds the threshold by radix
+//           select on the order-preserving bits, and takes its part of the chosen pages, in page order.
 //   attend  mma m16n8k16 on the raw fp16 keys and values, again from memory into operand registers, with the fp32
 //           query as hi + lo halves in rows 0-7 and 8-15 (a power of two of its own brings each head's query into
 //           fp16's range) and the fp32 weights split the same way: products are exact and the result is fp32 to about
@@ -40,6 +40,7 @@ namespace {
 
 constexpr int SP_WARPS = 8;
 constexpr int SP_THREADS = SP_WARPS * 32;
+constexpr int SP_CLUSTER = 8;  // most CTAs of a cluster
 constexpr int SP_HEADS = 8;  // query heads per pass: half of an mma's 16 rows
 constexpr float SP_LOG2E = 1.4426950408889634f;
 constexpr size_t SP_SMEM_MAX = 220 * 1024;
@@ -48,7 +49,8 @@ struct SparseDev {
   SparseAttnArgs a;
   int cap_pages;  // pages that max_ctx allows
   int share;      // list entries of a CTA: ceil(budget / S)
-  int key_words;  // words of the region that holds a CTA's scores, later the warps' outputs
+  int key_words;  // scores a CTA holds: all pages', where there may be more than the budget
+  int id_words;   // page ids it holds beside them: as many, or 0 where shared memory does not have the room
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -84,10 +86,21 @@ __device__ __forceinline__ void tf32_pair(float v, uint32_t& hi, uint32_t& lo) {
   lo = tf32_of(v - __uint_as_float(hi));
 }
 
-__device__ __forceinline__ uint4 ld_once(const void* p) {
-  const int4 v = ld_stream_v4(p);
-  return make_uint4(v.x, v.y, v.z, v.w);
+// 16 bytes from memory into shared memory, zeros where !ok (nothing is read then)
+__device__ __forceinline__ void copy16(void* dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+               "r"(ok ? 16 : 0)
+               : "memory");
 }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>  // all but the last N groups of this thread have landed
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// 16-byte piece of a row in a warp's buffer.  Operand reads of keys and bounds take rows g, pieces 4 j + c, those of
+// values rows 2 c and 2 c + 1, pieces 8 j + g: either exchange puts the eight lanes of an access on all banks.
+__device__ __forceinline__ int key_piece(int row, int piece) { return piece ^ ((row & 1) * 4); }
+__device__ __forceinline__ int value_piece(int row, int piece) { return piece ^ (row & 6); }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // Unsigned key whose order is the float's (NaN above everything, -0 below 0: callers pass sums that are never -0).
@@ -100,25 +113,28 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 // signed), columns [min(qi, 0) per dim | max(qi, 0) per dim].  sq: s_q per head, -inf factor handled by the caller.
 template <int HD>
 __device__ void stage_score_query(const float* q, int heads, int8_t* qs, int stride, float* sq) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;  // one warp per head
-  float v[HD / 32], top = 0.f;
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int i = 0; i < HD / 32; ++i) {
-    v[i] = warp < heads ? q[warp * HD + lane + 32 * i] : 0.f;
-    top = fmaxf(top, fabsf(v[i]));
-  }
-  top = warp_max(top);
-  const float s = __fdiv_rn(top, 32512.f);
-  if (lane == 0) sq[warp] = s;
+  for (int h = threadIdx.x >> 5; h < SP_HEADS; h += SP_WARPS) {  // one warp per head
+    float v[HD / 32], top = 0.f;
 #pragma unroll
-  for (int i = 0; i < HD / 32; ++i) {
-    const int qi = s > 0.f ? min(max(__float2int_rn(__fdiv_rn(v[i], s)), -32512), 32512) : 0;
-    const int neg = min(qi, 0), pos = max(qi, 0), d = lane + 32 * i;
-    const int8_t nl = (int8_t)(neg & 255), pl = (int8_t)(pos & 255);
-    qs[warp * stride + d] = (int8_t)((neg - nl) >> 8);
-    qs[(warp + 8) * stride + d] = nl;
-    qs[warp * stride + HD + d] = (int8_t)((pos - pl) >> 8);
-    qs[(warp + 8) * stride + HD + d] = pl;
+    for (int i = 0; i < HD / 32; ++i) {
+      v[i] = h < heads ? q[h * HD + lane + 32 * i] : 0.f;
+      top = fmaxf(top, fabsf(v[i]));
+    }
+    top = warp_max(top);
+    const float s = __fdiv_rn(top, 32512.f);
+    if (lane == 0) sq[h] = s;
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) {
+      const int qi = s > 0.f ? min(max(__float2int_rn(__fdiv_rn(v[i], s)), -32512), 32512) : 0;
+      const int neg = min(qi, 0), pos = max(qi, 0), d = lane + 32 * i;
+      const int8_t nl = (int8_t)(neg & 255), pl = (int8_t)(pos & 255);
+      qs[h * stride + d] = (int8_t)((neg - nl) >> 8);
+      qs[(h + 8) * stride + d] = nl;
+      qs[h * stride + HD + d] = (int8_t)((pos - pl) >> 8);
+      qs[(h + 8) * stride + HD + d] = pl;
+    }
   }
 }
 
@@ -126,34 +142,36 @@ __device__ void stage_score_query(const float* q, int heads, int8_t* qs, int str
 // ex[head] = 2^-e undoes the power of two, which puts the largest |q| of the head at 2^7 .. 2^8.
 template <int HD, bool HALF>
 __device__ void stage_query(const float* q, int heads, float scale_log2, void* qa, int stride, float* ex) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float v[HD / 32], top = 0.f;
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int i = 0; i < HD / 32; ++i) {
-    v[i] = warp < heads ? q[warp * HD + lane + 32 * i] * scale_log2 : 0.f;
-    top = fmaxf(top, fabsf(v[i]));
-  }
-  top = warp_max(top);
-  float up = 1.f, down = 1.f;
-  const int e = (int)((__float_as_uint(top) >> 23) & 255u) - 127;  // floor(log2(top)) of a normal number
-  if (HALF && top > 0.f && top < INFINITY) {
-    const int k = min(max(7 - e, -126), 126);
-    up = __uint_as_float((uint32_t)(127 + k) << 23);
-    down = __uint_as_float((uint32_t)(127 - k) << 23);
-  }
-  if (lane == 0) ex[warp] = down;
+  for (int h = threadIdx.x >> 5; h < SP_HEADS; h += SP_WARPS) {
+    float v[HD / 32], top = 0.f;
 #pragma unroll
-  for (int i = 0; i < HD / 32; ++i) {
-    const int d = lane + 32 * i;
-    if (HALF) {
-      __half* o = reinterpret_cast<__half*>(qa);
-      store_hl(o + warp * stride + d, (size_t)8 * stride, v[i] * up);
-    } else {
-      uint32_t hi, lo;
-      tf32_pair(v[i], hi, lo);
-      uint32_t* o = reinterpret_cast<uint32_t*>(qa);
-      o[warp * stride + d] = hi;
-      o[(warp + 8) * stride + d] = lo;
+    for (int i = 0; i < HD / 32; ++i) {
+      v[i] = h < heads ? q[h * HD + lane + 32 * i] * scale_log2 : 0.f;
+      top = fmaxf(top, fabsf(v[i]));
+    }
+    top = warp_max(top);
+    float up = 1.f, down = 1.f;
+    const int e = (int)((__float_as_uint(top) >> 23) & 255u) - 127;  // floor(log2(top)) of a normal number
+    if (HALF && top > 0.f && top < INFINITY) {
+      const int k = min(max(7 - e, -126), 126);
+      up = __uint_as_float((uint32_t)(127 + k) << 23);
+      down = __uint_as_float((uint32_t)(127 - k) << 23);
+    }
+    if (lane == 0) ex[h] = down;
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) {
+      const int d = lane + 32 * i;
+      if (HALF) {
+        store_hl(reinterpret_cast<__half*>(qa) + h * stride + d, (size_t)8 * stride, v[i] * up);
+      } else {
+        uint32_t hi, lo;
+        tf32_pair(v[i], hi, lo);
+        uint32_t* o = reinterpret_cast<uint32_t*>(qa);
+        o[h * stride + d] = hi;
+        o[(h + 8) * stride + d] = lo;
+      }
     }
   }
 }
@@ -193,17 +211,22 @@ struct State {
   }
 };
 
-template <int HD, bool HALF>
-__global__ void __launch_bounds__(SP_THREADS) sparse_attn_kernel(SparseDev dv) {
+template <int HD, bool HALF, int CTAS>
+__global__ void __launch_bounds__(SP_THREADS, CTAS) sparse_attn_kernel(SparseDev dv) {
   const SparseAttnArgs& a = dv.a;
   constexpr int QS = 2 * HD + 16;                    // bytes of a score operand row
   constexpr int QA = HALF ? HD + 8 : HD + 4;         // elements of an attention operand row
   constexpr int ES = HALF ? 2 : 4;
   extern __shared__ __align__(16) unsigned char smem[];
-  uint32_t* keys = reinterpret_cast<uint32_t*>(smem);              // [key_words]: scores of this CTA's pages,
-  float* so = reinterpret_cast<float*>(smem);                      // then [warp][head][HD] outputs
-  unsigned char* at = smem + (size_t)dv.key_words * 4;
-  float* part = reinterpret_cast<float*>(at);                      // [8][HD] this CTA's output
+  constexpr int RING = 64 * HD;                      // a warp's buffer: 32 bounds records, or a block's keys and values
+  unsigned char* ring = smem + (threadIdx.x >> 5) * RING;
+  float* so = reinterpret_cast<float*>(smem);                      // at the end: each warp's outputs
+  unsigned char* at = smem + SP_WARPS * RING;
+  uint32_t* keys = reinterpret_cast<uint32_t*>(at);                // [key_words]: scores of all pages
+  at += (size_t)dv.key_words * 4;
+  int32_t* ids = reinterpret_cast<int32_t*>(at);                   // [id_words]: page ids of the table row
+  at += (size_t)dv.id_words * 4;
+  float* part = reinterpret_cast<float*>(at);                      // this CTA's output, 8 HD floats
   at += SP_HEADS * HD * 4;
   int8_t* qs = reinterpret_cast<int8_t*>(at);                      // [16][QS]
   at += 16 * QS;
@@ -215,12 +238,12 @@ __global__ void __launch_bounds__(SP_THREADS) sparse_attn_kernel(SparseDev dv) {
   __shared__ float wm[SP_WARPS][SP_HEADS], wl[SP_WARPS][SP_HEADS];
   __shared__ float pm[SP_HEADS], pl[SP_HEADS];
   __shared__ int red[2][SP_WARPS];
-  __shared__ int2 counts;
   __shared__ int s_digit, s_rem, s_all;
   pdl_trigger();
   pdl_wait();
 
   cg::cluster_group cluster = cg::this_cluster();
+  cluster.barrier_arrive();
   const int rank = cluster.block_rank(), S = cluster.num_blocks();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const int g = lane >> 2, c = lane & 3;
@@ -234,13 +257,27 @@ __global__ void __launch_bounds__(SP_THREADS) sparse_attn_kernel(SparseDev dv) {
   const int want = min(a.budget, n);
   const float* q = a.q + (size_t)b * a.q_stride + (size_t)kvh * group * HD;
   float* out = a.out + ((size_t)b * a.hq + (size_t)kvh * group) * HD;
+  const bool wide = (uintptr_t)a.out % 16 == 0;  // 16-byte stores
   int32_t* sel = a.sel + ((size_t)b * a.hkv + kvh) * a.budget;
   for (int i = want + rank * SP_THREADS + tid; i < a.budget; i += S * SP_THREADS) sel[i] = -1;
   if (n == 0) {  // the same for the whole cluster
     for (int i = rank * SP_THREADS + tid; i < group * HD; i += S * SP_THREADS) out[i] = 0.f;
+    cluster.barrier_wait();
     return;
   }
   const int32_t* pt = a.page_table + (size_t)row * a.max_pages;
+  const bool keep_ids = dv.id_words > 0 && n > a.budget;
+  if (keep_ids) {
+    for (int i = tid; i < n; i += SP_THREADS)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(ids + i)),
+                   "l"(pt + i)
+                   : "memory");
+  }
+  copies_commit();
+  // the first head tile's operands, while the ids are on their way
+  stage_score_query<HD>(q, min(SP_HEADS, group), qs, QS, sq);
+  stage_query<HD, HALF>(q, min(SP_HEADS, group), a.scale * SP_LOG2E, qa, QA, ex);
+  auto id_of = [&](int p) { return keep_ids ? ids[p] : pt[p]; };
   const int share = (want + S - 1) / S;
 
   if (n <= a.budget) {
@@ -248,16 +285,21 @@ __global__ void __launch_bounds__(SP_THREADS) sparse_attn_kernel(SparseDev dv) {
       list[i - rank * share] = make_int2(pt[i], i);
       sel[i] = i;
     }
+    cluster.barrier_wait();
   } else {
     // ---- score ----
     const int cs = (n + S - 1) / S, p_begin = min(n, rank * cs), p_end = min(n, p_begin + cs);
     for (int i = tid; i < 4 * 256; i += SP_THREADS) hist[0][i] = 0;
-    constexpr int KS = 2 * HD / 64;  // 16-byte pieces of a record per lane; two k-steps of 32 each
+    constexpr int KS = 2 * HD / 64;      // 16-byte pieces of a record per lane; two k-steps of 32 each
+    constexpr int RP = 2 * HD / 16;      // pieces of a record
     for (int h0 = 0; h0 < group; h0 += SP_HEADS) {
       const int heads = min(SP_HEADS, group - h0);
-      __syncthreads();  // hist cleared, the last tile's operand no longer read
-      stage_score_query<HD>(q + (size_t)h0 * HD, heads, qs, QS, sq);
-      __syncthreads();
+      if (h0 > 0) {
+        __syncthreads();  // the last tile's operand is no longer read
+        stage_score_query<HD>(q + (size_t)h0 * HD, heads, qs, QS, sq);
+      }
+      copies_wait<0>();
+      __syncthreads();  // staged, the ids there, and the histograms cleared
       uint4 ah[KS], al[KS];
 #pragma unroll
       for (int j = 0; j < KS; ++j) {
@@ -266,33 +308,67 @@ __global__ void __launch_bounds__(SP_THREADS) sparse_attn_kernel(SparseDev dv) {
       }
       const float s_q = sq[g];
       const bool last = h0 + SP_HEADS >= group;
-      int ph[2];
-      auto page_at = [&](int p) { return p < p_end ? pt[p] : -1; };
-      ph[0] = page_at(p_begin + warp * 16 + g);
-      ph[1] = page_at(p_begin + warp * 16 + 8 + g);
-      for (int p0 = p_begin + warp * 16; p0 < p_end; p0 += SP_WARPS * 16) {
-        uint4 r[2][KS];
-        float scale[2];
-        bool ok[2];
+      // Sixteen pages a stage, two stages in flight; lanes 0-15 hold the pages' ids, scales and whether they exist.
+      int id = -1;
+      float scale[2] = {0.f, 0.f};
+      bool ok[2] = {false, false};
+      auto fetch_ids = [&](int p0) {
+        const int p = p0 + lane;
+        id = lane < 16 && p < p_end ? id_of(p) : -1;
+      };
+      auto issue = [&](int p0, int buf) {
+        const bool in_pool = (unsigned)id < (unsigned)a.num_pages;
+        const size_t rec = in_pool ? (size_t)id * a.hkv + kvh : 0;
+        if (p0 < p_end) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          ok[u] = (unsigned)ph[u] < (unsigned)a.num_pages;
-          const size_t rec = ok[u] ? (size_t)ph[u] * a.hkv + kvh : 0;
-          const int8_t* src = a.bounds + rec * (2 * HD) + 16 * c;
-#pragma unroll
-          for (int j = 0; j < KS; ++j) r[u][j] = ok[u] ? ld_once(src + 64 * j) : make_uint4(0, 0, 0, 0);
-          scale[u] = ok[u] && last ? __ldg(a.scales + rec) : 0.f;
+          for (int i = 0; i < RP / 2; ++i) {
+            const int r = (i * 32 + lane) / RP, piece = (i * 32 + lane) % RP;
+            const size_t from = __shfl_sync(0xffffffffu, rec, r);
+            copy16(ring + buf * 16 * 2 * HD + r * 2 * HD + key_piece(r, piece) * 16, a.bounds + from * (2 * HD) + piece * 16,
+                   __shfl_sync(0xffffffffu, (int)in_pool, r));
+          }
         }
-        ph[0] = page_at(p0 + SP_WARPS * 16 + g);
-        ph[1] = page_at(p0 + SP_WARPS * 16 + 8 + g);
+        copies_commit();
+        scale[0] = scale[1];
+        ok[0] = ok[1];
+        ok[1] = in_pool;
+        scale[1] = in_pool && last ? __ldg(a.scales + rec) : 0.f;
+      };
+      constexpr int STEP = SP_WARPS * 16;
+      const int first = p_begin + warp * 16;
+      fetch_ids(first);
+      issue(first, 0);
+      fetch_ids(first + STEP);
+      issue(first + STEP, 1);
+      fetch_ids(first + 2 * STEP);
+      int buf = 0;
+      for (int p0 = first; p0 < p_end; p0 += STEP) {
+        copies_wait<1>();
+        __syncwarp();
+        int d2[2][4];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           int d[4] = {0, 0, 0, 0};
 #pragma unroll
           for (int j = 0; j < KS; ++j) {
-            mma_s8(d, ah[j].x, al[j].x, ah[j].y, al[j].y, r[u][j].x, r[u][j].y);
-            mma_s8(d, ah[j].z, al[j].z, ah[j].w, al[j].w, r[u][j].z, r[u][j].w);
+            const int r = 8 * u + g;
+            const uint4 rec = *reinterpret_cast<const uint4*>(ring + buf * 16 * 2 * HD + r * 2 * HD +
+                                                              key_piece(r, 4 * j + c) * 16);
+            mma_s8(d, ah[j].x, al[j].x, ah[j].y, al[j].y, rec.x, rec.y);
+            mma_s8(d, ah[j].z, al[j].z, ah[j].w, al[j].w, rec.z, rec.w);
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d2[u][i] = d[i];
+        }
+        __syncwarp();
+        const float sc = scale[0];
+        const bool exists = ok[0];
+        issue(p0 + 2 * STEP, buf);
+        fetch_ids(p0 + 3 * STEP);
+        buf ^= 1;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int(&d)[4] = d2[u];
           // columns (pages) 2c and 2c + 1 of head g; the maximum over the tile's heads
           float f0 = g < heads ? __fmul_rn((float)(d[0] * 256 + d[2]), s_q) : -INFINITY;
           float f1 = g < heads ? __fmul_rn((float)(d[1] * 256 + d[3]), s_q) : -INFINITY;
@@ -301,45 +377,72 @@ __global__ void __launch_bounds__(SP_THREADS) sparse_attn_kernel(SparseDev dv) {
             f0 = fmaxf(f0, __shfl_xor_sync(0xffffffffu, f0, o));
             f1 = fmaxf(f1, __shfl_xor_sync(0xffffffffu, f1, o));
           }
-          // lanes 4i hold page i's scale and validity; lanes 0-3 take the pages 2c and 2c + 1
-          const float c0 = __shfl_sync(0xffffffffu, scale[u], 8 * c), c1 = __shfl_sync(0xffffffffu, scale[u], 8 * c + 4);
-          const int v0 = __shfl_sync(0xffffffffu, (int)ok[u], 8 * c), v1 = __shfl_sync(0xffffffffu, (int)ok[u], 8 * c + 4);
+          // lanes 0-3 take the pages 2c and 2c + 1
+          const int at0 = 8 * u + 2 * c;
+          const float c0 = __shfl_sync(0xffffffffu, sc, at0), c1 = __shfl_sync(0xffffffffu, sc, at0 + 1);
+          const int v0 = __shfl_sync(0xffffffffu, (int)exists, at0), v1 = __shfl_sync(0xffffffffu, (int)exists, at0 + 1);
           if (g == 0) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               const int p = p0 + 8 * u + 2 * c + k;
               if (p >= p_end) continue;
               float f = k ? f1 : f0;
-              if (h0 > 0) f = fmaxf(f, __uint_as_float(keys[p - p_begin]));
-              if (!last) {
-                keys[p - p_begin] = __float_as_uint(f);
-                continue;
-              }
-              uint32_t key = order_key(__fmul_rn(f, k ? c1 : c0) + 0.f);  // + 0: -0 orders as 0
-              if (!(k ? v1 : v0)) key = 0;
-              if (p < a.sink || p >= n - a.recent) key = 0xffffffffu;
-              keys[p - p_begin] = key;
-              atomicAdd(&hist[0][key >> 24], 1u);
+              if (h0 > 0) f = fmaxf(f, __uint_as_float(keys[p]));
+              if (last)  // + 0: -0 orders as 0
+                keys[p] = (k ? v1 : v0) ? order_key(__fmul_rn(f, k ? c1 : c0) + 0.f) : 0u;
+              else
+                keys[p] = __float_as_uint(f);
             }
           }
         }
       }
     }
-    // ---- select the `want` largest keys ----
-    uint32_t prefix = 0, mask = 0;
-    int rem = want;
-    for (int pass = 0; pass < 4; ++pass) {
-      const int shift = 24 - 8 * pass;
-      if (pass > 0)
-        for (int i = p_begin + tid; i < p_end; i += SP_THREADS) {
-          const uint32_t k = keys[i - p_begin];
-          if ((k & mask) == prefix) atomicAdd(&hist[pass][(k >> shift) & 255u], 1u);
-        }
-      cluster.sync();
-      const int digit = 255 - tid;  // SP_THREADS == 256: thread 0 has the highest digit
-      int tot = 0;
-      for (int r = 0; r < S; ++r) tot += (int)cluster.map_shared_rank(&hist[pass][0], r)[digit];
-      int inc = tot;
+    // ---- every CTA gets every key ----
+    __syncthreads();
+    cluster.barrier_wait();  // the other CTAs have started
+    for (int r = 0; r < S; ++r)
+      if (r != rank) {
+        uint32_t* to = cluster.map_shared_rank(keys, r);
+        for (int i = p_begin + tid; i < p_end; i += SP_THREADS) to[i] = keys[i];
+      }
+    cluster.sync();
+    // ---- select: the forced pages, and the `rem` largest keys of the pages [f0, f1) between them ----
+    const int f0 = min(a.sink, n), f1 = max(f0, n - a.recent);
+    int rem = want - (n - (f1 - f0));
+    uint32_t kmin = 0xffffffffu, kmax = 0;
+    for (int i = f0 + tid; i < f1; i += SP_THREADS) {
+      kmin = min(kmin, keys[i]);
+      kmax = max(kmax, keys[i]);
+    }
+    kmin = __reduce_min_sync(0xffffffffu, kmin);
+    kmax = __reduce_max_sync(0xffffffffu, kmax);
+    if (lane == 0) red[0][warp] = (int)kmin, red[1][warp] = (int)kmax;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < SP_WARPS; ++w) {
+      kmin = min(kmin, (uint32_t)red[0][w]);
+      kmax = max(kmax, (uint32_t)red[1][w]);
+    }
+    // Radix select on key - kmin from its highest bit in use (scores share their leading bits): after a pass `cur` are
+    // the leading bits of the threshold, down to bit `shift`.
+    uint32_t cur = 0;
+    int shift = f1 > f0 ? 32 - __clz((int)(kmax - kmin)) : 0;
+    for (int pass = 0; rem > 0; ++pass) {  // at most four: 8 bits each
+      const int bits = min(8, shift);
+      shift -= bits;
+      for (int i = f0 + tid; i < f1; i += SP_THREADS) {
+        const uint32_t k = (keys[i] - kmin) >> shift;
+        if (k >> bits == cur) atomicAdd(&hist[pass][k & ((1u << bits) - 1u)], 1u);
+      }
+      __syncthreads();
+      constexpr int DG = 256 / SP_THREADS;  // digits a thread, the highest first
+      int tot[DG], inc = 0;
+#pragma unroll
+      for (int k = 0; k < DG; ++k) {
+        tot[k] = (int)hist[pass][255 - (tid * DG + k)];
+        inc += tot[k];
+      }
+      const int own = inc;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, inc, o);
@@ -347,72 +450,58 @@ __global__ void __launch_bounds__(SP_THREADS) sparse_attn_kernel(SparseDev dv) {
       }
       if (lane == 31) red[0][warp] = inc;
       __syncthreads();
-      for (int w = 0; w < warp; ++w) inc += red[0][w];
-      if (inc >= rem && inc - tot < rem) {
-        s_digit = digit;
-        s_rem = rem - (inc - tot);
-        s_all = s_rem == tot;
+#pragma unroll
+      for (int w = 0; w < SP_WARPS; ++w) inc += w < warp ? red[0][w] : 0;
+      inc -= own;  // keys with a higher digit than this thread's
+#pragma unroll
+      for (int k = 0; k < DG; ++k) {
+        if (inc < rem && inc + tot[k] >= rem) {
+          s_digit = 255 - (tid * DG + k);
+          s_rem = rem - inc;
+          s_all = rem - inc == tot[k];
+        }
+        inc += tot[k];
       }
       __syncthreads();
-      prefix |= (uint32_t)s_digit << shift;
-      mask |= 255u << shift;
+      cur = cur << bits | (uint32_t)s_digit;
       rem = s_rem;
-      const bool all = s_all;
-      __syncthreads();
-      if (all) break;  // every key with this prefix is taken
+      if (s_all || shift == 0) break;  // every key with these leading bits is taken, or they are all its bits
     }
-    // ---- hand them out in page order: keys above the prefix, and the first `rem` equal to it ----
+    // ---- this CTA's part of the list, in page order: forced, above the threshold, the first `rem` equal to it ----
+    const bool some = want > n - (f1 - f0);  // a threshold was found
+    const int seg = ((n + SP_WARPS - 1) / SP_WARPS + 31) / 32 * 32, w0 = min(n, warp * seg), w1 = min(n, w0 + seg);
+    auto kind = [&](int i) {  // 2: taken, 1: equal to the threshold, 0: not
+      if (i >= w1) return 0;
+      if (i < f0 || i >= f1) return 2;
+      if (!some) return 0;
+      const uint32_t k = (keys[i] - kmin) >> shift;
+      return k > cur ? 2 : k == cur ? 1 : 0;
+    };
     int gt = 0, eq = 0;
-    for (int i = p_begin + tid; i < p_end; i += SP_THREADS) {
-      const uint32_t k = keys[i - p_begin] & mask;
-      gt += k > prefix;
-      eq += k == prefix;
+    for (int i = w0; i < w1; i += 32) {
+      const int k = kind(i + lane);
+      gt += __popc(__ballot_sync(0xffffffffu, k == 2));
+      eq += __popc(__ballot_sync(0xffffffffu, k == 1));
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      gt += __shfl_xor_sync(0xffffffffu, gt, o);
-      eq += __shfl_xor_sync(0xffffffffu, eq, o);
-    }
+    __syncthreads();
     if (lane == 0) red[0][warp] = gt, red[1][warp] = eq;
     __syncthreads();
-    if (tid == 0) {
-      int2 t = make_int2(0, 0);
-      for (int w = 0; w < SP_WARPS; ++w) t.x += red[0][w], t.y += red[1][w];
-      counts = t;
-    }
-    cluster.sync();
-    int eq_seen = 0, pos = 0;  // before this CTA: keys equal to the prefix, entries handed out
-    for (int r = 0; r < rank; ++r) {
-      const int2 t = *cluster.map_shared_rank(&counts, r);
-      pos += t.x;
-      eq_seen += t.y;
-    }
-    pos += min(eq_seen, rem);
-    for (int i0 = p_begin; i0 < p_end; i0 += SP_THREADS) {
-      const int i = i0 + tid;
-      const uint32_t k = i < p_end ? keys[i - p_begin] & mask : 0u;
-      const bool is_eq = i < p_end && k == prefix, is_gt = i < p_end && k > prefix;
-      const unsigned beq = __ballot_sync(0xffffffffu, is_eq), bgt = __ballot_sync(0xffffffffu, is_gt);
-      __syncthreads();
-      if (lane == 0) red[0][warp] = __popc(bgt), red[1][warp] = __popc(beq);
-      __syncthreads();
-      int before_gt = __popc(bgt & ((1u << lane) - 1u)), before_eq = __popc(beq & ((1u << lane) - 1u));
-      int all_gt = 0, all_eq = 0;
-      for (int w = 0; w < SP_WARPS; ++w) {
-        if (w < warp) before_gt += red[0][w], before_eq += red[1][w];
-        all_gt += red[0][w];
-        all_eq += red[1][w];
+    int gt_seen = 0, eq_seen = 0;
+    for (int w = 0; w < warp; ++w) gt_seen += red[0][w], eq_seen += red[1][w];
+    const int l0 = rank * share, l1 = min(want, l0 + share);
+    for (int i = w0; i < w1; i += 32) {
+      const int k = kind(i + lane);
+      const unsigned bgt = __ballot_sync(0xffffffffu, k == 2), beq = __ballot_sync(0xffffffffu, k == 1);
+      const unsigned below = (1u << lane) - 1u;
+      const int e = eq_seen + __popc(beq & below);  // rank among the equal ones
+      const int to = gt_seen + __popc(bgt & below) + min(e, rem);
+      if ((k == 2 || (k == 1 && e < rem)) && to >= l0 && to < l1) {
+        sel[to] = i + lane;
+        list[to - l0] = make_int2(id_of(i + lane), i + lane);
       }
-      const int e = eq_seen + before_eq;  // rank among the equal ones
-      if (is_gt || (is_eq && e < rem)) {
-        const int to = pos + before_gt + min(e, rem) - min(eq_seen, rem);
-        sel[to] = i;
-        cluster.map_shared_rank(list, to / share)[to % share] = make_int2(pt[i], i);
-      }
-      pos += all_gt + min(eq_seen + all_eq, rem) - min(eq_seen, rem);
-      eq_seen += all_eq;
+      gt_seen += __popc(bgt);
+      eq_seen += __popc(beq);
     }
-    cluster.sync();
   }
 
   // ---- attend ----
@@ -434,52 +523,114 @@ __global__ void __launch_bounds__(SP_THREADS) sparse_attn_kernel(SparseDev dv) {
   for (int h0 = 0; h0 < group; h0 += SP_HEADS) {
     const int heads = min(SP_HEADS, group - h0);
     __syncthreads();  // the list is written; the last tile's operand and outputs are no longer read
-    stage_query<HD, HALF>(q + (size_t)h0 * HD, heads, a.scale * SP_LOG2E, qa, QA, ex);
-    __syncthreads();
+    if (h0 > 0) {
+      stage_query<HD, HALF>(q + (size_t)h0 * HD, heads, a.scale * SP_LOG2E, qa, QA, ex);
+      __syncthreads();
+    }
     const float down = ex[g];
     State<HD, HALF> st;
     st.init();
+    // A block is 16 tokens (fp32 pools: 8) of keys and as many of values in the warp's buffer.  The next block's keys
+    // are on their way from when this block's have been read, its values likewise.
+    constexpr int TB = HALF ? 16 : 8, NB = TB / 8;
+    constexpr int ROWB = HD * ES, RPC = ROWB / 16;  // bytes and 16-byte pieces of a row
+    constexpr int HALF_RING = TB * ROWB;            // keys, then values
+    static_assert(2 * HALF_RING == RING, "a block's keys and values fill the warp's buffer");
     const long long row_bytes = a.slot_stride * ES;
-    if constexpr (HALF) {
-      const __half* qh = reinterpret_cast<const __half*>(qa);
-      for (int i0 = warp * 16; i0 < tokens; i0 += SP_WARPS * 16) {
-        long long off[2];
-        int nv[2];
-        nv[0] = locate(i0, off[0]);
-        nv[1] = locate(i0 + 8, off[1]);
-        uint4 kr[2][HD / 32], vr[4][HD / 64];
+    constexpr int RPI = 32 / RPC > 0 ? 32 / RPC : 1;  // rows that a warp's copy instruction covers
+    constexpr int IPR = RPC > 32 ? RPC / 32 : 1;      // instructions per row where a row has more than 32 pieces
+    const int row0 = IPR > 1 ? 0 : lane / RPC, piece0 = IPR > 1 ? lane : lane % RPC;
+    const unsigned char* const k_lane = kb + row0 * row_bytes + piece0 * 16;
+    const unsigned char* const v_lane = vb + row0 * row_bytes + piece0 * 16;
+    auto copy_rows = [&](const unsigned char* from, unsigned char* to, const long long (&off)[NB], const int (&nv)[NB],
+                         bool keys_) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < NB; ++u) {
+        const unsigned char* src = from + off[u];
 #pragma unroll
-          for (int j = 0; j < HD / 32; ++j)
-            kr[u][j] = g < nv[u] ? ld_once(kb + off[u] + g * row_bytes + 64 * j + 16 * c) : make_uint4(0, 0, 0, 0);
-        auto load_v = [&]() {
+        for (int i = 0; i < 8; i += RPI) {
+          const int r = i + row0;
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
+          for (int k = 0; k < IPR; ++k) {
+            const int piece = piece0 + 32 * k;
+            copy16(to + (8 * u + r) * ROWB + (keys_ ? key_piece(r, piece) : value_piece(r, piece)) * 16, src + 512 * k,
+                   r < nv[u]);
+          }
+          src += RPI * row_bytes;
+        }
+      }
+      copies_commit();
+    };
+    long long off[NB];
+    int nv[NB];
+    int i0 = warp * TB;
+    if (i0 < tokens) {
 #pragma unroll
-            for (int j = 0; j < HD / 64; ++j) {
-              const int t = 2 * c + (u & 1);
-              vr[u][j] = t < nv[u >> 1] ? ld_once(vb + off[u >> 1] + t * row_bytes + 128 * j + 16 * g)
-                                        : make_uint4(0, 0, 0, 0);
-            }
-        };
-        if (HD <= 128) load_v();
-        float s[4];
+      for (int u = 0; u < NB; ++u) nv[u] = locate(i0 + 8 * u, off[u]);
+      copy_rows(k_lane, ring, off, nv, true);
+      copy_rows(v_lane, ring + HALF_RING, off, nv, false);
+    }
+    for (; i0 < tokens; i0 += SP_WARPS * TB) {
+      const bool more = i0 + SP_WARPS * TB < tokens;
+      long long off_next[NB];
+      int nv_next[NB];
+#pragma unroll
+      for (int u = 0; u < NB; ++u) nv_next[u] = locate(i0 + SP_WARPS * TB + 8 * u, off_next[u]);
+      copies_wait<1>();  // the keys
+      __syncwarp();
+      float s[2 * NB];
+      if constexpr (HALF) {
+        const __half* qh = reinterpret_cast<const __half*>(qa);
+        float z[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) {
+          const uint4 ah = *reinterpret_cast<const uint4*>(qh + g * QA + 32 * j + 8 * c);
+          const uint4 al = *reinterpret_cast<const uint4*>(qh + (g + 8) * QA + 32 * j + 8 * c);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            // 32 dims a sum in the tensor core, whose accumulator truncates; the sums are added with rounding
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint4 k = *reinterpret_cast<const uint4*>(ring + (8 * u + g) * ROWB + key_piece(g, 4 * j + c) * 16);
+            mma_f16(d, ah.x, al.x, ah.y, al.y, k.x, k.y);
+            mma_f16(d, ah.z, al.z, ah.w, al.w, k.z, k.w);
+            z[2 * u] += d[0] + d[2];
+            z[2 * u + 1] += d[1] + d[3];
+          }
+        }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < HD / 32; ++j) {
-            const uint4 ah = *reinterpret_cast<const uint4*>(qh + g * QA + 32 * j + 8 * c);
-            const uint4 al = *reinterpret_cast<const uint4*>(qh + (g + 8) * QA + 32 * j + 8 * c);
-            mma_f16(d, ah.x, al.x, ah.y, al.y, kr[u][j].x, kr[u][j].y);
-            mma_f16(d, ah.z, al.z, ah.w, al.w, kr[u][j].z, kr[u][j].w);
-          }
-          s[2 * u] = 2 * c < nv[u] ? (d[0] + d[2]) * down : -INFINITY;
-          s[2 * u + 1] = 2 * c + 1 < nv[u] ? (d[1] + d[3]) * down : -INFINITY;
+          s[2 * u] = 2 * c < nv[u] ? z[2 * u] * down : -INFINITY;
+          s[2 * u + 1] = 2 * c + 1 < nv[u] ? z[2 * u + 1] * down : -INFINITY;
         }
-        if (HD > 128) load_v();  // 256: keys and values do not fit the registers together
-        const float base = st.raise(s);
+      } else {
+        const uint32_t* qt = reinterpret_cast<const uint32_t*>(qa);
+        float z0 = 0.f, z1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < HD / 16; ++j) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f}, dl[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint4 ah = *reinterpret_cast<const uint4*>(qt + g * QA + 16 * j + 4 * c);
+          const uint4 al = *reinterpret_cast<const uint4*>(qt + (g + 8) * QA + 16 * j + 4 * c);
+          const uint4 k = *reinterpret_cast<const uint4*>(ring + g * ROWB + key_piece(g, 4 * j + c) * 16);
+          uint32_t h[4], l[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tf32_pair(__uint_as_float(word(k, i)), h[i], l[i]);
+          mma_tf32(d, ah.x, al.x, ah.y, al.y, h[0], h[1]);
+          mma_tf32(dl, ah.x, al.x, ah.y, al.y, l[0], l[1]);
+          mma_tf32(d, ah.z, al.z, ah.w, al.w, h[2], h[3]);
+          mma_tf32(dl, ah.z, al.z, ah.w, al.w, l[2], l[3]);
+          z0 += d[0] + ((dl[0] + dl[2]) + d[2]);
+          z1 += d[1] + ((dl[1] + dl[3]) + d[3]);
+        }
+        s[0] = 2 * c < nv[0] ? z0 : -INFINITY;
+        s[1] = 2 * c + 1 < nv[0] ? z1 : -INFINITY;
+      }
+      __syncwarp();
+      if (more)
+        copy_rows(k_lane, ring, off_next, nv_next, true);
+      else
+        copies_commit();  // an empty group, so that the wait below counts the same
+      const float base = st.raise(s);
+      if constexpr (HALF) {
         uint32_t p_hi[2], p_lo[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -491,73 +642,71 @@ __global__ void __launch_bounds__(SP_THREADS) sparse_attn_kernel(SparseDev dv) {
           p_hi[u] = *reinterpret_cast<const uint32_t*>(&h);
           p_lo[u] = *reinterpret_cast<const uint32_t*>(&lo);
         }
+        copies_wait<1>();  // the values
+        __syncwarp();
 #pragma unroll
-        for (int j = 0; j < HD / 64; ++j)
+        for (int j = 0; j < HD / 64; ++j) {
+          uint4 v[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int r = 2 * c + (u & 1) + 8 * (u >> 1);
+            v[u] = *reinterpret_cast<const uint4*>(ring + HALF_RING + r * ROWB + value_piece(r, 8 * j + g) * 16);
+          }
 #pragma unroll
           for (int e = 0; e < 8; ++e) {  // column n of tile (j, e) is dim 64 j + 8 n + e
-            const uint32_t b0 = __byte_perm(word(vr[0][j], e / 2), word(vr[1][j], e / 2), e & 1 ? 0x7632 : 0x5410);
-            const uint32_t b1 = __byte_perm(word(vr[2][j], e / 2), word(vr[3][j], e / 2), e & 1 ? 0x7632 : 0x5410);
+            const uint32_t b0 = __byte_perm(word(v[0], e / 2), word(v[1], e / 2), e & 1 ? 0x7632 : 0x5410);
+            const uint32_t b1 = __byte_perm(word(v[2], e / 2), word(v[3], e / 2), e & 1 ? 0x7632 : 0x5410);
             mma_f16(st.acc[8 * j + e], p_hi[0], p_lo[0], p_hi[1], p_lo[1], b0, b1);
           }
-      }
-    } else {
-      const uint32_t* qt = reinterpret_cast<const uint32_t*>(qa);
-      for (int i0 = warp * 8; i0 < tokens; i0 += SP_WARPS * 8) {
-        long long off;
-        const int nv = locate(i0, off);
-        uint4 kr[HD / 16], vr[2][HD / 32];
-#pragma unroll
-        for (int j = 0; j < HD / 16; ++j)
-          kr[j] = g < nv ? ld_once(kb + off + g * row_bytes + 64 * j + 16 * c) : make_uint4(0, 0, 0, 0);
-        auto load_v = [&]() {
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int j = 0; j < HD / 32; ++j)
-              vr[u][j] = 2 * c + u < nv ? ld_once(vb + off + (2 * c + u) * row_bytes + 128 * j + 16 * g)
-                                        : make_uint4(0, 0, 0, 0);
-        };
-        if (HD <= 128) load_v();
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < HD / 16; ++j) {
-          const uint4 ah = *reinterpret_cast<const uint4*>(qt + g * QA + 16 * j + 4 * c);
-          const uint4 al = *reinterpret_cast<const uint4*>(qt + (g + 8) * QA + 16 * j + 4 * c);
-          uint32_t h[4], l[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) tf32_pair(__uint_as_float(word(kr[j], i)), h[i], l[i]);
-          mma_tf32(d, ah.x, al.x, ah.y, al.y, h[0], h[1]);
-          mma_tf32(d, ah.x, al.x, ah.y, al.y, l[0], l[1]);
-          mma_tf32(d, ah.z, al.z, ah.w, al.w, h[2], h[3]);
-          mma_tf32(d, ah.z, al.z, ah.w, al.w, l[2], l[3]);
         }
-        if (HD > 128) load_v();
-        float s[2];
-        s[0] = 2 * c < nv ? d[0] + d[2] : -INFINITY;
-        s[1] = 2 * c + 1 < nv ? d[1] + d[3] : -INFINITY;
-        const float base = st.raise(s);
+      } else {
         const float p0 = exp2f(s[0] - base), p1 = exp2f(s[1] - base);
         st.l += p0 + p1;
         uint32_t h0w, l0w, h1w, l1w;
         tf32_pair(p0, h0w, l0w);
         tf32_pair(p1, h1w, l1w);
+        copies_wait<1>();
+        __syncwarp();
 #pragma unroll
-        for (int j = 0; j < HD / 32; ++j)
+        for (int j = 0; j < HD / 32; ++j) {
+          uint4 v[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            v[u] = *reinterpret_cast<const uint4*>(ring + HALF_RING + (2 * c + u) * ROWB +
+                                                   value_piece(2 * c + u, 8 * j + g) * 16);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {  // column n of tile (j, e) is dim 32 j + 4 n + e
             uint32_t vh0, vl0, vh1, vl1;
-            tf32_pair(__uint_as_float(word(vr[0][j], e)), vh0, vl0);
-            tf32_pair(__uint_as_float(word(vr[1][j], e)), vh1, vl1);
+            tf32_pair(__uint_as_float(word(v[0], e)), vh0, vl0);
+            tf32_pair(__uint_as_float(word(v[1], e)), vh1, vl1);
             mma_tf32(st.acc[4 * j + e], h0w, l0w, h1w, l1w, vh0, vh1);
             mma_tf32(st.acc[4 * j + e], h0w, l0w, h1w, l1w, vl0, vl1);
           }
+        }
+      }
+      __syncwarp();
+      if (more)
+        copy_rows(v_lane, ring + HALF_RING, off_next, nv_next, false);
+      else
+        copies_commit();
+#pragma unroll
+      for (int u = 0; u < NB; ++u) {
+        off[u] = off_next[u];
+        nv[u] = nv_next[u];
       }
     }
+    copies_wait<0>();
+    __syncthreads();  // every warp is done with its buffer, where the outputs go now
     // ---- join: this CTA's warps ----
     st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
     st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
     if (c == 0) wm[warp][g] = st.m, wl[warp][g] = st.l;
-    constexpr int E = HALF ? 8 : 4;  // tiles whose column n is dims E n + e of a block of 8 E dims
+    // Outputs stay in accumulator order, 4 at a time: piece (slot, lane) with slot = (j, k, e / 4) is dims
+    // 8 E j + (2 c + k) E + e .. + 3 of head g (lane = 4 g + c), so that every access below is 16 bytes a lane in a row.
+    constexpr int E = HALF ? 8 : 4;  // column n of tile E j + e is dim 8 E j + E n + e
+    constexpr int PIECES = SP_HEADS * HD / 4;
+    float4* so4 = reinterpret_cast<float4*>(so);
+    float4* part4 = reinterpret_cast<float4*>(part);
 #pragma unroll
     for (int j = 0; j < HD / (8 * E); ++j)
 #pragma unroll
@@ -569,39 +718,65 @@ __global__ void __launch_bounds__(SP_THREADS) sparse_attn_kernel(SparseDev dv) {
           o.y = st.acc[E * j + e + 1][k] + st.acc[E * j + e + 1][k + 2];
           o.z = st.acc[E * j + e + 2][k] + st.acc[E * j + e + 2][k + 2];
           o.w = st.acc[E * j + e + 3][k] + st.acc[E * j + e + 3][k + 2];
-          *reinterpret_cast<float4*>(so + (warp * SP_HEADS + g) * HD + 8 * E * j + (2 * c + k) * E + e) = o;
+          so4[warp * PIECES + (((j * 2 + k) * (E / 4) + e / 4) * 32 + lane)] = o;
         }
+    auto store = [&](int i, float4 O, float L) {  // piece i of the result
+      const int h = (i & 31) >> 2;
+      if (h >= heads) return;
+      const int slot = i >> 5, j = slot / (2 * (E / 4)), k = slot / (E / 4) % 2, e = slot % (E / 4) * 4;
+      float* to = out + (size_t)(h0 + h) * HD + 8 * E * j + (2 * (i & 3) + k) * E + e;
+      const float d = L == 0.f ? 1.f : L;  // 0: none of the row's pages exists, and O is 0
+      O = make_float4(O.x / d, O.y / d, O.z / d, O.w / d);
+      if (wide)
+        *reinterpret_cast<float4*>(to) = O;
+      else
+        to[0] = O.x, to[1] = O.y, to[2] = O.z, to[3] = O.w;
+    };
     __syncthreads();
-    for (int i = tid; i < SP_HEADS * HD; i += SP_THREADS) {
-      const int h = i / HD;
+    for (int i = tid; i < PIECES; i += SP_THREADS) {
+      const int h = (i & 31) >> 2;
       float M = -INFINITY;
 #pragma unroll
       for (int w = 0; w < SP_WARPS; ++w) M = fmaxf(M, wm[w][h]);
       const float base = M == -INFINITY ? 0.f : M;  // no token: the factors are exp2(-inf) = 0, and a NaN stays one
-      float L = 0.f, O = 0.f;
+      float L = 0.f;
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < SP_WARPS; ++w) {
         const float f = exp2f(wm[w][h] - base);
+        const float4 o = so4[w * PIECES + i];
         L = fmaf(wl[w][h], f, L);
-        O = fmaf(so[w * SP_HEADS * HD + i], f, O);
+        O.x = fmaf(o.x, f, O.x), O.y = fmaf(o.y, f, O.y), O.z = fmaf(o.z, f, O.z), O.w = fmaf(o.w, f, O.w);
       }
-      part[i] = O;
-      if (i % HD == 0) pm[h] = M, pl[h] = L;
+      if (S == 1) {
+        store(i, O, L);
+      } else {
+        part4[i] = O;
+        if (i < 32 && (i & 3) == 0) pm[h] = M, pl[h] = L;
+      }
     }
+    if (S == 1) continue;
     // ---- and the cluster's CTAs, each of them a share of the outputs ----
     cluster.sync();
-    for (int i = rank * SP_THREADS + tid; i < heads * HD; i += S * SP_THREADS) {
-      const int h = i / HD;
+    for (int i = rank * SP_THREADS + tid; i < PIECES; i += S * SP_THREADS) {
+      const int h = (i & 31) >> 2;
+      if (h >= heads) continue;
       float M = -INFINITY;
-      for (int r = 0; r < S; ++r) M = fmaxf(M, cluster.map_shared_rank(pm, r)[h]);
+#pragma unroll
+      for (int r = 0; r < SP_CLUSTER; ++r)
+        if (r < S) M = fmaxf(M, cluster.map_shared_rank(pm, r)[h]);
       const float base = M == -INFINITY ? 0.f : M;
-      float L = 0.f, O = 0.f;
-      for (int r = 0; r < S; ++r) {
+      float L = 0.f;
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int r = 0; r < SP_CLUSTER; ++r) {
+        if (r >= S) break;
         const float f = exp2f(cluster.map_shared_rank(pm, r)[h] - base);
+        const float4 o = cluster.map_shared_rank(part4, r)[i];
         L = fmaf(cluster.map_shared_rank(pl, r)[h], f, L);
-        O = fmaf(cluster.map_shared_rank(part, r)[i], f, O);
+        O.x = fmaf(o.x, f, O.x), O.y = fmaf(o.y, f, O.y), O.z = fmaf(o.z, f, O.z), O.w = fmaf(o.w, f, O.w);
       }
-      out[(size_t)h0 * HD + i] = L == 0.f ? 0.f : O / L;  // 0: none of the row's pages exists
+      store(i, O, L);
     }
     cluster.sync();  // no CTA leaves, or writes its state again, while another reads it
   }
@@ -613,19 +788,22 @@ int launch(const SparseAttnArgs& a, cudaStream_t s) {
   d.a = a;
   d.cap_pages = (int)std::min<long long>(((long long)a.max_ctx + a.page_size - 1) / a.page_size, a.max_pages);
   const long long pairs = (long long)a.batch * a.hkv;
+  // CTAs per pair: as many as leave all of them resident, two an SM.  What a CTA does once whatever its share (query
+  // staging, threshold, joins: about 8 us) is then paid once in time; twice as many CTAs in two waves measured
+  // 113 us where one wave takes 97 (32 sequences of up to 32k tokens, 8 KV heads).
   int S = 1;
-  while (S < 8 && pairs * S < 4 * 148) S <<= 1;
-  size_t smem = 0;
-  for (;; S <<= 1) {  // more CTAs where one CTA's scores would not fit
-    const int scored = d.cap_pages > a.budget ? (d.cap_pages + S - 1) / S : 0;
-    d.key_words = (std::max(scored, SP_WARPS * SP_HEADS * HD) + 3) / 4 * 4;
-    d.share = (std::min(a.budget, d.cap_pages) + S - 1) / S;
-    smem = (size_t)d.key_words * 4 + SP_HEADS * HD * 4 + 16 * (2 * HD + 16) + 16 * (HALF ? (HD + 8) * 2 : (HD + 4) * 4) +
-           (size_t)d.share * 8;
-    if (smem <= SP_SMEM_MAX || S == 8) break;
-  }
+  while (S < SP_CLUSTER && pairs * S * 2 <= 2 * 148) S <<= 1;
+  d.key_words = d.cap_pages > a.budget ? (d.cap_pages + 3) / 4 * 4 : 0;
+  d.share = (std::min(a.budget, d.cap_pages) + S - 1) / S;
+  size_t smem = (size_t)SP_WARPS * 64 * HD + (size_t)d.key_words * 4 + SP_HEADS * HD * 4 + 16 * (2 * HD + 16) +
+                16 * (HALF ? (HD + 8) * 2 : (HD + 4) * 4) + (size_t)d.share * 8;
+  d.id_words = smem + (size_t)d.key_words * 4 <= SP_SMEM_MAX ? d.key_words : 0;
+  smem += (size_t)d.id_words * 4;
   if (smem > SP_SMEM_MAX || pairs * S > 0x7fffffffLL) return kTooLarge;
-  auto kernel = sparse_attn_kernel<HD, HALF>;
+  // One CTA an SM is left its registers: a single sequence of 8k tokens takes 13.3 us so, 16.3 us within 128 registers,
+  // which two CTAs an SM need.  Outputs of 256 dims leave room for one only.
+  const bool two = HD <= 128 && pairs * S > 148;
+  auto kernel = two ? sparse_attn_kernel<HD, HALF, HD <= 128 ? 2 : 1> : sparse_attn_kernel<HD, HALF, 1>;
   if (allow_smem(kernel, smem)) return kCudaError;
   return launch_cluster_pdl(kernel, dim3((unsigned)(pairs * S)), dim3(SP_THREADS), S, smem, s, d) == cudaSuccess
              ? kOk
