@@ -411,6 +411,19 @@ ZC_API int32_t zcu_sparse_paged_attention(const float* q, int64_t q_stride, cons
                                           int64_t head_stride, float scale, int32_t max_ctx, int32_t budget,
                                           int32_t sink, int32_t recent, void* stream);
 
+/* Low-rank adapters of many requests beside a shared projection (whose output is y; zcu_gemv_*, zcu_gemm_*):
+ *   out[r] = y[r] + scales[e] * (x[r] A_e^T) B_e^T,  e = adapter[r];  a row whose adapter is outside [0, adapters): y[r]
+ * x [rows][k_cols], y and out [rows][n_rows] fp32 with strides in elements; out may be y itself (no other overlap).
+ * a [adapters][rank][k_cols] and b [adapters][n_rows][rank] (w_dtype 0 = fp32, 1 = fp16, 2 = bf16); of adapter e the
+ * first ranks[e] of `rank` are used (NULL: all), scales NULL: 1.  fp32 arithmetic, or tf32 hi + lo pairs on the tensor
+ * cores for many rows (about 2^-22); a row's result does not depend on the other rows' adapters.
+ * rank a multiple of 8 up to 128, k_cols a multiple of 32 (else -4); x, a and b 16-byte aligned, x_stride a multiple
+ * of 4. */
+ZC_API int32_t zcu_lora_add(const float* x, int64_t x_stride, const float* y, int64_t y_stride, float* out,
+                            int64_t out_stride, const void* a, const void* b, int32_t w_dtype, const int32_t* adapter,
+                            const int32_t* ranks, const float* scales, int32_t rows, int32_t k_cols, int32_t n_rows,
+                            int32_t adapters, int32_t rank, void* stream);
+
 /* Per-request rules on logits [rows][vocab] (dtype 0 = fp32, 1 = fp16, 2 = bf16; strides in elements) before zcu_sample,
  * written as fp32 to out (which may be the logits themselves when these are fp32; no other overlap).  For token t of
  * row r, with `seen` whether t stands in the row's history and c how often it stands behind the prompt:

@@ -485,6 +485,109 @@ def test_sparse_attention_in_a_captured_graph():
 
 
 # ---------------------------------------------------------------------------------------------------------
+# adapters
+# ---------------------------------------------------------------------------------------------------------
+
+
+def lora_case(rng, rows, k, n, rank, adapters, w, run):
+    t = getattr(torch, w)
+    x = rng.standard_normal((rows, k)).astype(np.float32)
+    y = rng.standard_normal((rows, n)).astype(np.float32)
+    a = (torch.from_numpy(rng.standard_normal((adapters, rank, k)).astype(np.float32)) / k ** 0.5).to(t)
+    b = (torch.from_numpy(rng.standard_normal((adapters, n, rank)).astype(np.float32)) / rank ** 0.5).to(t)
+    adapter = rng.integers(-1, adapters + 1, -(-rows // run)).repeat(run)[:rows].astype(np.int32)
+    ranks = rng.integers(0, rank + 1, adapters).astype(np.int32)
+    ranks[0] = rank
+    scales = (rng.random(adapters) * 2 - 0.5).astype(np.float32)
+    return x, y, a, b, adapter, ranks, scales
+
+
+def plain_lora(x, y, a, b, adapter, ranks, scales):
+    """(result, size of the products added up), in 64 bits."""
+    out, mag = y.astype(np.float64), np.abs(y).astype(np.float64)
+    for e in range(len(ranks)):
+        at = adapter == e
+        r = ranks[e]
+        A, B = a[e, :r].double().numpy(), b[e, :, :r].double().numpy()
+        xe = x[at].astype(np.float64)
+        out[at] += float(scales[e]) * (xe @ A.T) @ B.T
+        mag[at] += abs(float(scales[e])) * (np.abs(xe) @ np.abs(A.T)) @ np.abs(B.T)
+    return out, mag
+
+
+@pytest.mark.parametrize("w", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("rows,k,n,rank,adapters,run", [
+    (1, 32, 1, 8, 1, 1), (1, 4096, 4096, 16, 2, 1), (3, 96, 77, 24, 2, 1), (64, 768, 2304, 64, 9, 1),
+    (17, 2048, 1001, 128, 4, 3), (200, 256, 300, 40, 30, 1), (257, 512, 255, 16, 5, 70), (300, 1024, 640, 64, 40, 1),
+    (1000, 768, 768, 8, 3, 333), (513, 4096, 515, 128, 3, 100), (2000, 160, 1030, 32, 7, 11)])
+def test_lora(rows, k, n, rank, adapters, run, w):
+    """Tolerance, relative to the products added up in each element: (k / 8 + 40) half ulps of fp32 for the two sums (at
+    most 8 products between two roundings of a partial sum, truncated in the tensor core, hence whole ulps: 2^-23), and
+    2^-21 for the pairs that hold x and t."""
+    rng = np.random.default_rng(rows * 3 + rank)
+    c = x, y, a, b, adapter, ranks, scales = lora_case(rng, rows, k, n, rank, adapters, w, run)
+    want, mag = plain_lora(*c)
+    tol = ((k / 8 + 40) * 2.0 ** -23 + 2.0 ** -21) * mag
+    d = dev(x), a.cuda(), b.cuda(), dev(adapter)
+    kw = dict(ranks=dev(ranks), scales=dev(scales))
+    out = ops.lora_add(dev(y), *d, out=torch.full((rows, n), 7.0, device="cuda"), **kw)
+    assert (np.abs(out.cpu().numpy() - want) <= tol).all()
+    # in place on a slice of a wider, misaligned activation, from a slice of one
+    wide = torch.full((rows, n + 5), 3.0, device="cuda")
+    wide[:, 1:1 + n] = dev(y)
+    xw = torch.zeros((rows, k + 8), device="cuda")
+    xw[:, 4:4 + k] = d[0]
+    ops.lora_add(wide[:, 1:1 + n], xw[:, 4:4 + k], *d[1:], **kw)
+    assert torch.equal(wide[:, 1:1 + n], out)
+    assert (wide[:, 0] == 3).all() and (wide[:, 1 + n:] == 3).all()
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+def test_lora_rows_do_not_meet(rows):
+    """NaN and infinities of one adapter, of an unused rank, and of one row's input stay where they are."""
+    rng = np.random.default_rng(21)
+    x, y, a, b, adapter, ranks, scales = lora_case(rng, rows, 64, 50, 16, 4, "float16", 1)
+    adapter[:] = np.arange(rows) % 4
+    adapter[4] = -1
+    ranks[:] = [16, 11, 3, 16]
+    for e in (1, 2):  # unused ranks of two adapters
+        a[e, ranks[e]:] = float("nan")
+        b[e, :, ranks[e]:] = float("inf")
+    a[3], x[0, 7] = float("nan"), np.inf
+    args = dev(x), a.cuda(), b.cuda(), dev(adapter)
+    out = ops.lora_add(dev(y), *args, ranks=dev(ranks), scales=dev(scales)).cpu().numpy()
+    bad = (adapter == 3) | (np.arange(rows) == 0)
+    assert np.isfinite(out[~bad]).all() and not np.isfinite(out[bad]).any()
+    keep = ~bad & (adapter >= 0)
+    a[3], x[0] = 0, 0
+    want, mag = plain_lora(x, y, a.nan_to_num(0), b.nan_to_num(0, 0, 0), adapter, ranks, scales)
+    assert (np.abs(out - want)[keep] <= 1e-5 * mag[keep]).all()
+    assert (out[4] == y[4]).all()
+
+
+def test_lora_same_rows_alone_and_in_a_batch():
+    """A row's bits do not depend on what shares the batch (same form of the kernel)."""
+    rng = np.random.default_rng(22)
+    x, y, a, b, adapter, ranks, scales = lora_case(rng, 100, 512, 700, 32, 6, "bfloat16", 1)
+    d = a.cuda(), b.cuda()
+    kw = dict(ranks=dev(ranks), scales=dev(scales))
+    out = ops.lora_add(dev(y), dev(x), *d, dev(adapter), **kw)
+    for r in (0, 41, 99):
+        one = ops.lora_add(dev(y[r:r + 1]), dev(x[r:r + 1]), *d, dev(adapter[r:r + 1]), **kw)
+        assert torch.equal(one[0], out[r])
+
+
+def test_lora_refuse():
+    y, x = torch.zeros((2, 40), device="cuda"), torch.zeros((2, 64), device="cuda")
+    a, b = torch.zeros((1, 8, 64), device="cuda"), torch.zeros((1, 40, 8), device="cuda")
+    ops.lora_add(y, x, a, b, ints([0, 0]))
+    for bad in ((y, x[:1], a, b), (y, x, a, b.half()), (y, x, a.double(), b.double()), (y, x, a, b[:, :39]),
+                (y.half(), x, a, b), (y.t(), x, a, b), (y, x, a.cpu(), b)):
+        with pytest.raises(ZcError):
+            ops.lora_add(*bad, ints([0, 0]))
+
+
+# ---------------------------------------------------------------------------------------------------------
 # logits rules
 # ---------------------------------------------------------------------------------------------------------
 

@@ -90,6 +90,25 @@ def test_sparse_attention_covers_three_head_sizes_and_pages_of_eights():
     assert sparse(batch=0) == 0
 
 
+def lora(x=P, xs=64, y=P, ys=40, out=P, os=40, a=P, b=P, w=1, adapter=P, ranks=None, scales=None, rows=2, k=64, n=40,
+         adapters=3, rank=8):
+    return _lib.lib().zcu_lora_add(x, xs, y, ys, out, os, a, b, w, adapter, ranks, scales, rows, k, n, adapters, rank,
+                                   None)
+
+
+@pytest.mark.parametrize("bad", [dict(x=None), dict(y=None), dict(out=None), dict(a=None), dict(b=None),
+                                 dict(adapter=None), dict(w=3), dict(w=-1), dict(rows=-1), dict(k=0), dict(n=0),
+                                 dict(adapters=0), dict(rank=0), dict(xs=63), dict(xs=66), dict(ys=39), dict(os=39),
+                                 dict(os=48), dict(x=P + 8), dict(a=P + 2), dict(b=P + 8)])
+def test_lora_refuses(bad):
+    assert lora(**bad) == -2
+
+
+def test_lora_covers_ranks_of_eights_to_128_and_columns_of_32():
+    assert lora(rank=12) == -4 and lora(rank=136) == -4 and lora(k=48, xs=48) == -4
+    assert lora(rows=0, x=None) == 0
+
+
 def logits(x=P, dtype=0, xs=64, out=P + 1024, os=64, rows=2, vocab=64, **rules):
     r = _lib.LogitsRules(**rules)
     return _lib.lib().zcu_process_logits(x, dtype, xs, out, os, rows, vocab, C.byref(r), None)

@@ -164,6 +164,7 @@ SIGNATURES.update({
                             vp]),
     "zcu_sparse_paged_attention": (i32, [vp, i64, vp, vp, i32, vp, vp, vp, i32, vp, vp, vp, vp] + [i32] * 7 +
                                    [i64, i64, i64, f32, i32, i32, i32, i32, vp]),
+    "zcu_lora_add": (i32, [vp, i64, vp, i64, vp, i64, vp, vp, i32, vp, vp, vp] + [i32] * 5 + [vp]),
     "zcu_process_logits": (i32, [vp, i32, i64, vp, i64, i32, i32, C.POINTER(LogitsRules), vp]),
 })
 

@@ -130,6 +130,31 @@ int32_t zcu_sparse_paged_attention(const float* q, int64_t q_stride, const void*
   return done(sparse_attention(a, as_stream(stream)), "zcu_sparse_paged_attention");
 }
 
+int32_t zcu_lora_add(const float* x, int64_t x_stride, const float* y, int64_t y_stride, float* out, int64_t out_stride,
+                     const void* a, const void* b, int32_t w_dtype, const int32_t* adapter, const int32_t* ranks,
+                     const float* scales, int32_t rows, int32_t k_cols, int32_t n_rows, int32_t adapters, int32_t rank,
+                     void* stream) {
+  LoraArgs p{};
+  p.x = x;
+  p.y = y;
+  p.out = out;
+  p.x_stride = x_stride;
+  p.y_stride = y_stride;
+  p.out_stride = out_stride;
+  p.a = a;
+  p.b = b;
+  p.w_type = w_dtype;
+  p.adapter = adapter;
+  p.ranks = ranks;
+  p.scales = scales;
+  p.rows = rows;
+  p.k = k_cols;
+  p.n = n_rows;
+  p.adapters = adapters;
+  p.rank = rank;
+  return done(lora_add(p, as_stream(stream)), "zcu_lora_add");
+}
+
 int32_t zcu_process_logits(const void* logits, int32_t dtype, int64_t logits_stride, float* out, int64_t out_stride,
                            int32_t rows, int32_t vocab, const zcu_logits_rules* r, void* stream) {
   if (!r) return done(kBadArgument, "zcu_process_logits");

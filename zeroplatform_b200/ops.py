@@ -7,7 +7,7 @@ Names and argument meaning follow the reference (kzxl/ZeroPlatform):
 * ``TensorBlas.gemv_q8_0 / gemv_q4_0`` -- ZeroTensor/src/ZeroTensor.Core/TensorBlas.Quantized.cs:447-485
   (host arrays in, host array out; goes through the reference bridge ABI ``zc_gemv_*``)
 * ``TensorOps.paged_attention`` -- ZeroTensor/src/ZeroTensor.Core/TensorOps.Neural.cs:2372-2476
-* ``reserve_pages``, ``trim_pages``, ``append_kv``, ``sparse_paged_attention``, ``process_logits`` --
+* ``reserve_pages``, ``trim_pages``, ``append_kv``, ``sparse_paged_attention``, ``lora_add``, ``process_logits`` --
   one step of a mixed serving batch, its state on the device (no counterpart in the reference, whose page tables,
   histories and sampling rules are per call on the host)
 * ``QuantizedWeight`` -- a weight uploaded once and kept in the device layout (the repack of the
@@ -399,6 +399,33 @@ def sparse_paged_attention(q, k_pool, v_pool, bounds, scales, page_table, ctx_le
           _arg("out", out, f, dev, (batch, hq, hd)), _arg("sel", sel, i, dev, (batch, hkv, budget)), batch, hq, hkv,
           hd, page, max_pages, pages, sp, ss, sh, scale, max_ctx, budget, sink, recent)
     return out, sel
+
+
+def lora_add(y, x, a, b, adapter, ranks=None, scales=None, out=None, stream=None):
+    """out[r] = y[r] + scales[e] * (x[r] a[e].T) b[e].T for e = adapter[r] (rows with an adapter outside the tensor: y[r]):
+    each request's low-rank adapter beside a shared projection's output y (zcu_lora_add).
+
+    x [rows, k], y [rows, n] fp32 (any row stride), a [adapters, rank, k], b [adapters, n, rank] fp32, fp16 or bf16,
+    adapter [rows] int32; ranks [adapters] int32 for adapters that use fewer than rank, scales [adapters] fp32.  out
+    defaults to y, in place."""
+    dev = _cuda("y", y)
+    if out is None:
+        out = y
+    if y.dim() != 2 or x.dim() != 2 or a.dim() != 3 or b.dim() != 3:
+        raise ZcError("x and y must be matrices, a and b stacks of matrices")
+    rows, n = y.shape
+    na, rank, k = a.shape
+    for name, t, shape in (("x", x, (rows, k)), ("y", y, (rows, n)), ("out", out, (rows, n))):
+        if t.shape != shape or t.dtype is not torch.float32 or t.device != dev or (t.numel() and t.stride(1) != 1):
+            raise ZcError(f"{name} must be {list(shape)} fp32 on {dev} with contiguous rows")
+    if a.dtype not in _FLOAT_CODE:
+        raise ZcError("a and b must be fp32, fp16 or bf16")
+    i, f = torch.int32, torch.float32
+    _call(lib().zcu_lora_add, "lora_add", dev, stream, x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0),
+          out.data_ptr(), out.stride(0), _arg("a", a, a.dtype, dev), _arg("b", b, a.dtype, dev, (na, n, rank)),
+          _FLOAT_CODE[a.dtype], _arg("adapter", adapter, i, dev, (rows,)), _arg("ranks", ranks, i, dev, (na,)),
+          _arg("scales", scales, f, dev, (na,)), rows, k, n, na, rank)
+    return out
 
 
 def process_logits(logits, out=None, past=None, past_len=None, prompt_len=None, past_rows=None, repetition=None,
