@@ -12,9 +12,10 @@
 //   B is read by rank / 8 lanes, and the first rows of B are on their way before the cluster has summed t.  Bound: the
 //   adapters' bytes (each row reads its own; rows that share an adapter meet in L2), at small sizes the chain
 //   A -> t -> B of one launch.
-// lora_tile_kernel (many rows, as in prefill): 64 rows per cluster on the tensor cores, mma m16n8k8 with x, t (and fp32
-//   weights) as tf32 hi + lo pairs, which hold fp32 to 2^-22 and any range; 16-bit weights are exact in tf32.  A warp
-//   takes its 16 rows one adapter at a time, usually one.  Bound: x, y and out once, or the tensor pipe at large ranks.
+// lora_tile_kernel (many rows, as in prefill): 64 rows per cluster on the tensor cores (mma.sync), x and t split into
+//   terms of the weights' type that hold fp32 to 2^-22 (Step).  x and A, then y and
+//   B, pass through one cp.async ring, whose second filling starts before the cluster has summed t.  The adapter that most of a tile's rows name is staged; warps whose rows name others fetch those weights themselves.  Bound: x, y and out once
+//   through HBM, or the tensor pipe at large ranks.
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -36,11 +37,6 @@ constexpr int LR_WARPS = LR_THREADS / 32;
 constexpr int LR_CLUSTER = 8;
 constexpr int LR_MAX_RANK = 128;
 
-// Eight weights as floats; p is 16-byte aligned.
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
 template <typename W>
 struct Raw;  // eight weights as they lie in memory
 template <>
@@ -239,11 +235,24 @@ __global__ void __launch_bounds__(LR_THREADS) lora_row_kernel(LoraArgs a) {
 
 // ---- tiles of 64 rows ----
 
-constexpr int LT_ROWS = 64;
+constexpr int LT_ROWS = 64, LT_K = 64, LT_STAGES = 3;
+constexpr int LT_XROW = LT_K * 4 + 16;  // bytes of a staged row of x: 16 more put an access's two rows on other banks
 
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -252,215 +261,490 @@ __device__ __forceinline__ uint32_t tf32_of(float v) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
   return r;
 }
+// 16 bytes from memory into shared memory, zeros where !ok (nothing is read then)
+__device__ __forceinline__ void copy16(void* dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+               "r"(ok ? 16 : 0)
+               : "memory");
+}
 
-// The A operand of a 16-row, 32-deep step: lane (g, c) gives elements 8 c .. 8 c + 7 of rows g and g + 8; k-step s takes
-// elements 2 s and 2 s + 1 of each lane.  The B operand's lane (g, c) gives the same elements of column g.
-struct Step {
-  uint32_t hi[4][4], lo[4][4];
-};
-__device__ __forceinline__ void split_step(const float (&r0)[8], const float (&r1)[8], Step& s) {
+// A 16-row, 32-deep step of a product with fp32 rows.  Lane (g, c) holds elements 8 c .. 8 c + 7 of rows g and g + 8 and
+// the same elements of weight row (column) g: the contraction index is permuted alike on both sides.  The rows are
+// split into terms of the weights' type that hold them to at least 2^-22:
+//   fp16   hi + lo, with a power of two of the row's own that keeps it in range;  2 terms, k-steps of 16
+//   bf16   three terms, in fp32's range;                                          3 terms, k-steps of 16
+//   fp32   tf32 hi + lo of both sides, lo x lo left out;                          3 products, k-steps of 8
+// (a k-step of either kind takes the tensor cores the same time: 540 TFLOP/s at k 16, 270 at k 8).
+template <typename W>
+struct Step;
+template <>
+struct Step<__half> {
+  static constexpr bool SCALED = true;
+  uint32_t hi[2][4], lo[2][4];
+  __device__ __forceinline__ void split(const float (&r0)[8], const float (&r1)[8]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float v[4] = {r0[2 * i], r1[2 * i], r0[2 * i + 1], r1[2 * i + 1]};
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      s.hi[i][q] = tf32_of(v[q]);
-      s.lo[i][q] = tf32_of(v[q] - __uint_as_float(s.hi[i][q]));
+      for (int q = 0; q < 4; ++q) {  // row g or g + 8, elements 4 i + (0, 1) or (2, 3)
+        const float(&r)[8] = q & 1 ? r1 : r0;
+        const float u = r[4 * i + (q >> 1) * 2], v = r[4 * i + (q >> 1) * 2 + 1];
+        const __half2 h = __floats2half2_rn(u, v);
+        const float2 f = __half22float2(h);
+        const __half2 l = __floats2half2_rn(u - f.x, v - f.y);
+        hi[i][q] = *reinterpret_cast<const uint32_t*>(&h);
+        lo[i][q] = *reinterpret_cast<const uint32_t*>(&l);
+      }
+  }
+  __device__ __forceinline__ void mma(float (&d)[4], const Raw<__half>& w) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mma_f16(d, lo[i], word_of(w.a, 2 * i), word_of(w.a, 2 * i + 1));
+      mma_f16(d, hi[i], word_of(w.a, 2 * i), word_of(w.a, 2 * i + 1));
     }
   }
+};
+template <>
+struct Step<__nv_bfloat16> {
+  static constexpr bool SCALED = false;
+  uint32_t t[3][2][4];
+  __device__ __forceinline__ void split(const float (&r0)[8], const float (&r1)[8]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float(&r)[8] = q & 1 ? r1 : r0;
+        float u = r[4 * i + (q >> 1) * 2], v = r[4 * i + (q >> 1) * 2 + 1];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(u, v);
+          t[k][i][q] = *reinterpret_cast<const uint32_t*>(&h);
+          u -= __uint_as_float(t[k][i][q] << 16);
+          v -= __uint_as_float(t[k][i][q] & 0xffff0000u);
+        }
+      }
+  }
+  __device__ __forceinline__ void mma(float (&d)[4], const Raw<__nv_bfloat16>& w) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 2; k >= 0; --k) mma_bf16(d, t[k][i], word_of(w.a, 2 * i), word_of(w.a, 2 * i + 1));
+  }
+};
+template <>
+struct Step<float> {
+  static constexpr bool SCALED = false;
+  uint32_t hi[4][4], lo[4][4];
+  __device__ __forceinline__ void split(const float (&r0)[8], const float (&r1)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float v[4] = {r0[2 * i], r1[2 * i], r0[2 * i + 1], r1[2 * i + 1]};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        hi[i][q] = tf32_of(v[q]);
+        lo[i][q] = tf32_of(v[q] - __uint_as_float(hi[i][q]));
+      }
+    }
+  }
+  __device__ __forceinline__ void mma(float (&d)[4], const Raw<float>& w) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 p = pair_of(w, i);
+      const uint32_t h0 = tf32_of(p.x), h1 = tf32_of(p.y);
+      mma_tf32(d, hi[i], tf32_of(p.x - __uint_as_float(h0)), tf32_of(p.y - __uint_as_float(h1)));
+      mma_tf32(d, lo[i], h0, h1);
+      mma_tf32(d, hi[i], h0, h1);
+    }
+  }
+};
+
+__device__ __forceinline__ float top8(const float (&v)[8]) {
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t = fmaxf(t, fabsf(v[i]));
+  return t;
+}
+__device__ __forceinline__ float top_quad(float t) {
+  t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+  return fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+}
+// The power of two that brings `top` to 2^6 .. 2^7 (fp16 holds up to 2^16 and 2^-24): 1 for 0 and what is not finite.
+__device__ __forceinline__ float scale_for(float top) {
+  if (!(top > 0.f && top < INFINITY)) return 1.f;
+  const int e = (int)((__float_as_uint(top) >> 23) & 255u) - 127;
+  return __uint_as_float((uint32_t)(127 + min(max(6 - e, -126), 126)) << 23);
+}
+__device__ __forceinline__ void times(float (&v)[8], float f) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] *= f;
+}
+__device__ __forceinline__ void load_row8(const float* p, float (&v)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+__device__ __forceinline__ void load_raw(const unsigned char* p, Raw<float>& r) {
+  r.a = *reinterpret_cast<const float4*>(p);
+  r.b = *reinterpret_cast<const float4*>(p + 16);
 }
 template <typename W>
-__device__ __forceinline__ void step_mma(float (&d)[4], const Step& s, const Raw<W>& w) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 p = pair_of(w, i);
-    if constexpr (sizeof(W) == 4) {
-      const uint32_t h0 = tf32_of(p.x), h1 = tf32_of(p.y);
-      mma_tf32(d, s.hi[i], tf32_of(p.x - __uint_as_float(h0)), tf32_of(p.y - __uint_as_float(h1)));
-      mma_tf32(d, s.lo[i], h0, h1);
-      mma_tf32(d, s.hi[i], h0, h1);
-    } else {
-      mma_tf32(d, s.lo[i], __float_as_uint(p.x), __float_as_uint(p.y));
-      mma_tf32(d, s.hi[i], __float_as_uint(p.x), __float_as_uint(p.y));
-    }
-  }
+__device__ __forceinline__ void load_raw(const unsigned char* p, Raw<W>& r) {
+  r.a = *reinterpret_cast<const uint4*>(p);
 }
 
-// NT: column tiles of 8 ranks, 8 NT >= rank.
+// 4 bytes likewise, for rows that do not start on 16
+__device__ __forceinline__ void copy4(void* dst, const void* src, bool ok) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+               "r"(ok ? 4 : 0)
+               : "memory");
+}
+
+// Shared memory of a tile: a ring of stages, then this CTA's part of t.  A stage is 64 columns of x and of A, or of y and
+// of B's rows.  NT: column tiles of 8 ranks, 8 NT >= rank.  Rows are padded so that operand reads (row g, piece c)
+// spread over all banks.
+template <typename W, int NT>
+struct Tile {
+  static constexpr int TS = 8 * NT + 4;                                                // floats of a row of t
+  static constexpr int AROW = LT_K * (int)sizeof(W) + (sizeof(W) == 4 ? 16 : 64);      // bytes of a staged row of A
+  static constexpr int BROW = 8 * NT * (int)sizeof(W) + (sizeof(W) == 4 ? 16 : NT >= 8 ? 64 : 0);  // and of B
+  static constexpr int WBYTES = 8 * NT * AROW > LT_K * BROW ? 8 * NT * AROW : LT_K * BROW;
+  static constexpr int STAGE = LT_ROWS * LT_XROW + WBYTES;
+  static constexpr int BYTES = LT_STAGES * STAGE + LT_ROWS * TS * 4;
+  static_assert(LT_ROWS * TS * 4 <= STAGE, "t takes the last stage's place");
+};
+
 template <typename W, int NT>
 __global__ void __launch_bounds__(LR_THREADS) lora_tile_kernel(LoraArgs a) {
-  constexpr int TS = 8 * NT + 4;  // floats of a row of t
-  constexpr int STEPS = (8 * NT + 31) / 32;
-  extern __shared__ __align__(16) float sm[];
-  float* part = sm;                        // [2][LT_ROWS][TS]: the two k halves' sums, then [0] all of this CTA's
-  float* t = sm + 2 * LT_ROWS * TS;        // [LT_ROWS][TS]
+  using T = Tile<W, NT>;
+  constexpr int TS = T::TS, STEPS = (8 * NT + 31) / 32, EPP = 16 / (int)sizeof(W);  // weights of a 16-byte piece
+  extern __shared__ __align__(16) unsigned char smem[];
+  float* t = reinterpret_cast<float*>(smem + (LT_STAGES - 1) * T::STAGE);  // [LT_ROWS][TS]
+  float* part = reinterpret_cast<float*>(smem + LT_STAGES * T::STAGE);     // [LT_ROWS][TS]: this CTA's part of k
+  __shared__ int ids[LT_ROWS];
+  __shared__ int s_main;
   pdl_trigger();
   pdl_wait();
   cg::cluster_group cluster = cg::this_cluster();
   const int cr = cluster.block_rank(), C = cluster.num_blocks();
   const int row0 = (int)(blockIdx.x / C) * LT_ROWS, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, c = lane & 3;
-  const int mt = warp & 3, half = warp >> 2;  // 16 rows, and a half of k or n
-  const int ra = row0 + mt * 16 + g, rb = ra + 8;
-  const int ida = adapter_of(a, ra), idb = adapter_of(a, rb);
-  for (int i = tid; i < 2 * LT_ROWS * TS; i += LR_THREADS) part[i] = 0.f;
+  const int mt = warp & 3, half = warp >> 2;  // 16 rows, and a half of every 64 k or of the columns
+  if (tid < LT_ROWS) ids[tid] = adapter_of(a, row0 + tid);
+  if (tid == 0) s_main = 0;
   __syncthreads();
+  if (tid < LT_ROWS && ids[tid] >= 0) {  // the adapter that most rows name, the lowest row among equals
+    int same = 0;
+#pragma unroll 8
+    for (int i = 0; i < LT_ROWS; ++i) same += ids[i] == ids[tid];
+    atomicMax(&s_main, same * LT_ROWS + (LT_ROWS - 1 - tid));
+  }
+  __syncthreads();
+  // Its weights are staged with the rows; a warp whose rows name others fetches those weights itself.
+  const int main_ad = s_main ? ids[LT_ROWS - 1 - s_main % LT_ROWS] : -1;
+  const int main_rank = main_ad >= 0 ? rank_of(a, main_ad) : 0;
+  const int la = mt * 16 + g, lb = la + 8, ra = row0 + la, rb = row0 + lb;
+  const int ida = ids[la], idb = ids[lb];
+  const unsigned low_id = __reduce_min_sync(0xffffffffu, min((unsigned)ida, (unsigned)idb));  // -1 is the highest
+  const int high_id = __reduce_max_sync(0xffffffffu, max(ida, idb));
+  const bool none = high_id < 0;                    // no row of this warp has an adapter
+  const bool alone = (unsigned)high_id == low_id;   // or they all have the same one (rows without may be among them)
+  // Calls f(adapter, whether row g has it, whether row g + 8 has it) for each adapter of the warp's rows.
+  auto each = [&](auto f) {
+    if (none) return;
+    if (alone) return f((int)low_id, ida >= 0, idb >= 0);
+    unsigned after = low_id;
+    for (;;) {
+      f((int)after, ida == (int)after, idb == (int)after);
+      const unsigned na = ida >= 0 && (unsigned)ida > after ? (unsigned)ida : 0xffffffffu;
+      const unsigned nb = idb >= 0 && (unsigned)idb > after ? (unsigned)idb : 0xffffffffu;
+      after = __reduce_min_sync(0xffffffffu, min(na, nb));
+      if (after == 0xffffffffu) break;
+    }
+  };
 
-  // ---- t = x A^T ----
-  {
-    const int steps = a.k / 32, u0 = (int)((long long)steps * (2 * cr + half) / (2 * C)),
-              u1 = (int)((long long)steps * (2 * cr + half + 1) / (2 * C));
-    unsigned todo_a = ida >= 0, todo_b = idb >= 0;
-    for (;;) {  // one adapter of the 16 rows at a time
-      const unsigned ad = __reduce_min_sync(0xffffffffu, min(todo_a ? (unsigned)ida : 0xffffffffu,
-                                                             todo_b ? (unsigned)idb : 0xffffffffu));
-      if (ad == 0xffffffffu) break;
-      const bool ma = todo_a && ida == (int)ad, mb = todo_b && idb == (int)ad;
-      if (ma) todo_a = 0;
-      if (mb) todo_b = 0;
-      const int R = rank_of(a, (int)ad), tiles = (R + 7) / 8;
-      const W* A = reinterpret_cast<const W*>(a.a) + (size_t)ad * a.rank * a.k + 8 * c;
-      const float* xa = a.x + (size_t)ra * a.x_stride + 8 * c;
-      const float* xb = a.x + (size_t)rb * a.x_stride + 8 * c;
-      float acc[NT][4];
+  // ---- t = x A^T: the cluster's CTAs take 64 columns in turn, so that they read a row's neighbouring pieces together ----
+  const int chunks = (a.k + LT_K - 1) / LT_K, turns = (chunks - cr + C - 1) / C;
+  auto issue = [&](int q) {
+    if (q < turns) {
+      unsigned char* st = smem + q % LT_STAGES * T::STAGE;
+      const int k0 = (q * C + cr) * LT_K;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-      for (int u = u0; u < u1; ++u) {
-        float va[8] = {}, vb[8] = {};
-        if (ma) load8(xa + 32 * u, va);
-        if (mb) load8(xb + 32 * u, vb);
-        Raw<W> w[NT];
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          if (8 * i + g < R)
-            fetch(A + (size_t)(8 * i + g) * a.k + 32 * u, w[i]);
-          else
-            clear(w[i]);
-        }
-        Step s;
-        split_step(va, vb, s);
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-          if (i < tiles) step_mma<W>(acc[i], s, w[i]);
+      for (int i = 0; i < LT_ROWS * 16 / LR_THREADS; ++i) {
+        const int r = (i * LR_THREADS + tid) / 16, piece = (i * LR_THREADS + tid) % 16, k = k0 + piece * 4;
+        const bool ok = ids[r] >= 0 && k < a.k;
+        copy16(st + r * LT_XROW + piece * 16, a.x + (ok ? (size_t)(row0 + r) * a.x_stride + k : 0), ok);
       }
-      float* pa = part + (half * LT_ROWS + mt * 16 + g) * TS;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        if (ma) *reinterpret_cast<float2*>(pa + 8 * i + 2 * c) = make_float2(acc[i][0], acc[i][1]);
-        if (mb) *reinterpret_cast<float2*>(pa + 8 * TS + 8 * i + 2 * c) = make_float2(acc[i][2], acc[i][3]);
+      unsigned char* wt = st + LT_ROWS * LT_XROW;
+      const W* A = reinterpret_cast<const W*>(a.a) + (size_t)max(main_ad, 0) * a.rank * a.k;
+      for (int i = tid; i < (main_rank + 7) / 8 * 8 * (LT_K / EPP); i += LR_THREADS) {
+        const int r = i / (LT_K / EPP), piece = i % (LT_K / EPP), k = k0 + piece * EPP;
+        const bool ok = r < main_rank && k < a.k;
+        copy16(wt + r * T::AROW + piece * 16, A + (ok ? (size_t)r * a.k + k : 0), ok);
       }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  {
+    float acc[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+    float sa = 0.f, sb = 0.f;  // 0: not chosen yet
+    issue(0);
+    issue(1);
+    for (int q = 0; q < turns; ++q) {
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      __syncthreads();
+      issue(q + 2);
+      if (none) continue;
+      const unsigned char* st = smem + q % LT_STAGES * T::STAGE;
+      float va[8], vb[8];
+      load_row8(reinterpret_cast<const float*>(st + la * LT_XROW) + half * 32 + 8 * c, va);
+      load_row8(reinterpret_cast<const float*>(st + lb * LT_XROW) + half * 32 + 8 * c, vb);
+      if constexpr (Step<W>::SCALED) {
+        // The rows' powers of two come from their first 32 elements that are not all 0, with room for 2^8 times as
+        // much; where more comes, the sums so far follow.
+        float ta = top8(va), tb = top8(vb);
+        const bool low = (sa == 0.f && ta > 0.f) || (sb == 0.f && tb > 0.f);
+        const bool high = (ta * sa > 32768.f && ta < INFINITY) || (tb * sb > 32768.f && tb < INFINITY);
+        if (__any_sync(0xffffffffu, low || high)) {
+          ta = top_quad(ta);
+          tb = top_quad(tb);
+          auto follow = [&](float& s, float top, int k) {
+            if ((s == 0.f && top > 0.f) || (top * s > 32768.f && top < INFINITY)) {
+              const float n = scale_for(top);
+              if (s != 0.f)
+#pragma unroll
+                for (int i = 0; i < NT; ++i) acc[i][k] *= n / s, acc[i][k + 1] *= n / s;
+              s = n;
+            }
+          };
+          follow(sa, ta, 0);
+          follow(sb, tb, 2);
+        }
+        times(va, sa);
+        times(vb, sb);
+      }
+      Step<W> s;
+      s.split(va, vb);
+      if (alone && (int)low_id == main_ad) {
+        const unsigned char* wt = st + LT_ROWS * LT_XROW + g * T::AROW + (half * 32 + 8 * c) * (int)sizeof(W);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+          if (8 * i < main_rank) {
+            Raw<W> w;
+            load_raw(wt + i * 8 * T::AROW, w);
+            s.mma(acc[i], w);
+          }
+      } else {
+        const int k = (q * C + cr) * LT_K + half * 32 + 8 * c;
+        each([&](int ad, bool ma, bool mb) {
+          const int R = rank_of(a, ad);
+          const W* A = reinterpret_cast<const W*>(a.a) + ((size_t)ad * a.rank + g) * a.k + k;
+          Raw<W> w[NT];  // all on their way before the first is used
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            if (8 * i + g < R && k < a.k)
+              fetch(A + (size_t)8 * i * a.k, w[i]);
+            else
+              clear(w[i]);
+          }
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+            if (8 * i < R) {
+              // a sum of its own: what this adapter holds reaches its own rows only
+              float d[4] = {0.f, 0.f, 0.f, 0.f};
+              s.mma(d, w[i]);
+              if (ma) acc[i][0] += d[0], acc[i][1] += d[1];
+              if (mb) acc[i][2] += d[2], acc[i][3] += d[3];
+            }
+        });
+      }
+    }
+    // the two halves of each 64, in turn
+    const float ia = Step<W>::SCALED && sa != 0.f ? 1.f / sa : 1.f, ib = Step<W>::SCALED && sb != 0.f ? 1.f / sb : 1.f;
+#pragma unroll
+    for (int h = 1; h >= 0; --h) {
+      if (half == h) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          float2* pa = reinterpret_cast<float2*>(part + la * TS + 8 * i + 2 * c);
+          float2* pb = reinterpret_cast<float2*>(part + lb * TS + 8 * i + 2 * c);
+          float2 u = make_float2(acc[i][0] * ia, acc[i][1] * ia), v = make_float2(acc[i][2] * ib, acc[i][3] * ib);
+          if (h == 0) u.x += pa->x, u.y += pa->y, v.x += pb->x, v.y += pb->y;
+          *pa = u;
+          *pb = v;
+        }
+      }
+      __syncthreads();
+    }
   }
+
+  // ---- out = y + t B^T: 64 columns in turn ----
+  const int pieces64 = (a.n + 63) / 64, passes = (pieces64 - cr + C - 1) / C;
+  const bool y16 = (uintptr_t)a.y % 16 == 0 && a.y_stride % 4 == 0;
+  const bool out8 = (uintptr_t)a.out % 8 == 0 && a.out_stride % 2 == 0;
+  const bool move = a.out != a.y;  // rows without an adapter are copied
+  auto issue_cols = [&](int p) {
+    if (p < passes) {
+      unsigned char* st = smem + p % LT_STAGES * T::STAGE;
+      const int n0 = (p * C + cr) * 64;
+#pragma unroll
+      for (int i = 0; i < LT_ROWS * 16 / LR_THREADS; ++i) {
+        const int r = (i * LR_THREADS + tid) / 16, piece = (i * LR_THREADS + tid) % 16, n = n0 + piece * 4;
+        const bool ok = row0 + r < a.rows && (ids[r] >= 0 || move);
+        const float* from = a.y + (ok ? (size_t)(row0 + r) * a.y_stride : 0);
+        unsigned char* to = st + r * LT_XROW + piece * 16;
+        if (y16 && n + 4 <= a.n) {
+          copy16(to, from + n, ok);
+        } else {
+          for (int k = 0; k < 4; ++k) copy4(to + 4 * k, from + (n + k < a.n ? n + k : 0), ok && n + k < a.n);
+        }
+      }
+      unsigned char* wt = st + LT_ROWS * LT_XROW;
+      const int pieces = (main_rank + EPP - 1) / EPP;
+      const W* B = reinterpret_cast<const W*>(a.b) + (size_t)max(main_ad, 0) * a.n * a.rank;
+      for (int i = tid; i < 64 * pieces; i += LR_THREADS) {
+        const int r = i / pieces, piece = i - r * pieces, n = n0 + r;
+        copy16(wt + r * T::BROW + piece * 16, B + (n < a.n ? (size_t)n * a.rank + piece * EPP : 0), n < a.n);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  issue_cols(0);  // while the cluster sums t, whose place is the last stage
+  issue_cols(1);
   cluster.sync();
-  // ---- every CTA sums a part of t over the cluster and gives it to the others ----
+  // every CTA sums a part of t over the cluster and gives it to the others
   for (int i = cr * LR_THREADS + tid; i < LT_ROWS * 2 * NT; i += C * LR_THREADS) {  // 4 ranks of a row
     const int r = i / (2 * NT), j = i % (2 * NT) * 4;
-    float4 v[LR_CLUSTER][2];
+    float4 v[LR_CLUSTER];
 #pragma unroll
     for (int q = 0; q < LR_CLUSTER; ++q)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        v[q][h] = q < C ? *reinterpret_cast<const float4*>(cluster.map_shared_rank(part, q) + (h * LT_ROWS + r) * TS + j)
-                        : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[q] = q < C ? *reinterpret_cast<const float4*>(cluster.map_shared_rank(part, q) + r * TS + j)
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int q = 0; q < LR_CLUSTER; ++q)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) s.x += v[q][h].x, s.y += v[q][h].y, s.z += v[q][h].z, s.w += v[q][h].w;
-    const int ad = adapter_of(a, row0 + r);
+    for (int q = 0; q < LR_CLUSTER; ++q) s.x += v[q].x, s.y += v[q].y, s.z += v[q].z, s.w += v[q].w;
+    const int ad = ids[r];
     if (ad >= 0) {
       const int R = rank_of(a, ad);
       const float f = a.scales ? a.scales[ad] : 1.f;
       s.x = j < R ? s.x * f : 0.f, s.y = j + 1 < R ? s.y * f : 0.f;
       s.z = j + 2 < R ? s.z * f : 0.f, s.w = j + 3 < R ? s.w * f : 0.f;
     }
-    for (int q = 0; q < C; ++q) *reinterpret_cast<float4*>(cluster.map_shared_rank(t, q) + r * TS + j) = s;
+#pragma unroll
+    for (int q = 0; q < LR_CLUSTER; ++q)
+      if (q < C) *reinterpret_cast<float4*>(cluster.map_shared_rank(t, q) + r * TS + j) = s;
   }
   cluster.sync();
 
-  // ---- out = y + t B^T ----
-  const int tiles = (a.n + 7) / 8, t0 = (int)((long long)tiles * (2 * cr + half) / (2 * C)),
-            t1 = (int)((long long)tiles * (2 * cr + half + 1) / (2 * C));
-  const float* ya = a.y + (size_t)ra * a.y_stride;
-  const float* yb = a.y + (size_t)rb * a.y_stride;
-  float* oa = a.out + (size_t)ra * a.out_stride;
-  float* ob = a.out + (size_t)rb * a.out_stride;
-  auto add = [&](const float* y, float* o, int n, float d0, float d1) {
-    if (n < a.n) o[n] = y[n] + d0;
-    if (n + 1 < a.n) o[n + 1] = y[n + 1] + d1;
-  };
-  // both row starts on 8 bytes: two columns an access
-  const bool wide = ((uintptr_t)a.y | (uintptr_t)a.out) % 8 == 0 && a.y_stride % 2 == 0 && a.out_stride % 2 == 0;
-  unsigned todo_a = ida >= 0, todo_b = idb >= 0;
-  for (;;) {
-    const unsigned ad = __reduce_min_sync(0xffffffffu, min(todo_a ? (unsigned)ida : 0xffffffffu,
-                                                           todo_b ? (unsigned)idb : 0xffffffffu));
-    if (ad == 0xffffffffu) break;
-    const bool ma = todo_a && ida == (int)ad, mb = todo_b && idb == (int)ad;
-    if (ma) todo_a = 0;
-    if (mb) todo_b = 0;
-    const int R = rank_of(a, (int)ad);
-    const W* B = reinterpret_cast<const W*>(a.b) + (size_t)ad * a.n * a.rank + 8 * c;
-    Step s[STEPS];
+  // this warp's rows of t, as operands: each row belongs to one pass only
+  Step<W> s[STEPS];
+  float ia = 1.f, ib = 1.f;
+  {
+    float va[STEPS][8], vb[STEPS][8], ta = 0.f, tb = 0.f;
 #pragma unroll
     for (int q = 0; q < STEPS; ++q) {
-      float va[8] = {}, vb[8] = {};
-      const float* p = t + (mt * 16 + g) * TS + 32 * q + 8 * c;
-      if (32 * q + 8 * c < 8 * NT) {
-        if (ma)
-          for (int i = 0; i < 8; ++i) va[i] = p[i];
-        if (mb)
-          for (int i = 0; i < 8; ++i) vb[i] = p[8 * TS + i];
-      }
-      split_step(va, vb, s[q]);
-    }
-    constexpr int COLS = 4;  // column tiles in flight
-    for (int i0 = t0; i0 < t1; i0 += COLS) {
-      Raw<W> w[COLS][STEPS];
-      float2 y0[COLS], y1[COLS];
+      const float* p = t + la * TS + 32 * q + 8 * c;
 #pragma unroll
-      for (int i = 0; i < COLS; ++i) {
-        const int n = 8 * (i0 + i) + g, col = 8 * (i0 + i) + 2 * c;
-        const bool in = i0 + i < t1;
+      for (int i = 0; i < 8; ++i) va[q][i] = vb[q][i] = 0.f;
+      if (32 * q + 8 * c < 8 * NT) {
+        load_row8(p, va[q]);
+        load_row8(p + 8 * TS, vb[q]);
+      }
+      ta = fmaxf(ta, top8(va[q]));
+      tb = fmaxf(tb, top8(vb[q]));
+    }
+    if constexpr (Step<W>::SCALED) {
+      const float fa = scale_for(top_quad(ta)), fb = scale_for(top_quad(tb));
+      ia = 1.f / fa;
+      ib = 1.f / fb;
+#pragma unroll
+      for (int q = 0; q < STEPS; ++q) times(va[q], fa), times(vb[q], fb);
+    }
+#pragma unroll
+    for (int q = 0; q < STEPS; ++q) s[q].split(va[q], vb[q]);
+  }
+  float* oa = a.out + (size_t)ra * a.out_stride;
+  float* ob = a.out + (size_t)rb * a.out_stride;
+  constexpr int AT = STEPS * (int)sizeof(W) > 4 ? 1 : 4;  // column tiles whose weights are fetched at once
+  const bool wa = ra < a.rows && (ida >= 0 || move), wb = rb < a.rows && (idb >= 0 || move);
+  __syncthreads();  // t is in registers
+  for (int p = 0; p < passes; ++p) {
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncthreads();
+    issue_cols(p + 2);
+    const unsigned char* st = smem + p % LT_STAGES * T::STAGE;
+    const int n0 = (p * C + cr) * 64;
+    float d[4][4];  // this warp's four column tiles
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i][0] = d[i][1] = d[i][2] = d[i][3] = 0.f;
+    if (alone && (int)low_id == main_ad) {
+      const unsigned char* wt = st + LT_ROWS * LT_XROW + (32 * half + g) * T::BROW + 8 * c * (int)sizeof(W);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int q = 0; q < STEPS; ++q) {
-          if (in && n < a.n && 32 * q + 8 * c < R)
-            fetch(B + (size_t)n * a.rank + 32 * q, w[i][q]);
+          const int valid = main_rank - 32 * q - 8 * c;  // ranks of this lane's piece; B may hold anything behind them
+          if (32 * q >= main_rank) break;
+          Raw<W> w;
+          if (valid > 0)
+            load_raw(wt + 8 * i * T::BROW + 32 * q * (int)sizeof(W), w);
           else
-            clear(w[i][q]);
-          // ranks at and past R are 0 in t; what B holds there must not turn them into NaN
-          if (32 * q + 8 * c < R && 32 * q + 8 * c + 8 > R) cut(w[i][q], R - 32 * q - 8 * c);
+            clear(w);
+          if (valid > 0 && valid < 8) cut(w, valid);
+          s[q].mma(d[i], w);
         }
-        if (wide && in && col + 1 < a.n) {
-          if (ma) y0[i] = *reinterpret_cast<const float2*>(ya + col);
-          if (mb) y1[i] = *reinterpret_cast<const float2*>(yb + col);
+    } else {
+      each([&](int ad, bool ma, bool mb) {
+        const int R = rank_of(a, ad), n = n0 + 32 * half + g;
+        const W* B = reinterpret_cast<const W*>(a.b) + ((size_t)ad * a.n + n) * a.rank + 8 * c;
+#pragma unroll
+        for (int i0 = 0; i0 < 4; i0 += AT) {
+          Raw<W> w[AT][STEPS];
+#pragma unroll
+          for (int i = 0; i < AT; ++i)
+#pragma unroll
+            for (int q = 0; q < STEPS; ++q) {
+              const int valid = R - 32 * q - 8 * c;
+              if (valid > 0 && n + 8 * (i0 + i) < a.n)
+                fetch(B + (size_t)8 * (i0 + i) * a.rank + 32 * q, w[i][q]);
+              else
+                clear(w[i][q]);
+              if (valid > 0 && valid < 8) cut(w[i][q], valid);
+            }
+#pragma unroll
+          for (int i = 0; i < AT; ++i) {
+            float e[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < STEPS; ++q)
+              if (32 * q < R) s[q].mma(e, w[i][q]);
+            if (ma) d[i0 + i][0] = e[0], d[i0 + i][1] = e[1];
+            if (mb) d[i0 + i][2] = e[2], d[i0 + i][3] = e[3];
+          }
         }
-      }
+      });
+    }
 #pragma unroll
-      for (int i = 0; i < COLS; ++i) {
-        if (i0 + i >= t1) break;
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int q = 0; q < STEPS; ++q)
-          if (32 * q < R) step_mma<W>(d, s[q], w[i][q]);
-        const int col = 8 * (i0 + i) + 2 * c;
-        if (wide && col + 1 < a.n) {
-          if (ma) *reinterpret_cast<float2*>(oa + col) = make_float2(y0[i].x + d[0], y0[i].y + d[1]);
-          if (mb) *reinterpret_cast<float2*>(ob + col) = make_float2(y1[i].x + d[2], y1[i].y + d[3]);
-        } else {
-          if (ma) add(ya, oa, col, d[0], d[1]);
-          if (mb) add(yb, ob, col, d[2], d[3]);
+    for (int i = 0; i < 4; ++i) {
+      const int in_tile = 32 * half + 8 * i + 2 * c, col = n0 + in_tile;
+      if (col >= a.n) continue;
+      const float2 y0 = *reinterpret_cast<const float2*>(st + la * LT_XROW + in_tile * 4);
+      const float2 y1 = *reinterpret_cast<const float2*>(st + lb * LT_XROW + in_tile * 4);
+      // rows without an adapter have a sum of 0 or, among rows that have one, of whatever its weights times 0 are
+      const float2 u = ida >= 0 ? make_float2(y0.x + d[i][0] * ia, y0.y + d[i][1] * ia) : y0;
+      const float2 v = idb >= 0 ? make_float2(y1.x + d[i][2] * ib, y1.y + d[i][3] * ib) : y1;
+      if (out8 && col + 1 < a.n) {
+        if (wa) *reinterpret_cast<float2*>(oa + col) = u;
+        if (wb) *reinterpret_cast<float2*>(ob + col) = v;
+      } else {
+        if (wa) oa[col] = u.x;
+        if (wb) ob[col] = v.x;
+        if (col + 1 < a.n) {
+          if (wa) oa[col + 1] = u.y;
+          if (wb) ob[col + 1] = v.y;
         }
       }
     }
   }
-  if (a.out != a.y)  // rows without an adapter
-    for (int r = mt * 16; r < mt * 16 + 16 && row0 + r < a.rows; ++r) {
-      if (adapter_of(a, row0 + r) >= 0) continue;
-      const float* y = a.y + (size_t)(row0 + r) * a.y_stride;
-      float* o = a.out + (size_t)(row0 + r) * a.out_stride;
-      for (int n = 8 * t0 + lane; n < min(8 * t1, a.n); n += 32) o[n] = y[n];
-    }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 template <typename W, int LG>
@@ -477,7 +761,7 @@ int launch_row(const LoraArgs& a, cudaStream_t s) {
 template <typename W, int NT>
 int launch_tile(const LoraArgs& a, cudaStream_t s) {
   const int tiles = (a.rows + LT_ROWS - 1) / LT_ROWS;
-  const size_t smem = (size_t)3 * LT_ROWS * (8 * NT + 4) * 4;
+  const size_t smem = Tile<W, NT>::BYTES;
   auto kernel = lora_tile_kernel<W, NT>;
   if (allow_smem(kernel, smem)) return kCudaError;
   if ((long long)tiles * LR_CLUSTER > 0x7fffffffLL) return kTooLarge;
