@@ -412,7 +412,7 @@ struct Tile {
 };
 
 template <typename W, int NT>
-__global__ void __launch_bounds__(LR_THREADS) lora_tile_kernel(LoraArgs a) {
+__global__ void __launch_bounds__(LR_THREADS, sizeof(W) == 2 && NT <= 8 ? 2 : 1) lora_tile_kernel(LoraArgs a) {
   using T = Tile<W, NT>;
   constexpr int TS = T::TS, STEPS = (8 * NT + 31) / 32, EPP = 16 / (int)sizeof(W);  // weights of a 16-byte piece
   extern __shared__ __align__(16) unsigned char smem[];
@@ -444,75 +444,98 @@ __global__ void __launch_bounds__(LR_THREADS) lora_tile_kernel(LoraArgs a) {
   const int ida = ids[la], idb = ids[lb];
   const unsigned low_id = __reduce_min_sync(0xffffffffu, min((unsigned)ida, (unsigned)idb));  // -1 is the highest
   const int high_id = __reduce_max_sync(0xffffffffu, max(ida, idb));
-  const bool none = high_id < 0;                    // no row of this warp has an adapter
-  const bool alone = (unsigned)high_id == low_id;   // or they all have the same one (rows without may be among them)
-  // Calls f(adapter, whether row g has it, whether row g + 8 has it) for each adapter of the warp's rows.
-  auto each = [&](auto f) {
-    if (none) return;
-    if (alone) return f((int)low_id, ida >= 0, idb >= 0);
-    unsigned after = low_id;
-    for (;;) {
-      f((int)after, ida == (int)after, idb == (int)after);
-      const unsigned na = ida >= 0 && (unsigned)ida > after ? (unsigned)ida : 0xffffffffu;
-      const unsigned nb = idb >= 0 && (unsigned)idb > after ? (unsigned)idb : 0xffffffffu;
-      after = __reduce_min_sync(0xffffffffu, min(na, nb));
-      if (after == 0xffffffffu) break;
-    }
+  const bool none = high_id < 0;                                  // no row of this warp has an adapter
+  const bool only_main = low_id == (unsigned)main_ad && high_id == main_ad;  // all of them the staged one
+  const bool has_main = __any_sync(0xffffffffu, main_ad >= 0 && (ida == main_ad || idb == main_ad));
+  // The warp's other adapters in ascending order; -1 where there is none.  The first one's weights are fetched ahead.
+  auto other_after = [&](int prev) {
+    const unsigned na = ida > prev && ida != main_ad ? (unsigned)ida : 0xffffffffu;
+    const unsigned nb = idb > prev && idb != main_ad ? (unsigned)idb : 0xffffffffu;
+    return (int)__reduce_min_sync(0xffffffffu, min(na, nb));
   };
+  const int other = other_after(-1);
+  const int other_rank = other >= 0 ? rank_of(a, other) : 0;
 
   // ---- t = x A^T: the cluster's CTAs take 64 columns in turn, so that they read a row's neighbouring pieces together ----
   const int chunks = (a.k + LT_K - 1) / LT_K, turns = (chunks - cr + C - 1) / C;
-  auto issue = [&](int q) {
-    if (q < turns) {
-      unsigned char* st = smem + q % LT_STAGES * T::STAGE;
-      const int k0 = (q * C + cr) * LT_K;
+  // This thread's pieces of a stage: of x (and y) rows r16, r16 + 16, .., piece p16; of A rows wr, wr + WSTEP, .., piece
+  // wp.  Sources advance by a turn's columns.
+  constexpr int XROWS = LR_THREADS / 16, XN = LT_ROWS / XROWS;
+  constexpr int APR = LT_K / EPP, WSTEP = LR_THREADS / APR, AN = (8 * NT + WSTEP - 1) / WSTEP;
+  const int r16 = tid / 16, p16 = tid % 16, wr = tid / APR, wp = tid % APR;
+  unsigned have = 0;  // bit i: row r16 + 16 i has an adapter
 #pragma unroll
-      for (int i = 0; i < LT_ROWS * 16 / LR_THREADS; ++i) {
-        const int r = (i * LR_THREADS + tid) / 16, piece = (i * LR_THREADS + tid) % 16, k = k0 + piece * 4;
-        const bool ok = ids[r] >= 0 && k < a.k;
-        copy16(st + r * LT_XROW + piece * 16, a.x + (ok ? (size_t)(row0 + r) * a.x_stride + k : 0), ok);
-      }
-      unsigned char* wt = st + LT_ROWS * LT_XROW;
-      const W* A = reinterpret_cast<const W*>(a.a) + (size_t)max(main_ad, 0) * a.rank * a.k;
-      for (int i = tid; i < (main_rank + 7) / 8 * 8 * (LT_K / EPP); i += LR_THREADS) {
-        const int r = i / (LT_K / EPP), piece = i % (LT_K / EPP), k = k0 + piece * EPP;
-        const bool ok = r < main_rank && k < a.k;
-        copy16(wt + r * T::AROW + piece * 16, A + (ok ? (size_t)r * a.k + k : 0), ok);
-      }
+  for (int i = 0; i < XN; ++i) have |= (ids[r16 + XROWS * i] >= 0 ? 1u : 0u) << i;
+  const float* x_src = a.x + (size_t)(row0 + r16) * a.x_stride + cr * LT_K + p16 * 4;
+  const W* a_src = reinterpret_cast<const W*>(a.a) + ((size_t)max(main_ad, 0) * a.rank + wr) * a.k + cr * LT_K + wp * EPP;
+  unsigned char* const x_dst = smem + r16 * LT_XROW + p16 * 16;
+  unsigned char* const a_dst = smem + LT_ROWS * LT_XROW + wr * T::AROW + wp * 16;
+  int k_left = a.k - cr * LT_K, fill = 0;  // columns from this turn's first; stage that is filled next
+  auto issue = [&]() {
+    if (k_left > 0) {
+      const bool in_x = p16 * 4 < k_left, in_a = wp * EPP < k_left;
+#pragma unroll
+      for (int i = 0; i < XN; ++i)
+        copy16(x_dst + fill * T::STAGE + i * XROWS * LT_XROW, x_src + (size_t)i * XROWS * a.x_stride,
+               in_x && (have >> i & 1u));
+#pragma unroll
+      for (int i = 0; i < AN; ++i)
+        if ((8 * NT) % WSTEP == 0 || wr + i * WSTEP < 8 * NT)
+          copy16(a_dst + fill * T::STAGE + i * WSTEP * T::AROW, a_src + (size_t)i * WSTEP * a.k,
+                 in_a && wr + i * WSTEP < main_rank);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
+    x_src += C * LT_K;
+    a_src += C * LT_K;
+    k_left -= C * LT_K;
+    fill = fill == LT_STAGES - 1 ? 0 : fill + 1;
   };
   {
     float acc[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-    float sa = 0.f, sb = 0.f;  // 0: not chosen yet
-    issue(0);
-    issue(1);
+    // Powers of two of the two rows: no element times them passes 2^15.  They start so high that the first element
+    // which is not 0 (or below 2^-85) chooses them.
+    constexpr float UNSET = 1.2676506e30f;  // 2^100
+    float sa = UNSET, sb = UNSET;
+    issue();
+    issue();
+    int use = 0;  // stage that is read next
+    auto fetch_a = [&](int ad, int R, int q, Raw<W>(&w)[NT]) {
+      const int k = (q * C + cr) * LT_K + half * 32 + 8 * c;
+      const W* A = reinterpret_cast<const W*>(a.a) + ((size_t)ad * a.rank + g) * a.k + k;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        if (8 * i + g < R && k < a.k)
+          fetch(A + (size_t)8 * i * a.k, w[i]);
+        else
+          clear(w[i]);
+      }
+    };
     for (int q = 0; q < turns; ++q) {
+      Raw<W> w[NT];
+      if (other >= 0) fetch_a(other, other_rank, q, w);
       asm volatile("cp.async.wait_group 1;" ::: "memory");
       __syncthreads();
-      issue(q + 2);
+      issue();
+      const unsigned char* st = smem + use * T::STAGE;
+      use = use == LT_STAGES - 1 ? 0 : use + 1;
       if (none) continue;
-      const unsigned char* st = smem + q % LT_STAGES * T::STAGE;
       float va[8], vb[8];
       load_row8(reinterpret_cast<const float*>(st + la * LT_XROW) + half * 32 + 8 * c, va);
       load_row8(reinterpret_cast<const float*>(st + lb * LT_XROW) + half * 32 + 8 * c, vb);
       if constexpr (Step<W>::SCALED) {
-        // The rows' powers of two come from their first 32 elements that are not all 0, with room for 2^8 times as
-        // much; where more comes, the sums so far follow.
+        // A row's power of two comes from its first 32 elements, with room for 2^8 times as much; where more comes, the
+        // sums so far follow.
         float ta = top8(va), tb = top8(vb);
-        const bool low = (sa == 0.f && ta > 0.f) || (sb == 0.f && tb > 0.f);
-        const bool high = (ta * sa > 32768.f && ta < INFINITY) || (tb * sb > 32768.f && tb < INFINITY);
-        if (__any_sync(0xffffffffu, low || high)) {
+        if (__any_sync(0xffffffffu, fmaxf(ta * sa, tb * sb) > 32768.f)) {
           ta = top_quad(ta);
           tb = top_quad(tb);
           auto follow = [&](float& s, float top, int k) {
-            if ((s == 0.f && top > 0.f) || (top * s > 32768.f && top < INFINITY)) {
-              const float n = scale_for(top);
-              if (s != 0.f)
+            if (top * s > 32768.f && top < INFINITY) {
+              const float n = scale_for(top), f = n / s;
 #pragma unroll
-                for (int i = 0; i < NT; ++i) acc[i][k] *= n / s, acc[i][k + 1] *= n / s;
+              for (int i = 0; i < NT; ++i) acc[i][k] *= f, acc[i][k + 1] *= f;
               s = n;
             }
           };
@@ -524,42 +547,43 @@ __global__ void __launch_bounds__(LR_THREADS) lora_tile_kernel(LoraArgs a) {
       }
       Step<W> s;
       s.split(va, vb);
-      if (alone && (int)low_id == main_ad) {
-        const unsigned char* wt = st + LT_ROWS * LT_XROW + g * T::AROW + (half * 32 + 8 * c) * (int)sizeof(W);
+      const unsigned char* wt = st + LT_ROWS * LT_XROW + g * T::AROW + (half * 32 + 8 * c) * (int)sizeof(W);
+      if (only_main) {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
           if (8 * i < main_rank) {
-            Raw<W> w;
-            load_raw(wt + i * 8 * T::AROW, w);
-            s.mma(acc[i], w);
+            Raw<W> m;
+            load_raw(wt + i * 8 * T::AROW, m);
+            s.mma(acc[i], m);
           }
       } else {
-        const int k = (q * C + cr) * LT_K + half * 32 + 8 * c;
-        each([&](int ad, bool ma, bool mb) {
-          const int R = rank_of(a, ad);
-          const W* A = reinterpret_cast<const W*>(a.a) + ((size_t)ad * a.rank + g) * a.k + k;
-          Raw<W> w[NT];  // all on their way before the first is used
-#pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            if (8 * i + g < R && k < a.k)
-              fetch(A + (size_t)8 * i * a.k, w[i]);
-            else
-              clear(w[i]);
-          }
+        // Sums of their own: what an adapter holds reaches its own rows only.
+        auto put = [&](int i, const Raw<W>& m, int ad) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+          s.mma(d, m);
+          if (ida == ad) acc[i][0] += d[0], acc[i][1] += d[1];
+          if (idb == ad) acc[i][2] += d[2], acc[i][3] += d[3];
+        };
+        int R = other_rank;
+        for (int ad = other; ad >= 0;) {
 #pragma unroll
           for (int i = 0; i < NT; ++i)
-            if (8 * i < R) {
-              // a sum of its own: what this adapter holds reaches its own rows only
-              float d[4] = {0.f, 0.f, 0.f, 0.f};
-              s.mma(d, w[i]);
-              if (ma) acc[i][0] += d[0], acc[i][1] += d[1];
-              if (mb) acc[i][2] += d[2], acc[i][3] += d[3];
+            if (8 * i < R) put(i, w[i], ad);
+          ad = other_after(ad);
+          if (ad >= 0) fetch_a(ad, R = rank_of(a, ad), q, w);
+        }
+        if (has_main)
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+            if (8 * i < main_rank) {
+              Raw<W> m;
+              load_raw(wt + i * 8 * T::AROW, m);
+              put(i, m, main_ad);
             }
-        });
       }
     }
     // the two halves of each 64, in turn
-    const float ia = Step<W>::SCALED && sa != 0.f ? 1.f / sa : 1.f, ib = Step<W>::SCALED && sb != 0.f ? 1.f / sb : 1.f;
+    const float ia = Step<W>::SCALED ? 1.f / sa : 1.f, ib = Step<W>::SCALED ? 1.f / sb : 1.f;
 #pragma unroll
     for (int h = 1; h >= 0; --h) {
       if (half == h) {
@@ -582,34 +606,45 @@ __global__ void __launch_bounds__(LR_THREADS) lora_tile_kernel(LoraArgs a) {
   const bool y16 = (uintptr_t)a.y % 16 == 0 && a.y_stride % 4 == 0;
   const bool out8 = (uintptr_t)a.out % 8 == 0 && a.out_stride % 2 == 0;
   const bool move = a.out != a.y;  // rows without an adapter are copied
-  auto issue_cols = [&](int p) {
-    if (p < passes) {
-      unsigned char* st = smem + p % LT_STAGES * T::STAGE;
-      const int n0 = (p * C + cr) * 64;
+  constexpr int BPR = 8 * NT / EPP, BSTEP = LR_THREADS / BPR, BN = (64 + BSTEP - 1) / BSTEP;
+  const int br = tid / BPR, bp = tid % BPR;
+  unsigned need = 0;  // bit i: row r16 + 16 i passes through
 #pragma unroll
-      for (int i = 0; i < LT_ROWS * 16 / LR_THREADS; ++i) {
-        const int r = (i * LR_THREADS + tid) / 16, piece = (i * LR_THREADS + tid) % 16, n = n0 + piece * 4;
-        const bool ok = row0 + r < a.rows && (ids[r] >= 0 || move);
-        const float* from = a.y + (ok ? (size_t)(row0 + r) * a.y_stride : 0);
-        unsigned char* to = st + r * LT_XROW + piece * 16;
-        if (y16 && n + 4 <= a.n) {
-          copy16(to, from + n, ok);
+  for (int i = 0; i < XN; ++i)
+    need |= (row0 + r16 + XROWS * i < a.rows && (move || ids[r16 + XROWS * i] >= 0) ? 1u : 0u) << i;
+  const float* y_src = a.y + (size_t)(row0 + r16) * a.y_stride + cr * 64 + p16 * 4;
+  const W* b_src = reinterpret_cast<const W*>(a.b) + ((size_t)max(main_ad, 0) * a.n + cr * 64 + br) * a.rank + bp * EPP;
+  unsigned char* const b_dst = smem + LT_ROWS * LT_XROW + br * T::BROW + bp * 16;
+  int n_left = a.n - cr * 64;
+  fill = 0;
+  auto issue_cols = [&]() {
+    if (n_left > 0) {
+      unsigned char* to = x_dst + fill * T::STAGE;
+      const int in = n_left - p16 * 4;  // columns from this piece's first
+#pragma unroll
+      for (int i = 0; i < XN; ++i) {
+        const float* from = y_src + (size_t)i * XROWS * a.y_stride;
+        if (y16 && in >= 4) {
+          copy16(to + i * XROWS * LT_XROW, from, need >> i & 1u);
         } else {
-          for (int k = 0; k < 4; ++k) copy4(to + 4 * k, from + (n + k < a.n ? n + k : 0), ok && n + k < a.n);
+          for (int k = 0; k < 4; ++k)
+            copy4(to + i * XROWS * LT_XROW + 4 * k, k < in ? from + k : a.y, k < in && (need >> i & 1u));
         }
       }
-      unsigned char* wt = st + LT_ROWS * LT_XROW;
-      const int pieces = (main_rank + EPP - 1) / EPP;
-      const W* B = reinterpret_cast<const W*>(a.b) + (size_t)max(main_ad, 0) * a.n * a.rank;
-      for (int i = tid; i < 64 * pieces; i += LR_THREADS) {
-        const int r = i / pieces, piece = i - r * pieces, n = n0 + r;
-        copy16(wt + r * T::BROW + piece * 16, B + (n < a.n ? (size_t)n * a.rank + piece * EPP : 0), n < a.n);
-      }
+#pragma unroll
+      for (int i = 0; i < BN; ++i)
+        if (64 % BSTEP == 0 || br + i * BSTEP < 64)
+          copy16(b_dst + fill * T::STAGE + i * BSTEP * T::BROW, b_src + (size_t)i * BSTEP * a.rank,
+                 br + i * BSTEP < n_left && bp * EPP < main_rank);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
+    y_src += C * 64;
+    b_src += (size_t)C * 64 * a.rank;
+    n_left -= C * 64;
+    fill = fill == LT_STAGES - 1 ? 0 : fill + 1;
   };
-  issue_cols(0);  // while the cluster sums t, whose place is the last stage
-  issue_cols(1);
+  issue_cols();  // while the cluster sums t, whose place is the last stage
+  issue_cols();
   cluster.sync();
   // every CTA sums a part of t over the cluster and gives it to the others
   for (int i = cr * LR_THREADS + tid; i < LT_ROWS * 2 * NT; i += C * LR_THREADS) {  // 4 ranks of a row
@@ -667,80 +702,95 @@ __global__ void __launch_bounds__(LR_THREADS) lora_tile_kernel(LoraArgs a) {
   constexpr int AT = STEPS * (int)sizeof(W) > 4 ? 1 : 4;  // column tiles whose weights are fetched at once
   const bool wa = ra < a.rows && (ida >= 0 || move), wb = rb < a.rows && (idb >= 0 || move);
   __syncthreads();  // t is in registers
+  const bool ragged = main_rank % 8 != 0;  // the last piece of B's rows holds ranks that are not this adapter's
+  const bool bare = __any_sync(0xffffffffu, ida < 0 || idb < 0);
+  int use = 0;
+  auto fetch_b = [&](int ad, int R, int n0, int i0, Raw<W>(&w)[AT][STEPS]) {
+    const int n = n0 + 32 * half + g;
+    const W* B = reinterpret_cast<const W*>(a.b) + ((size_t)ad * a.n + n) * a.rank + 8 * c;
+#pragma unroll
+    for (int i = 0; i < AT; ++i)
+#pragma unroll
+      for (int q = 0; q < STEPS; ++q) {
+        const int valid = R - 32 * q - 8 * c;  // ranks of this lane's piece; B may hold anything behind them
+        if (valid > 0 && n + 8 * (i0 + i) < a.n)
+          fetch(B + (size_t)8 * (i0 + i) * a.rank + 32 * q, w[i][q]);
+        else
+          clear(w[i][q]);
+        if (valid > 0 && valid < 8) cut(w[i][q], valid);
+      }
+  };
   for (int p = 0; p < passes; ++p) {
+    Raw<W> w[AT][STEPS];
+    if (other >= 0) fetch_b(other, other_rank, (p * C + cr) * 64, 0, w);
     asm volatile("cp.async.wait_group 1;" ::: "memory");
     __syncthreads();
-    issue_cols(p + 2);
-    const unsigned char* st = smem + p % LT_STAGES * T::STAGE;
+    issue_cols();
+    const unsigned char* st = smem + use * T::STAGE;
+    use = use == LT_STAGES - 1 ? 0 : use + 1;
     const int n0 = (p * C + cr) * 64;
     float d[4][4];  // this warp's four column tiles
 #pragma unroll
     for (int i = 0; i < 4; ++i) d[i][0] = d[i][1] = d[i][2] = d[i][3] = 0.f;
-    if (alone && (int)low_id == main_ad) {
-      const unsigned char* wt = st + LT_ROWS * LT_XROW + (32 * half + g) * T::BROW + 8 * c * (int)sizeof(W);
+    const unsigned char* wt = st + LT_ROWS * LT_XROW + (32 * half + g) * T::BROW + 8 * c * (int)sizeof(W);
+    if (has_main) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int q = 0; q < STEPS; ++q) {
-          const int valid = main_rank - 32 * q - 8 * c;  // ranks of this lane's piece; B may hold anything behind them
           if (32 * q >= main_rank) break;
-          Raw<W> w;
-          if (valid > 0)
-            load_raw(wt + 8 * i * T::BROW + 32 * q * (int)sizeof(W), w);
+          Raw<W> m;
+          if (8 * NT >= 32 || 8 * c < 8 * NT)
+            load_raw(wt + 8 * i * T::BROW + 32 * q * (int)sizeof(W), m);
           else
-            clear(w);
-          if (valid > 0 && valid < 8) cut(w, valid);
-          s[q].mma(d[i], w);
-        }
-    } else {
-      each([&](int ad, bool ma, bool mb) {
-        const int R = rank_of(a, ad), n = n0 + 32 * half + g;
-        const W* B = reinterpret_cast<const W*>(a.b) + ((size_t)ad * a.n + n) * a.rank + 8 * c;
-#pragma unroll
-        for (int i0 = 0; i0 < 4; i0 += AT) {
-          Raw<W> w[AT][STEPS];
-#pragma unroll
-          for (int i = 0; i < AT; ++i)
-#pragma unroll
-            for (int q = 0; q < STEPS; ++q) {
-              const int valid = R - 32 * q - 8 * c;
-              if (valid > 0 && n + 8 * (i0 + i) < a.n)
-                fetch(B + (size_t)8 * (i0 + i) * a.rank + 32 * q, w[i][q]);
-              else
-                clear(w[i][q]);
-              if (valid > 0 && valid < 8) cut(w[i][q], valid);
-            }
-#pragma unroll
-          for (int i = 0; i < AT; ++i) {
-            float e[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int q = 0; q < STEPS; ++q)
-              if (32 * q < R) s[q].mma(e, w[i][q]);
-            if (ma) d[i0 + i][0] = e[0], d[i0 + i][1] = e[1];
-            if (mb) d[i0 + i][2] = e[2], d[i0 + i][3] = e[3];
+            clear(m);
+          if (ragged) {  // t is 0 there, but B may hold anything
+            const int valid = main_rank - 32 * q - 8 * c;
+            if (valid > 0 && valid < 8) cut(m, valid);
           }
+          s[q].mma(d[i], m);
         }
-      });
     }
+    int R = other_rank;
+    for (int ad = other; ad >= 0;) {  // each row's sum is its own adapter's
+#pragma unroll
+      for (int i0 = 0; i0 < 4; i0 += AT) {
+        if (i0 > 0) fetch_b(ad, R, n0, i0, w);
+#pragma unroll
+        for (int i = 0; i < AT; ++i) {
+          float e[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int q = 0; q < STEPS; ++q)
+            if (32 * q < R) s[q].mma(e, w[i][q]);
+          if (ida == ad) d[i0 + i][0] = e[0], d[i0 + i][1] = e[1];
+          if (idb == ad) d[i0 + i][2] = e[2], d[i0 + i][3] = e[3];
+        }
+      }
+      ad = other_after(ad);
+      if (ad >= 0) fetch_b(ad, R = rank_of(a, ad), n0, 0, w);
+    }
+    const bool whole = out8 && n0 + 64 <= a.n;
+    float* const pa = oa + n0 + 32 * half + 2 * c;
+    float* const pb = ob + n0 + 32 * half + 2 * c;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int in_tile = 32 * half + 8 * i + 2 * c, col = n0 + in_tile;
-      if (col >= a.n) continue;
-      const float2 y0 = *reinterpret_cast<const float2*>(st + la * LT_XROW + in_tile * 4);
-      const float2 y1 = *reinterpret_cast<const float2*>(st + lb * LT_XROW + in_tile * 4);
-      // rows without an adapter have a sum of 0 or, among rows that have one, of whatever its weights times 0 are
-      const float2 u = ida >= 0 ? make_float2(y0.x + d[i][0] * ia, y0.y + d[i][1] * ia) : y0;
-      const float2 v = idb >= 0 ? make_float2(y1.x + d[i][2] * ib, y1.y + d[i][3] * ib) : y1;
-      if (out8 && col + 1 < a.n) {
-        if (wa) *reinterpret_cast<float2*>(oa + col) = u;
-        if (wb) *reinterpret_cast<float2*>(ob + col) = v;
+      const float2 y0 = *reinterpret_cast<const float2*>(st + la * LT_XROW + (32 * half + 8 * i + 2 * c) * 4);
+      const float2 y1 = *reinterpret_cast<const float2*>(st + lb * LT_XROW + (32 * half + 8 * i + 2 * c) * 4);
+      float2 u = make_float2(fmaf(d[i][0], ia, y0.x), fmaf(d[i][1], ia, y0.y));
+      float2 v = make_float2(fmaf(d[i][2], ib, y1.x), fmaf(d[i][3], ib, y1.y));
+      if (bare) {  // rows without an adapter among rows that have one: whatever its weights times 0 are stays out
+        if (ida < 0) u = y0;
+        if (idb < 0) v = y1;
+      }
+      if (whole) {
+        if (wa) *reinterpret_cast<float2*>(pa + 8 * i) = u;
+        if (wb) *reinterpret_cast<float2*>(pb + 8 * i) = v;
       } else {
-        if (wa) oa[col] = u.x;
-        if (wb) ob[col] = v.x;
-        if (col + 1 < a.n) {
-          if (wa) oa[col + 1] = u.y;
-          if (wb) ob[col + 1] = v.y;
-        }
+        const int col = n0 + 32 * half + 8 * i + 2 * c;
+        if (wa && col < a.n) pa[8 * i] = u.x;
+        if (wb && col < a.n) pb[8 * i] = v.x;
+        if (wa && col + 1 < a.n) pa[8 * i + 1] = u.y;
+        if (wb && col + 1 < a.n) pb[8 * i + 1] = v.y;
       }
     }
   }
