@@ -23,12 +23,25 @@ namespace {
 
 constexpr int KA_WARPS = 8;
 constexpr int KA_UNROLL = 4;  // token rows of K and V in flight per lane
+constexpr int KA_HELD = 8;    // stored keys likewise
 
-__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float4 load4(const __half* p) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+// Four elements of a row as they lie in memory.
+template <typename T>
+struct Row;
+template <>
+struct Row<float> {
+  float4 v;
+};
+template <>
+struct Row<__half> {
+  uint2 v;
+};
+__device__ __forceinline__ Row<float> fetch(const float* p) { return {*reinterpret_cast<const float4*>(p)}; }
+__device__ __forceinline__ Row<__half> fetch(const __half* p) { return {*reinterpret_cast<const uint2*>(p)}; }
+__device__ __forceinline__ float4 floats(const Row<float>& r) { return r.v; }
+__device__ __forceinline__ float4 floats(const Row<__half>& r) {
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&r.v.x));
+  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&r.v.y));
   return make_float4(a.x, a.y, b.x, b.y);
 }
 // Stores v in the pool's type and returns what was stored.
@@ -51,17 +64,17 @@ __device__ __forceinline__ void widen(float4& lo, float4& hi, float4 k) {
   hi.x = fmaxf(hi.x, k.x), hi.y = fmaxf(hi.y, k.y), hi.z = fmaxf(hi.z, k.z), hi.w = fmaxf(hi.w, k.w);
 }
 
-// floor(x / s) of the real quotient, clamped to [-127, 127]; s > 0.  A rounded quotient is off by at most one step
-// of its last place, so only an integer next to it can be wrong: fma gives the residual's sign exactly.
-__device__ __forceinline__ int floor_code(float x, float s) {
-  float f = floorf(__fdiv_rn(x, s));
+// floor(x / s) of the real quotient, |x / s| <= 128, clamped to [-127, 127]; inv = 1 / s rounded.  The product is off by
+// less than 2^-15, so only an integer next to it can be wrong: fma gives the residual's sign exactly.
+__device__ __forceinline__ int floor_code(float x, float s, float inv) {
+  float f = floorf(inv > 0.f ? x * inv : __fdiv_rn(x, s));  // 0: s so small that 1 / s may not be finite
   if (__fmaf_rn(-f, s, x) < 0.f) f -= 1.f;
   else if (__fmaf_rn(-(f + 1.f), s, x) >= 0.f) f += 1.f;
   return (int)fminf(fmaxf(f, -127.f), 127.f);
 }
 
 template <int HD, typename IN, typename KV>
-__global__ void __launch_bounds__(KA_WARPS * 32) kv_append_kernel(KvAppendArgs a, int tile, long long units) {
+__global__ void __launch_bounds__(KA_WARPS * 32, 2) kv_append_kernel(KvAppendArgs a, int tile, long long units) {
   constexpr int VEC = HD / 4;                       // 4-element pieces of a row
   constexpr int LPR = VEC < 32 ? VEC : 32;          // lanes per row
   constexpr int ROWS = 32 / LPR;                    // rows a warp takes at once
@@ -108,18 +121,36 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv_append_kernel(KvAppendArgs a
       lo[p] = make_float4(INFINITY, INFINITY, INFINITY, INFINITY);
       hi[p] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     }
-    for (int i0 = sub; i0 < n; i0 += ROWS * KA_UNROLL) {
-      float4 kr[KA_UNROLL][PCS], vr[KA_UNROLL][PCS];
+    // the run's first rows and the keys that earlier calls stored are on their way together
+    Row<IN> kr[KA_UNROLL][PCS], vr[KA_UNROLL][PCS];
+    auto load_run = [&](int i0) {
 #pragma unroll
       for (int u = 0; u < KA_UNROLL; ++u) {
         const int i = i0 + u * ROWS;
         if (i < n)
 #pragma unroll
           for (int p = 0; p < PCS; ++p) {
-            kr[u][p] = load4(kin + (long long)(t + i) * a.k_stride + p * 128);
-            vr[u][p] = load4(vin + (long long)(t + i) * a.v_stride + p * 128);
+            kr[u][p] = fetch(kin + (long long)(t + i) * a.k_stride + p * 128);
+            vr[u][p] = fetch(vin + (long long)(t + i) * a.v_stride + p * 128);
           }
       }
+    };
+    load_run(sub);
+    if (a.bounds)
+      for (int i0 = sub; i0 < s0; i0 += ROWS * KA_HELD) {
+        Row<KV> hr[KA_HELD][PCS];
+#pragma unroll
+        for (int u = 0; u < KA_HELD; ++u)
+          if (i0 + u * ROWS < s0)
+#pragma unroll
+            for (int p = 0; p < PCS; ++p) hr[u][p] = fetch(kp + (long long)(i0 + u * ROWS) * a.slot_stride + p * 128);
+#pragma unroll
+        for (int u = 0; u < KA_HELD; ++u)
+          if (i0 + u * ROWS < s0)
+#pragma unroll
+            for (int p = 0; p < PCS; ++p) widen(lo[p], hi[p], floats(hr[u][p]));
+      }
+    for (int i0 = sub;;) {
 #pragma unroll
       for (int u = 0; u < KA_UNROLL; ++u) {
         const int i = i0 + u * ROWS;
@@ -127,26 +158,15 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv_append_kernel(KvAppendArgs a
 #pragma unroll
           for (int p = 0; p < PCS; ++p) {
             const long long at = (long long)(s0 + i) * a.slot_stride + p * 128;
-            widen(lo[p], hi[p], store4(kp + at, kr[u][p]));
-            store4(vp + at, vr[u][p]);
+            widen(lo[p], hi[p], store4(kp + at, floats(kr[u][p])));
+            store4(vp + at, floats(vr[u][p]));
           }
       }
+      i0 += ROWS * KA_UNROLL;
+      if (i0 >= n) break;
+      load_run(i0);
     }
     if (a.bounds) {
-      for (int i0 = sub; i0 < s0; i0 += ROWS * KA_UNROLL) {  // keys stored by earlier calls
-        float4 kr[KA_UNROLL][PCS];
-#pragma unroll
-        for (int u = 0; u < KA_UNROLL; ++u)
-          if (i0 + u * ROWS < s0)
-#pragma unroll
-            for (int p = 0; p < PCS; ++p)
-              kr[u][p] = load4(kp + (long long)(i0 + u * ROWS) * a.slot_stride + p * 128);
-#pragma unroll
-        for (int u = 0; u < KA_UNROLL; ++u)
-          if (i0 + u * ROWS < s0)
-#pragma unroll
-            for (int p = 0; p < PCS; ++p) widen(lo[p], hi[p], kr[u][p]);
-      }
       float top = 0.f;
 #pragma unroll
       for (int p = 0; p < PCS; ++p) {
@@ -165,16 +185,17 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv_append_kernel(KvAppendArgs a
                                fmaxf(fmaxf(fabsf(hi[p].x), fabsf(hi[p].y)), fmaxf(fabsf(hi[p].z), fabsf(hi[p].w)))));
       }
       const float s = __fdiv_rn(warp_max(top), 127.f);
+      const float inv = s > 1e-30f ? 1.f / s : 0.f;
       int8_t* codes = a.bounds + ((size_t)page * a.hkv + h) * 2 * HD + col;
       if (sub == 0)
 #pragma unroll
         for (int p = 0; p < PCS; ++p) {
           char4 l = make_char4(0, 0, 0, 0), u = l;
           if (s > 0.f && s < INFINITY) {
-            l = make_char4(floor_code(lo[p].x, s), floor_code(lo[p].y, s), floor_code(lo[p].z, s),
-                           floor_code(lo[p].w, s));
-            u = make_char4(-floor_code(-hi[p].x, s), -floor_code(-hi[p].y, s), -floor_code(-hi[p].z, s),
-                           -floor_code(-hi[p].w, s));
+            l = make_char4(floor_code(lo[p].x, s, inv), floor_code(lo[p].y, s, inv), floor_code(lo[p].z, s, inv),
+                           floor_code(lo[p].w, s, inv));
+            u = make_char4(-floor_code(-hi[p].x, s, inv), -floor_code(-hi[p].y, s, inv),
+                           -floor_code(-hi[p].z, s, inv), -floor_code(-hi[p].w, s, inv));
           }
           *reinterpret_cast<char4*>(codes + p * 128) = l;
           *reinterpret_cast<char4*>(codes + HD + p * 128) = u;

@@ -28,22 +28,81 @@ namespace zc {
 
 namespace {
 
-constexpr int LG_THREADS = 512;
+constexpr int LG_THREADS = 256;
 constexpr int LG_SMEM_MAX = 200 * 1024;
-constexpr unsigned SEEN = 0x80000000u;  // a history token; the other bits count its generated occurrences
+constexpr int LG_AHEAD = 8;  // 4-token groups per thread that are on their way while the history is counted
+
+// A token's count: the top bit marks a history token, the others its generated occurrences.  16 bits hold it (and four
+// CTAs an SM their slices of a vocabulary of 131,072) unless a history or a bias list is longer than 32767.
+template <typename H>
+struct Count;
+template <>
+struct Count<uint16_t> {
+  static constexpr unsigned SEEN = 0x8000u;
+  static __device__ __forceinline__ void note(unsigned* word_base, int i, bool generated) {  // word_base may be remote
+    unsigned* w = word_base + (i >> 1);
+    const int sh = 16 * (i & 1);
+    if (generated) atomicAdd(w, 1u << sh);
+    atomicOr(w, SEEN << sh);
+  }
+  static __device__ __forceinline__ void load(const uint16_t* p, unsigned (&h)[4]) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    h[0] = u.x & 0xffffu, h[1] = u.x >> 16, h[2] = u.y & 0xffffu, h[3] = u.y >> 16;
+  }
+  static __device__ __forceinline__ void raise(uint16_t* p, unsigned v) {
+    for (unsigned old = *p; old < v;) {
+      const unsigned was = atomicCAS(p, (unsigned short)old, (unsigned short)v);
+      if (was == old) break;
+      old = was;
+    }
+  }
+  static __device__ __forceinline__ void mark(uint16_t* p) {
+    for (unsigned old = *p; !(old & SEEN);) {
+      const unsigned was = atomicCAS(p, (unsigned short)old, (unsigned short)(old | SEEN));
+      if (was == old) break;
+      old = was;
+    }
+  }
+};
+template <>
+struct Count<uint32_t> {
+  static constexpr unsigned SEEN = 0x80000000u;
+  static __device__ __forceinline__ void note(unsigned* word_base, int i, bool generated) {
+    if (generated) atomicAdd(word_base + i, 1u);
+    atomicOr(word_base + i, SEEN);
+  }
+  static __device__ __forceinline__ void load(const uint32_t* p, unsigned (&h)[4]) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    h[0] = u.x, h[1] = u.y, h[2] = u.z, h[3] = u.w;
+  }
+  static __device__ __forceinline__ void raise(uint32_t* p, unsigned v) { atomicMax(p, v); }
+  static __device__ __forceinline__ void mark(uint32_t* p) { atomicOr(p, SEEN); }
+};
 
 __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-__device__ __forceinline__ void load_vec(const float* p, float* v) {
-  const float4 f = *reinterpret_cast<const float4*>(p);
-  v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+// Four logits as they lie in memory.
+template <typename T>
+struct Group {
+  uint2 v;
+};
+template <>
+struct Group<float> {
+  float4 v;
+};
+__device__ __forceinline__ Group<float> fetch(const float* p) { return {*reinterpret_cast<const float4*>(p)}; }
+template <typename T>
+__device__ __forceinline__ Group<T> fetch(const T* p) {
+  return {*reinterpret_cast<const uint2*>(p)};
+}
+__device__ __forceinline__ void floats(const Group<float>& g, float (&v)[4]) {
+  v[0] = g.v.x, v[1] = g.v.y, v[2] = g.v.z, v[3] = g.v.w;
 }
 template <typename T>
-__device__ __forceinline__ void load_vec(const T* p, float* v) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  const T* e = reinterpret_cast<const T*>(&u);
+__device__ __forceinline__ void floats(const Group<T>& g, float (&v)[4]) {
+  const T* e = reinterpret_cast<const T*>(&g.v);
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = to_f(e[i]);
 }
@@ -52,6 +111,7 @@ struct Rules {
   float repetition, frequency, presence;
 };
 
+template <unsigned SEEN>
 __device__ __forceinline__ float apply(float v, unsigned h, const Rules& r) {
   if (h) {
     v = v > 0.f ? __fdiv_rn(v, r.repetition) : v * r.repetition;
@@ -62,9 +122,11 @@ __device__ __forceinline__ float apply(float v, unsigned h, const Rules& r) {
 }
 
 // VEC: both row starts are 16-byte (8-byte for 16-bit input) aligned, so 4 tokens move per access.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(LG_THREADS) logits_kernel(LogitsArgs a, int slice, bool in_place) {
-  extern __shared__ __align__(16) unsigned hist[];  // [slice]
+template <typename T, typename H, bool VEC>
+__global__ void __launch_bounds__(LG_THREADS, 4) logits_kernel(LogitsArgs a, int slice, bool in_place) {
+  constexpr unsigned SEEN = Count<H>::SEEN;
+  extern __shared__ __align__(16) unsigned smem[];
+  H* hist = reinterpret_cast<H*>(smem);  // [slice]
   pdl_trigger();
   pdl_wait();
   cg::cluster_group cluster = cg::this_cluster();
@@ -88,50 +150,69 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(LogitsArgs a, int sl
     }
     if (rules.repetition == 1.f && rules.frequency == 0.f && rules.presence == 0.f) n_past = 0;
   }
+  const uint32_t* mask = nullptr;
+  if (a.mask) {
+    const int m = a.mask_rows ? a.mask_rows[row] : row;
+    if ((unsigned)m < (unsigned)a.masks) mask = a.mask + (size_t)m * a.mask_stride;
+  }
+  // the first groups of the slice and their mask words, unless in place, where most logits are not needed
+  const int n4 = VEC ? (v1 - v0) / 4 : 0;
+  Group<T> ahead[LG_AHEAD];
+  uint32_t words[LG_AHEAD];
+  auto load_ahead = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < LG_AHEAD; ++u) {
+      const int i = i0 + u * LG_THREADS;
+      if (i < n4 && !in_place) ahead[u] = fetch(x + v0 + 4 * i);
+      words[u] = mask && i < n4 ? __ldg(mask + ((v0 + 4 * i) >> 5)) : 0xffffffffu;
+    }
+  };
+  load_ahead(threadIdx.x);
   if (n_past > 0) {  // the same for every CTA of the cluster
-    for (int i = threadIdx.x * 4; i < slice; i += LG_THREADS * 4)  // slice is a multiple of 32
+    constexpr int PER = 16 / sizeof(H);
+    for (int i = threadIdx.x * PER; i < slice; i += LG_THREADS * PER)  // slice is a multiple of 32
       *reinterpret_cast<uint4*>(hist + i) = make_uint4(0, 0, 0, 0);
     cluster.sync();
     for (int i = rank * LG_THREADS + threadIdx.x; i < n_past; i += ranks * LG_THREADS) {
       const int t = past[i];
       if ((unsigned)t >= (unsigned)a.vocab) continue;
       const int owner = t / slice;
-      unsigned* h = cluster.map_shared_rank(hist, owner) + (t - owner * slice);
-      if (i >= n_prompt) atomicAdd(h, 1u);
-      atomicOr(h, SEEN);
+      Count<H>::note(cluster.map_shared_rank(smem, owner), t - owner * slice, i >= n_prompt);
     }
     cluster.sync();
   }
-  const uint32_t* mask = nullptr;
-  if (a.mask) {
-    const int m = a.mask_rows ? a.mask_rows[row] : row;
-    if ((unsigned)m < (unsigned)a.masks) mask = a.mask + (size_t)m * a.mask_stride;
-  }
 
   const bool hashed = n_past > 0;
-  if (VEC) {
-    const int n4 = (v1 - v0) / 4;
-    for (int i = threadIdx.x; i < n4; i += LG_THREADS) {
-      const int t = v0 + 4 * i;
-      const unsigned bits = mask ? (__ldg(mask + (t >> 5)) >> (t & 31)) & 15u : 15u;
-      uint4 h = make_uint4(0, 0, 0, 0);
-      if (hashed) h = *reinterpret_cast<const uint4*>(hist + 4 * i);
-      if (in_place && bits == 15u && !(h.x | h.y | h.z | h.w)) continue;
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
-      if (bits) load_vec(x + t, v);
-      float4 r;
-      r.x = bits & 1u ? apply(v[0], h.x, rules) : -INFINITY;
-      r.y = bits & 2u ? apply(v[1], h.y, rules) : -INFINITY;
-      r.z = bits & 4u ? apply(v[2], h.z, rules) : -INFINITY;
-      r.w = bits & 8u ? apply(v[3], h.w, rules) : -INFINITY;
-      *reinterpret_cast<float4*>(out + t) = r;
+  for (int i0 = threadIdx.x; i0 < n4;) {
+#pragma unroll
+    for (int u = 0; u < LG_AHEAD; ++u) {
+      const int i = i0 + u * LG_THREADS, t = v0 + 4 * i;
+      if (i >= n4) break;
+      const unsigned bits = (words[u] >> (t & 31)) & 15u;
+      unsigned h[4] = {0, 0, 0, 0};
+      if (hashed) Count<H>::load(hist + 4 * i, h);
+      if (in_place) {
+        if (bits == 15u && !(h[0] | h[1] | h[2] | h[3])) continue;
+        ahead[u] = fetch(x + t);
+      }
+      float v[4];
+      floats(ahead[u], v);
+      if (h[0] | h[1] | h[2] | h[3]) {  // few groups hold a token of the history
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = apply<SEEN>(v[k], h[k], rules);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = bits >> k & 1u ? v[k] : -INFINITY;
+      *reinterpret_cast<float4*>(out + t) = make_float4(v[0], v[1], v[2], v[3]);
     }
+    i0 += LG_AHEAD * LG_THREADS;
+    load_ahead(i0);
   }
   for (int t = v0 + (VEC ? (v1 - v0) / 4 * 4 : 0) + threadIdx.x; t < v1; t += LG_THREADS) {
     const bool ok = !mask || (__ldg(mask + (t >> 5)) >> (t & 31)) & 1u;
     const unsigned h = hashed ? hist[t - v0] : 0u;
     if (in_place && ok && !h) continue;
-    out[t] = ok ? apply(to_f(x[t]), h, rules) : -INFINITY;
+    out[t] = ok ? apply<SEEN>(to_f(x[t]), h, rules) : -INFINITY;
   }
 
   if (a.bias_start) {
@@ -149,12 +230,13 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(LogitsArgs a, int sl
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += LG_THREADS) {
       const int t = ids[i];
-      if (t >= v0 && t < v1) atomicMax(hist + (t - v0), (unsigned)(n - i));
+      if (t >= v0 && t < v1) Count<H>::raise(hist + (t - v0), (unsigned)(n - i));
     }
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += LG_THREADS) {
       const int t = ids[i];
-      if (t >= v0 && t < v1 && (hist[t - v0] & ~SEEN) != (unsigned)(n - i)) atomicOr(hist + (t - v0), SEEN);
+      if (t >= v0 && t < v1 && (hist[t - v0] & ~SEEN) != (unsigned)(n - i))
+        Count<H>::mark(hist + (t - v0));
     }
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += LG_THREADS) {
@@ -170,25 +252,29 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(LogitsArgs a, int sl
   }
 }
 
-template <typename T>
+template <typename T, typename H>
 int launch(const LogitsArgs& a, cudaStream_t s) {
-  // CTAs per row: 8 while the rows alone do not fill the GPU or a row's slice would not leave room for three CTAs an SM
-  // (64 KB of counts), fewer for small vocabularies, whose slices would be a few loads a thread.
+  // CTAs per row: 8, fewer for small vocabularies, whose slices would be a few loads a thread.
   int ranks = 8;
-  while (ranks > 1 && a.vocab <= ranks * 2 * LG_THREADS) ranks >>= 1;
+  while (ranks > 1 && a.vocab <= ranks * 8 * LG_THREADS) ranks >>= 1;
   const int slice = ((a.vocab + ranks - 1) / ranks + 31) / 32 * 32;
-  if ((size_t)slice * 4 > LG_SMEM_MAX) return kTooLarge;
+  if ((size_t)slice * 4 > LG_SMEM_MAX) return kTooLarge;  // by the wider count, whichever is used
   if ((long long)a.rows * ranks > 0x7fffffffLL) return kTooLarge;
-  const size_t smem = a.past || a.bias_start ? (size_t)slice * 4 : 0;
+  const size_t smem = a.past || a.bias_start ? (size_t)slice * sizeof(H) : 0;
   const bool in_place = (const void*)a.out == a.x;
   const bool vec = (uintptr_t)a.x % (4 * sizeof(T)) == 0 && (uintptr_t)a.out % 16 == 0 &&
                    (a.rows == 1 || (a.x_stride % 4 == 0 && a.out_stride % 4 == 0));
-  auto kernel = vec ? logits_kernel<T, true> : logits_kernel<T, false>;
+  auto kernel = vec ? logits_kernel<T, H, true> : logits_kernel<T, H, false>;
   if (allow_smem(kernel, smem)) return kCudaError;
   return launch_cluster_pdl(kernel, dim3(a.rows * ranks), dim3(LG_THREADS), ranks, smem, s, a, slice, in_place) ==
                  cudaSuccess
              ? kOk
              : kCudaError;
+}
+
+template <typename T>
+int launch(const LogitsArgs& a, cudaStream_t s) {
+  return a.past_cap > 32767 || a.n_bias > 32767 ? launch<T, uint32_t>(a, s) : launch<T, uint16_t>(a, s);
 }
 
 }  // namespace

@@ -822,6 +822,9 @@ int launch_tile(const LoraArgs& a, cudaStream_t s) {
 
 template <typename W, int LG>
 int launch(const LoraArgs& a, cudaStream_t s) {
+  // A cluster per row up to 256 rows: 0.16 us a row of rank 64 (0.06 of rank 16; k = n = 4096), whatever adapters the
+  // rows use.  Tiles take 29 us (20) for 64 to 256 rows of runs and 38 (27) for 1024, but 130 (75) where every row has
+  // an adapter of its own, which only the device knows: 256 rows of rank 64 are 41 us against 29 or 132.
   return a.rows <= 256 ? launch_row<W, LG>(a, s) : launch_tile<W, LG>(a, s);
 }
 

@@ -235,34 +235,34 @@ class LlmSampler:
 _FLOAT_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-def _call(fn, what: str, device: torch.device, stream, *args):
-    """fn(*args, stream) on `device`, whichever device is current; the stream defaults to that device's current one."""
-    if device.index == torch.cuda.current_device():
-        s = torch._C._cuda_getCurrentRawStream(device.index) if stream is None else stream.cuda_stream
-        rc = fn(*args, s)
+def _call(fn, what: str, device: int, stream, *args):
+    """fn(*args, stream) on CUDA device `device`, whichever is current; the stream defaults to that device's current one."""
+    if device == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream)
     else:
         with torch.cuda.device(device):
-            s = torch.cuda.current_stream() if stream is None else stream
-            rc = fn(*args, s.cuda_stream)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream)
     if rc:
         check(rc, what)
 
 
-def _arg(what: str, t, dtype, device, shape=None):
-    """The address of a contiguous CUDA tensor of that type (None: NULL) and, if given, shape."""
+def _arg(what: str, t, dtype, device: int, shape=None):
+    """The address of a contiguous tensor on that CUDA device, of that type and, if given, shape (None: NULL)."""
     if t is None:
         return None
-    if t.dtype is not dtype or t.device != device or not t.is_contiguous() or (shape is not None and t.shape != shape):
-        raise ZcError(f"{what} must be a contiguous {dtype} tensor on {device}"
+    if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous() or \
+            (shape is not None and t.shape != shape):
+        raise ZcError(f"{what} must be a contiguous {dtype} tensor on cuda:{device}"
                       f"{'' if shape is None else f' of shape {tuple(shape)}'}, got {t.dtype} {tuple(t.shape)} "
                       f"on {t.device}")
     return t.data_ptr()
 
 
-def _cuda(what: str, t) -> torch.device:
-    if not (torch.is_tensor(t) and t.is_cuda):
+def _cuda(what: str, t) -> int:
+    """The index of the CUDA device that a tensor is on."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
         raise ZcError(f"{what} must be a CUDA tensor")
-    return t.device
+    return t.get_device()
 
 
 def _pool_args(page_table, seq_len, free_pages, free_count, page_size):
@@ -305,7 +305,7 @@ def reserve_pages(page_table, seq_len, free_pages, free_count, n_new, page_size:
     if out is None:
         if tokens is None:
             raise ZcError("reserve_pages needs tokens, the length of the step's token arrays, or out")
-        out = PagePlan.empty(batch, tokens, dev)
+        out = PagePlan.empty(batch, tokens, page_table.device)
     start, slots, positions, token_rows, ctx_len, granted = out
     n = slots.shape[0]
     if tokens is not None and tokens != n:
@@ -331,15 +331,14 @@ def trim_pages(page_table, seq_len, free_pages, free_count, new_len, page_size: 
 def _kv_pools(k_pool, v_pool, dev):
     """(dtype code, pages, hkv, page size, hd, page / slot / head stride) of pools [pages, hkv, page size, hd], any
     strides with contiguous heads; a [pages, page size, hkv, hd] pool is passed as pool.transpose(1, 2)."""
-    if k_pool.dim() != 4 or k_pool.shape != v_pool.shape or k_pool.stride() != v_pool.stride():
+    shape, strides = k_pool.shape, k_pool.stride()
+    if len(shape) != 4 or shape != v_pool.shape or strides != v_pool.stride():
         raise ZcError("k_pool and v_pool must be [pages, kv heads, page size, head size] with the same strides")
     if k_pool.dtype not in (torch.float32, torch.float16) or v_pool.dtype != k_pool.dtype:
         raise ZcError("k_pool and v_pool must be fp32 or fp16")
-    if k_pool.device != dev or v_pool.device != dev or k_pool.stride(3) != 1:
-        raise ZcError(f"k_pool and v_pool must be on {dev} with contiguous heads")
-    n, hkv, page, hd = k_pool.shape
-    sp, sh, ss, _ = k_pool.stride()
-    return _FLOAT_CODE[k_pool.dtype], n, hkv, page, hd, sp, ss, sh
+    if k_pool.get_device() != dev or v_pool.get_device() != dev or strides[3] != 1:
+        raise ZcError(f"k_pool and v_pool must be on cuda:{dev} with contiguous heads")
+    return _FLOAT_CODE[k_pool.dtype], *shape, strides[0], strides[2], strides[1]
 
 
 def append_kv(k, v, slots, k_pool, v_pool, bounds=None, scales=None, stream=None) -> None:
@@ -349,16 +348,16 @@ def append_kv(k, v, slots, k_pool, v_pool, bounds=None, scales=None, stream=None
     pages by (zcu_append_kv)."""
     dev = _cuda("k", k)
     code, pages, hkv, page, hd, sp, ss, sh = _kv_pools(k_pool, v_pool, dev)
-    if k.shape != v.shape or k.dim() != 3 or k.shape[1:] != (hkv, hd) or k.dtype != v.dtype or v.device != dev:
+    shape, ks, vs = k.shape, k.stride(), v.stride()
+    if len(shape) != 3 or shape != v.shape or shape[1:] != (hkv, hd) or k.dtype != v.dtype or v.get_device() != dev:
         raise ZcError(f"k and v must both be [tokens, {hkv}, {hd}] of one type on one device")
     if k.dtype not in (torch.float32, torch.float16):
         raise ZcError("k and v must be fp32 or fp16")
-    tokens = k.shape[0]
-    for name, t in (("k", k), ("v", v)):
-        if t.stride(2) != 1 or (hkv > 1 and t.stride(1) != hd):
-            raise ZcError(f"{name}'s heads must be contiguous")
-    _call(lib().zcu_append_kv, "append_kv", dev, stream, k.data_ptr(), v.data_ptr(), _FLOAT_CODE[k.dtype], k.stride(0),
-          v.stride(0), _arg("slots", slots, torch.int64, dev, (tokens,)), tokens, k_pool.data_ptr(),
+    if ks[2] != 1 or vs[2] != 1 or (hkv > 1 and (ks[1] != hd or vs[1] != hd)):
+        raise ZcError("the heads of k and v must be contiguous")
+    tokens = shape[0]
+    _call(lib().zcu_append_kv, "append_kv", dev, stream, k.data_ptr(), v.data_ptr(), _FLOAT_CODE[k.dtype], ks[0],
+          vs[0], _arg("slots", slots, torch.int64, dev, (tokens,)), tokens, k_pool.data_ptr(),
           v_pool.data_ptr(), code, hkv, hd, page, pages, sp, ss, sh,
           _arg("bounds", bounds, torch.int8, dev, (pages, hkv, 2, hd)),
           _arg("scales", scales, torch.float32, dev, (pages, hkv)))
@@ -376,10 +375,11 @@ def sparse_paged_attention(q, k_pool, v_pool, bounds, scales, page_table, ctx_le
     hd], sel [batch, hkv, budget]: the chosen pages as indices into the table row, ascending, -1 behind them)."""
     dev = _cuda("q", q)
     code, pages, hkv, page, hd, sp, ss, sh = _kv_pools(k_pool, v_pool, dev)
-    if q.dim() != 3 or q.dtype is not torch.float32 or q.shape[2] != hd or \
-            (q.numel() and (q.stride(2) != 1 or (q.shape[1] > 1 and q.stride(1) != hd))):
+    shape, qs = q.shape, q.stride()
+    if len(shape) != 3 or q.dtype is not torch.float32 or shape[2] != hd or \
+            (q.numel() and (qs[2] != 1 or (shape[1] > 1 and qs[1] != hd))):
         raise ZcError(f"q must be [batch, hq, {hd}] fp32 with contiguous heads")
-    batch, hq, _ = q.shape
+    batch, hq, _ = shape
     if page_table.dim() != 2:
         raise ZcError("page_table must be [rows, max_pages]")
     table_rows, max_pages = page_table.shape
@@ -389,10 +389,10 @@ def sparse_paged_attention(q, k_pool, v_pool, bounds, scales, page_table, ctx_le
         max_ctx = min(max_pages * page, 0x7fffffff)
     i, f = torch.int32, torch.float32
     if out is None:
-        out = torch.empty((batch, hq, hd), dtype=f, device=dev)
+        out = torch.empty((batch, hq, hd), dtype=f, device=q.device)
     if sel is None:
-        sel = torch.empty((batch, hkv, budget), dtype=i, device=dev)
-    _call(lib().zcu_sparse_paged_attention, "sparse_paged_attention", dev, stream, q.data_ptr(), q.stride(0),
+        sel = torch.empty((batch, hkv, budget), dtype=i, device=q.device)
+    _call(lib().zcu_sparse_paged_attention, "sparse_paged_attention", dev, stream, q.data_ptr(), qs[0],
           k_pool.data_ptr(), v_pool.data_ptr(), code, _arg("bounds", bounds, torch.int8, dev, (pages, hkv, 2, hd)),
           _arg("scales", scales, f, dev, (pages, hkv)), _arg("page_table", page_table, i, dev), table_rows,
           _arg("rows", rows, i, dev, (batch,)), _arg("ctx_len", ctx_len, i, dev, (batch,)),
@@ -415,14 +415,15 @@ def lora_add(y, x, a, b, adapter, ranks=None, scales=None, out=None, stream=None
         raise ZcError("x and y must be matrices, a and b stacks of matrices")
     rows, n = y.shape
     na, rank, k = a.shape
-    for name, t, shape in (("x", x, (rows, k)), ("y", y, (rows, n)), ("out", out, (rows, n))):
-        if t.shape != shape or t.dtype is not torch.float32 or t.device != dev or (t.numel() and t.stride(1) != 1):
-            raise ZcError(f"{name} must be {list(shape)} fp32 on {dev} with contiguous rows")
+    xs, ys, os = x.stride(), y.stride(), out.stride()
+    for name, t, shape, st in (("x", x, (rows, k), xs), ("y", y, (rows, n), ys), ("out", out, (rows, n), os)):
+        if t.shape != shape or t.dtype is not torch.float32 or t.get_device() != dev or (st[1] != 1 and t.numel()):
+            raise ZcError(f"{name} must be {list(shape)} fp32 on cuda:{dev} with contiguous rows")
     if a.dtype not in _FLOAT_CODE:
         raise ZcError("a and b must be fp32, fp16 or bf16")
     i, f = torch.int32, torch.float32
-    _call(lib().zcu_lora_add, "lora_add", dev, stream, x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0),
-          out.data_ptr(), out.stride(0), _arg("a", a, a.dtype, dev), _arg("b", b, a.dtype, dev, (na, n, rank)),
+    _call(lib().zcu_lora_add, "lora_add", dev, stream, x.data_ptr(), xs[0], y.data_ptr(), ys[0],
+          out.data_ptr(), os[0], _arg("a", a, a.dtype, dev), _arg("b", b, a.dtype, dev, (na, n, rank)),
           _FLOAT_CODE[a.dtype], _arg("adapter", adapter, i, dev, (rows,)), _arg("ranks", ranks, i, dev, (na,)),
           _arg("scales", scales, f, dev, (na,)), rows, k, n, na, rank)
     return out
@@ -440,14 +441,16 @@ def process_logits(logits, out=None, past=None, past_len=None, prompt_len=None, 
     the prompt, each [rows] fp32.  bias_start [rows + 1], bias_ids, bias: each row's biased tokens.  mask [m, words]
     int32: bit t % 32 of word t / 32 allows token t; row r uses mask_rows[r] (None: r; outside: unmasked)."""
     dev = _cuda("logits", logits)
-    if logits.dim() != 2 or logits.dtype not in _FLOAT_CODE or (logits.numel() and logits.stride(1) != 1):
+    code, xs = _FLOAT_CODE.get(logits.dtype), logits.stride()
+    if len(xs) != 2 or code is None or (xs[1] != 1 and logits.numel()):
         raise ZcError("logits must be [rows, vocab] fp32, fp16 or bf16 with contiguous rows")
     rows, vocab = logits.shape
     if out is None:
-        out = logits if logits.dtype is torch.float32 else torch.empty((rows, vocab), dtype=torch.float32, device=dev)
-    if out.shape != logits.shape or out.dtype is not torch.float32 or out.device != dev or \
-            (out.numel() and out.stride(1) != 1):
-        raise ZcError(f"out must be [{rows}, {vocab}] fp32 on {dev} with contiguous rows")
+        out = torch.empty((rows, vocab), dtype=torch.float32, device=logits.device) if code else logits
+    os = out.stride()
+    if out.shape != (rows, vocab) or out.dtype is not torch.float32 or out.get_device() != dev or \
+            (os[1] != 1 and out.numel()):
+        raise ZcError(f"out must be [{rows}, {vocab}] fp32 on cuda:{dev} with contiguous rows")
     i, f, at = torch.int32, torch.float32, (rows,)
     n, cap = (0, 0) if past is None else past.shape
     masks, words = (0, 0) if mask is None else mask.shape
@@ -462,6 +465,6 @@ def process_logits(logits, out=None, past=None, past_len=None, prompt_len=None, 
                     _arg("presence", presence, f, dev, at), _arg("bias_start", bias_start, i, dev, (rows + 1,)),
                     _arg("bias_ids", bias_ids, i, dev, (n_bias,)), _arg("bias", bias, f, dev), n_bias, masks,
                     _arg("mask", mask, i, dev), _arg("mask_rows", mask_rows, i, dev, at), words)
-    _call(lib().zcu_process_logits, "process_logits", dev, stream, logits.data_ptr(), _FLOAT_CODE[logits.dtype],
-          logits.stride(0), out.data_ptr(), out.stride(0), rows, vocab, C.byref(r))
+    _call(lib().zcu_process_logits, "process_logits", dev, stream, logits.data_ptr(), code,
+          xs[0], out.data_ptr(), os[0], rows, vocab, C.byref(r))
     return out
