@@ -401,7 +401,8 @@ ZC_API int32_t zcu_append_kv(const void* k, const void* v, int32_t in_dtype, int
  * s_q = max|q| / 32512 and qi = rint(q / s_q): whole numbers summed exactly and two fp32 products, so the choice
  * does not depend on the launch; the lower page wins among equal scores.
  * hd 64, 128 or 256, page_size a multiple of 8 (else -4); -6 when a CTA's shared memory does not hold the scores of
- * max_ctx tokens (about 50,000 pages). */
+ * max_ctx tokens and its part of the budget (46,000 pages at hd 64, 35,000 at 128, 15,000 at 256), or when max_ctx and a
+ * page pass 2^30 tokens. */
 ZC_API int32_t zcu_sparse_paged_attention(const float* q, int64_t q_stride, const void* k_pool, const void* v_pool,
                                           int32_t kv_dtype, const int8_t* bounds, const float* scales,
                                           const int32_t* page_table, int32_t table_rows, const int32_t* rows,
@@ -415,8 +416,9 @@ ZC_API int32_t zcu_sparse_paged_attention(const float* q, int64_t q_stride, cons
  *   out[r] = y[r] + scales[e] * (x[r] A_e^T) B_e^T,  e = adapter[r];  a row whose adapter is outside [0, adapters): y[r]
  * x [rows][k_cols], y and out [rows][n_rows] fp32 with strides in elements; out may be y itself (no other overlap).
  * a [adapters][rank][k_cols] and b [adapters][n_rows][rank] (w_dtype 0 = fp32, 1 = fp16, 2 = bf16); of adapter e the
- * first ranks[e] of `rank` are used (NULL: all), scales NULL: 1.  fp32 arithmetic, or tf32 hi + lo pairs on the tensor
- * cores for many rows (about 2^-22); a row's result does not depend on the other rows' adapters.
+ * first ranks[e] of `rank` are used (NULL: all), scales NULL: 1.  fp32 arithmetic up to
+ * 256 rows, beyond on the tensor cores with x and x A^T split into terms that hold fp32 to 2^-22; what another row or its
+ * adapter holds, NaN included, does not reach a row.
  * rank a multiple of 8 up to 128, k_cols a multiple of 32 (else -4); x, a and b 16-byte aligned, x_stride a multiple
  * of 4. */
 ZC_API int32_t zcu_lora_add(const float* x, int64_t x_stride, const float* y, int64_t y_stride, float* out,
@@ -437,7 +439,7 @@ ZC_API int32_t zcu_lora_add(const float* x, int64_t x_stride, const float* y, in
  *   bias_start [rows + 1]: row r's entries of bias_ids / bias [n_bias]; a token named twice gets both, in list order
  *   mask [masks][mask_stride] 32-bit words, bit t % 32 of word t / 32 set = allowed; row r reads mask mask_rows[r]
  *     (NULL: r; outside [0, masks): unmasked)
- * -6 for a vocab above 409,600. */
+ * -6 for a vocab above 409,600, or a past_cap or n_bias above 2^30. */
 typedef struct {
   const int32_t *past, *past_len, *prompt_len, *past_rows;
   int32_t past_cap, past_count;

@@ -718,3 +718,171 @@ def test_logits_refuse():
         ops.process_logits(x.double())
     with pytest.raises(ZcError):
         ops.process_logits(x.t())
+
+
+# ---------------------------------------------------------------------------------------------------------
+# the operators together
+# ---------------------------------------------------------------------------------------------------------
+
+
+class Step:
+    """A small model's serving step over the operators: plan, projection with adapters, append, sparse attention, head,
+    rules, greedy token.  Every buffer is kept, so that a captured step replays on changed contents."""
+
+    def __init__(self, rng, batch, tokens, hq=4, hkv=2, hd=64, k=128, vocab=600, page=16, max_pages=12, budget=4):
+        self.hq, self.hkv, self.hd, self.page, self.budget, self.vocab = hq, hkv, hd, page, budget, vocab
+        n = (hq + 2 * hkv) * hd
+        self.host = Pool(rng, batch + 2, max_pages, batch * max_pages, page)
+        self.pool = upload(self.host)
+        f = lambda *s: dev(rng.standard_normal(s).astype(np.float32))  # noqa: E731
+        self.w, self.head = f(n, k) / k ** 0.5, f(vocab, hq * hd) / (hq * hd) ** 0.5
+        self.a, self.b = (f(3, 8, k) / k ** 0.5).half(), (f(3, n, 8) / 8 ** 0.5).half()
+        self.kv = [torch.zeros((batch * max_pages, hkv, page, hd), dtype=torch.float16, device="cuda") for _ in "kv"]
+        self.bounds = torch.zeros((batch * max_pages, hkv, 2, hd), dtype=torch.int8, device="cuda")
+        self.scales = torch.zeros((batch * max_pages, hkv), device="cuda")
+        self.new, self.rows = ints([0] * batch), ints(rng.permutation(batch + 2)[:batch])
+        self.plan = ops.PagePlan.empty(batch, tokens)
+        self.x, self.adapter = torch.zeros((tokens, k), device="cuda"), ints([-1] * tokens)
+        self.past = torch.zeros((batch + 2, 200), dtype=torch.int32, device="cuda")
+        self.past_len = ints([0] * (batch + 2))
+        self.rep = torch.full((tokens,), 1.3, device="cuda")
+        self.freq, self.pres = torch.full((tokens,), 0.2, device="cuda"), torch.full((tokens,), 0.1, device="cuda")
+        self.mask = torch.full((1, (vocab + 31) // 32), -1, dtype=torch.int32, device="cuda")
+        self.mask[0, 3] = 0
+        self.mask_rows = ints([0] * tokens)
+
+    def __call__(self):
+        ops.reserve_pages(*self.pool, self.new, self.page, rows=self.rows, out=self.plan)
+        qkv = ops.lora_add(self.x @ self.w.t(), self.x, self.a, self.b, self.adapter)
+        q, k, v = qkv.split([self.hq * self.hd, self.hkv * self.hd, self.hkv * self.hd], 1)
+        ops.append_kv(k.unflatten(1, (self.hkv, self.hd)), v.unflatten(1, (self.hkv, self.hd)), self.plan.slots,
+                      *self.kv, self.bounds, self.scales)
+        out, sel = ops.sparse_paged_attention(q.unflatten(1, (self.hq, self.hd)), *self.kv, self.bounds, self.scales,
+                                              self.pool[0], self.plan.ctx_len, self.budget,
+                                              rows=self.plan.token_rows)
+        raw = out.flatten(1) @ self.head.t()
+        logits = ops.process_logits(raw, out=torch.empty_like(raw), past=self.past, past_len=self.past_len,
+                                    past_rows=self.plan.token_rows, repetition=self.rep, frequency=self.freq,
+                                    presence=self.pres, mask=self.mask, mask_rows=self.mask_rows)
+        token = ops.LlmSampler.sample(logits.clone(), temperature=0.0, repetition_penalty=1.0)
+        return qkv, out, sel, raw, logits, token
+
+    def check(self, got, new, x, adapter):
+        """The step's results against the host, stage by stage on the stage's own inputs."""
+        qkv, out, sel, raw, logits, token = (t.cpu() for t in got)
+        rows = self.rows.tolist()
+        want = self.host.reserve(rows, new, len(self.plan.slots))
+        same_plan(self.plan, want)
+        same_pool(self.host, self.pool)
+        y = (dev(x) @ self.w.t()).cpu().numpy()
+        ref, mag = plain_lora(x, y, self.a.cpu(), self.b.cpu(), adapter, [8] * 3, [1.0] * 3)
+        assert (np.abs(qkv.numpy() - ref) <= (64 * 2.0 ** -23 + 2.0 ** -21) * mag).all()
+        kv = [t.cpu().numpy() for t in self.kv]
+        cut = self.hq * self.hd, (self.hq + self.hkv) * self.hd
+        for t, s in enumerate(want[1]):
+            if s >= 0:
+                for i, part in enumerate((qkv[t, cut[0]:cut[1]], qkv[t, cut[1]:])):
+                    np.testing.assert_array_equal(kv[i][s // self.page, :, s % self.page],
+                                                  part.half().numpy().reshape(self.hkv, self.hd))
+        codes, scales = self.bounds.cpu().numpy(), self.scales.cpu().numpy()
+        for r in rows:
+            for c in range(-(-int(self.host.lens[r]) // self.page)):
+                p, held = self.host.table[r, c], min(self.page, int(self.host.lens[r]) - c * self.page)
+                for have, ref in zip((codes[p], scales[p]), key_bounds(kv[0][p, :, :held])):
+                    np.testing.assert_array_equal(have, ref)
+        q = qkv[:, :cut[0]].numpy().reshape(-1, self.hq, self.hd)
+        check_sparse(q, *kv, codes, scales, self.host.table, want[4], self.budget, 1, 1, out, sel, rows=want[3])
+        past = self.past.cpu().numpy(), self.past_len.cpu().numpy()
+        zero = np.zeros_like(past[1])
+        ref, mag = plain_logits(raw.numpy(), *past, zero, want[3], *(t.cpu().numpy() for t in (
+            self.rep, self.freq, self.pres)), None, self.mask.cpu().numpy(), [0] * len(q))
+        fine = np.isfinite(ref)
+        np.testing.assert_array_equal(np.isfinite(logits.numpy()), fine)
+        assert (np.abs(logits.numpy() - ref)[fine] <= 8 * 2.0 ** -24 * mag[fine]).all()
+        assert (token.numpy() == logits.numpy().argmax(1)).all()
+        return want
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_steps_of_a_mixed_batch(captured):
+    """Prompts of different lengths, then decode steps of one to three tokens with rejected drafts and finished requests;
+    the same steps eagerly and as replays of one captured graph."""
+    rng = np.random.default_rng(31)
+    batch, tokens = 6, 96
+    step = Step(rng, batch, tokens)
+    graph = got = None
+    if captured:
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            step()  # no request adds a token
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+    plans = [[40, 3, 0, 17, 1, 30]] + [[1, 1, 2, 1, 3, 1], [1] * 6, [16, 1, 0, 1, 1, 20], [1, 3, 70, 2, 1, 0]]
+    for i, new in enumerate(plans):
+        x = rng.standard_normal((tokens, 128)).astype(np.float32)
+        adapter = rng.integers(-1, 3, tokens).astype(np.int32)
+        step.x.copy_(dev(x))
+        step.adapter.copy_(dev(adapter))
+        step.new.copy_(ints(new))
+        if captured:
+            graph.replay()
+        else:
+            got = step()
+        want = step.check(got, new, x, adapter)
+        # the sampled token of each request's last row joins its history
+        token = got[-1].tolist()
+        for b, r in enumerate(step.rows.tolist()):
+            if new[b] and want[5][b]:
+                n = int(step.past_len[r])
+                step.past[r, n] = token[want[0][b + 1] - 1]
+                step.past_len[r] = n + 1
+        # two drafts of request 4 are rejected after the second step; request 0 ends after the fourth
+        keep = step.host.lens[step.rows.tolist()].copy()
+        if i == 1:
+            keep[4] -= 2
+        if i == 3:
+            keep[0] = 0
+        ops.trim_pages(*step.pool, ints(keep), step.page, rows=step.rows)
+        step.host.trim(step.rows.tolist(), keep)
+        same_pool(step.host, step.pool)
+
+
+def test_operators_on_two_streams_at_once():
+    """Two steps on streams of their own, interleaved call by call, give what each gives alone."""
+    def make(seed):
+        rng = np.random.default_rng(seed)
+        s = Step(rng, 5, 64)
+        s.x.copy_(dev(rng.standard_normal((64, 128)).astype(np.float32)))
+        s.adapter.copy_(ints(rng.integers(-1, 3, 64)))
+        s.new.copy_(ints([20, 1, 7, 30, 3]))
+        return s
+
+    alone = [[t.clone() for t in make(seed)()] for seed in (41, 42)]
+    both, streams, got = [make(41), make(42)], [torch.cuda.Stream(), torch.cuda.Stream()], [None, None]
+    torch.cuda.synchronize()
+    for turn in range(3):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                if turn:  # take the last turn back, so that every turn is the first again
+                    ops.trim_pages(*both[i].pool, torch.zeros_like(both[i].new), both[i].page, rows=both[i].rows)
+                got[i] = both[i]()
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for a, b in zip(alone[i], got[i]):
+            assert torch.equal(a, b)
+
+
+def test_operators_when_another_device_is_current(monkeypatch):
+    """The call goes to the tensors' device, on its current stream, whichever device is current."""
+    seen = []
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: seen.append(1) or -1)
+    x = torch.randn((2, 100), device="cuda")
+    assert torch.equal(ops.process_logits(x.half()), x.half().float())
+    assert seen
+    if torch.cuda.device_count() > 1:
+        monkeypatch.undo()
+        y = torch.randn((2, 100), device="cuda:1", dtype=torch.float16)
+        assert torch.cuda.current_device() == 0 and torch.equal(ops.process_logits(y), y.float())

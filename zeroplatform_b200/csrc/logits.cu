@@ -282,6 +282,7 @@ int launch(const LogitsArgs& a, cudaStream_t s) {
 int process_logits(const LogitsArgs& a, cudaStream_t s) {
   if (a.rows < 0 || a.vocab <= 0 || a.x_type < 0 || a.x_type > 2) return kBadArgument;
   if (a.rows == 0) return kOk;
+  if (a.past_cap > 1 << 30 || a.n_bias > 1 << 30) return kTooLarge;
   if (!a.x || !a.out) return kBadArgument;
   if (a.rows > 1 && (a.x_stride < a.vocab || a.out_stride < a.vocab)) return kBadArgument;
   if (a.past && (!a.past_len || a.past_cap < 0 || a.past_count <= 0)) return kBadArgument;

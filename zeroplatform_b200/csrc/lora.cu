@@ -6,16 +6,19 @@
 // fp32, fp16 or bf16, and adapters whose own rank is below the stored one.  Both products in one launch: a cluster of
 // up to 8 CTAs owns a row (or a tile of rows), splits k for the first product, sums the partial t = x A^T through
 // distributed shared memory in a fixed order, and splits n for the second.  t never leaves the chip, there is no
-// scratch in memory, and no atomics: the result does not depend on what shares the batch.
+// scratch in memory and no atomics on results: the same call gives the same bits.
 //
-// lora_row_kernel (few rows, as in decode): fp32 arithmetic, one cluster per row.  A warp's lanes read along k, a row of
-//   B is read by rank / 8 lanes, and the first rows of B are on their way before the cluster has summed t.  Bound: the
-//   adapters' bytes (each row reads its own; rows that share an adapter meet in L2), at small sizes the chain
-//   A -> t -> B of one launch.
+// lora_row_kernel (few rows, as in decode): fp32 arithmetic, one cluster per row.  A warp's lanes read along k, a row
+//   of B is read by rank / 8 lanes, and the first rows of B are on their way before the cluster has summed t.  Bound:
+//   the adapters' bytes from L2 (each row reads its own; rows that share an adapter meet there), at small sizes the
+//   chain A -> t -> B of one launch.  k = n = 4096: one row of rank 16 4.1 us; 64 rows of rank 64 12.6 us, 64 MB from
+//   L2 at 5.3 TB/s.
 // lora_tile_kernel (many rows, as in prefill): 64 rows per cluster on the tensor cores (mma.sync), x and t split into
-//   terms of the weights' type that hold fp32 to 2^-22 (Step).  x and A, then y and
-//   B, pass through one cp.async ring, whose second filling starts before the cluster has summed t.  The adapter that most of a tile's rows name is staged; warps whose rows name others fetch those weights themselves.  Bound: x, y and out once
-//   through HBM, or the tensor pipe at large ranks.
+//   terms of the weights' type that hold fp32 to 2^-22 (Step).  x and A, then y and B, pass through one cp.async ring,
+//   whose second filling starts before the cluster has summed t.  The adapter that most of a tile's rows name is
+//   staged; warps whose rows name others fetch those weights themselves, the first one's a turn ahead.  2048 rows of
+//   rank 64 and one adapter, k = n = 4096: fp16 47 us, 2.1 TB/s of x, y and out; bound by the instructions and barriers
+//   of a turn (about 300 per warp and 64 columns, 14 warps an SM), not by HBM (16 us) or the tensor pipe (9 us).
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>

@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(PG_THREADS) reserve_kernel(PagePool p, const i
     const int old = r >= 0 ? max(p.len[r], 0) : 0;
     q.start[b] = (int)min(at, (long long)0x7fffffff);
     at += n;
-    const bool fits = r >= 0 && (long long)old + n <= (long long)p.max_pages * P && at <= tokens;
+    const bool fits = r >= 0 && (long long)old + n <= min((long long)p.max_pages * P, 0x7fffffffLL) && at <= tokens;
     const int have = pages_of(old, P);
     q.old[b] = old;
     q.first[b] = fits ? have : -1;
@@ -171,14 +171,15 @@ __global__ void __launch_bounds__(PG_THREADS) reserve_kernel(PagePool p, const i
   const int tid = rank * PG_THREADS + threadIdx.x, step = ranks * PG_THREADS;
   // new pages into the tables: the i-th page popped belongs to the last request whose poff is <= i.  A refused
   // request's poff is at least `used`, a request without new pages is followed by one with the same poff.
-  for (int i = tid; i < used; i += step) {
-    const int b = find(q.poff, batch, i);
+  for (unsigned i = tid; i < (unsigned)used; i += step) {
+    const int b = find(q.poff, batch, (int)i);
     p.table[(size_t)q.row[b] * p.max_pages + q.first[b] + (i - q.poff[b])] = p.free_list[count - 1 - i];
   }
   // Four tokens a thread: one search, and a page looked up when it changes.
   const bool wide = ((uintptr_t)o.slots | (uintptr_t)o.positions | (uintptr_t)o.token_rows | (uintptr_t)o.ctx_len) % 16 == 0;
   const int all = q.start[batch];
-  for (int t = 4 * tid; t < tokens; t += 4 * step) {
+  for (unsigned u = 4 * tid; u < (unsigned)tokens; u += 4 * step) {  // unsigned: 2^31 and a step do not wrap
+    const int t = (int)u;
     int64_t slot[4];
     int pos[4], row[4], ctx[4];
     int b = t < all ? find(q.start, batch, t) : batch, col = -1, page = 0;
@@ -186,7 +187,7 @@ __global__ void __launch_bounds__(PG_THREADS) reserve_kernel(PagePool p, const i
     for (int i = 0; i < 4; ++i) {
       slot[i] = -1;
       pos[i] = 0, row[i] = -1, ctx[i] = 0;
-      while (b < batch && t + i >= q.start[b + 1]) ++b, col = -1;  // requests without tokens are passed over
+      while (b < batch && u + i >= (unsigned)q.start[b + 1]) ++b, col = -1;  // requests without tokens are passed over
       if (b == batch || q.first[b] < 0) continue;
       pos[i] = q.old[b] + (t + i - q.start[b]);
       row[i] = q.row[b];
@@ -198,14 +199,14 @@ __global__ void __launch_bounds__(PG_THREADS) reserve_kernel(PagePool p, const i
       }
       slot[i] = (int64_t)page * P + (pos[i] - col * P);
     }
-    if (wide && t + 4 <= tokens) {
+    if (wide && u + 4 <= (unsigned)tokens) {
       *reinterpret_cast<longlong2*>(o.slots + t) = make_longlong2(slot[0], slot[1]);
       *reinterpret_cast<longlong2*>(o.slots + t + 2) = make_longlong2(slot[2], slot[3]);
       *reinterpret_cast<int4*>(o.positions + t) = make_int4(pos[0], pos[1], pos[2], pos[3]);
       *reinterpret_cast<int4*>(o.token_rows + t) = make_int4(row[0], row[1], row[2], row[3]);
       *reinterpret_cast<int4*>(o.ctx_len + t) = make_int4(ctx[0], ctx[1], ctx[2], ctx[3]);
     } else {
-      for (int i = 0; i < 4 && t + i < tokens; ++i) {
+      for (int i = 0; i < 4 && u + i < (unsigned)tokens; ++i) {
         o.slots[t + i] = slot[i];
         o.positions[t + i] = pos[i];
         o.token_rows[t + i] = row[i];
@@ -259,8 +260,8 @@ __global__ void __launch_bounds__(PG_THREADS) trim_kernel(PagePool p, const int3
   }
   const int tid = rank * PG_THREADS + threadIdx.x, step = ranks * PG_THREADS;
   const int moved = (int)min(total, 0x7fffffffLL);
-  for (int j = tid; j < moved; j += step) {
-    const int i = find(q.poff, batch, j), b = batch - 1 - i;
+  for (unsigned u = tid; u < (unsigned)moved; u += step) {
+    const int j = (int)u, i = find(q.poff, batch, j), b = batch - 1 - i;
     int32_t* e = p.table + (size_t)q.row[b] * p.max_pages + (q.old[b] - 1 - (j - q.poff[i]));
     if (j < back) p.free_list[count + j] = *e;
     *e = -1;

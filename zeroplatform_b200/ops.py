@@ -386,7 +386,7 @@ def sparse_paged_attention(q, k_pool, v_pool, bounds, scales, page_table, ctx_le
     if scale is None:
         scale = 1.0 / math.sqrt(hd)
     if max_ctx is None:
-        max_ctx = min(max_pages * page, 0x7fffffff)
+        max_ctx = min(max_pages * page, (1 << 30) - page)
     i, f = torch.int32, torch.float32
     if out is None:
         out = torch.empty((batch, hq, hd), dtype=f, device=q.device)
