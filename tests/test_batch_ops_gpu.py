@@ -875,6 +875,52 @@ def test_operators_on_two_streams_at_once():
             assert torch.equal(a, b)
 
 
+def test_operators_through_either_binding(monkeypatch):
+    """What _dispatch takes and what goes through ctypes (its absence, a stream argument, tensor subclasses) is the same."""
+    from zeroplatform_b200 import _lib
+
+    def make():
+        rng = np.random.default_rng(51)
+        s = Step(rng, 5, 64)
+        s.x.copy_(dev(rng.standard_normal((64, 128)).astype(np.float32)))
+        s.adapter.copy_(ints(rng.integers(-1, 3, 64)))
+        s.new.copy_(ints([20, 1, 7, 30, 3]))
+        return s
+
+    assert _lib.dispatch is not None
+    ref = [t.clone() for t in make()()]
+    x = torch.nn.Parameter(torch.randn((2, 50), device="cuda"), requires_grad=False)
+    plain = x.detach().clone()
+    assert not _lib.dispatch.process_logits(x, x, *[None] * 12)
+    assert torch.equal(ops.process_logits(x.half()), plain.half().float())
+    assert torch.equal(ops.process_logits(x), plain)
+    assert torch.equal(ops.process_logits(plain.half(), stream=torch.cuda.current_stream()), plain.half().float())
+    monkeypatch.setattr(_lib, "dispatch", None)
+    for a, b in zip(ref, make()()):
+        assert torch.equal(a, b)
+
+
+def test_dispatch_declines_what_it_must_not_take():
+    """Wrong types, shapes, devices, strides and argument counts are declined before anything is enqueued."""
+    from zeroplatform_b200 import _lib
+    d = _lib.dispatch
+    y, x = torch.zeros((2, 40), device="cuda"), torch.ones((2, 64), device="cuda")
+    a, b, e = torch.ones((1, 8, 64), device="cuda"), torch.ones((1, 40, 8), device="cuda"), ints([0, 0])
+    good = [y, x, a, b, e, None, None, y]
+    assert d.lora_add(*good)
+    torch.cuda.synchronize()
+    before = y.clone()
+    wrong = {0: [y.cpu(), y.half(), y[:1], y.t(), y[:, ::2], None, 3], 1: [x.cpu(), x[:, :32], x.double(), y],
+             2: [a.cpu(), a.transpose(1, 2), a[0], a.double(), None], 3: [b[:, :39], b.half(), None],
+             4: [e.long(), e.cpu(), ints([0]), None], 5: [e, ints([8, 8])], 6: [ints([1])], 7: [y[:1], None, y.cpu()]}
+    for i, values in wrong.items():
+        for v in values:
+            assert not d.lora_add(*good[:i], v, *good[i + 1:]), (i, v)
+    assert not d.lora_add(*good[:-1]) and not d.lora_add()
+    torch.cuda.synchronize()
+    assert torch.equal(y, before)
+
+
 def test_operators_when_another_device_is_current(monkeypatch):
     """The call goes to the tensors' device, on its current stream, whichever device is current."""
     seen = []

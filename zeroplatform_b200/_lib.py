@@ -187,7 +187,26 @@ def lib():
         fn.restype = res
         fn.argtypes = args
     _lib = L
+    _init_dispatch(L)
     return L
+
+
+dispatch = None  # the _dispatch module once the library is loaded, where it is built and PyTorch has what it needs
+
+
+def _init_dispatch(L) -> None:
+    global dispatch
+    try:
+        import torch
+
+        from . import _dispatch
+    except ImportError:  # ops.py makes the same calls through ctypes
+        return
+    at = [C.cast(getattr(L, n), vp).value for n in ("zcu_pages_reserve", "zcu_pages_trim", "zcu_append_kv",
+                                                    "zcu_sparse_paged_attention", "zcu_lora_add",
+                                                    "zcu_process_logits")]
+    if _dispatch.init(torch.Tensor, torch._C, *at):
+        dispatch = _dispatch
 
 
 def check(rc: int, what: str = "") -> None:

@@ -1,10 +1,11 @@
-"""Builds libzero_tensor.so (the C-ABI library with every CUDA kernel) in-tree for sm_100a.
+"""Builds libzero_tensor.so (the C-ABI library with every CUDA kernel) in-tree for sm_100a, and _dispatch.so (the
+CPython module beside it).
 
     python -m zeroplatform_b200.build          # incremental
     python -m zeroplatform_b200.build --clean  # from scratch
 
-nvcc cross-compiles without a GPU.  Objects go to zeroplatform_b200/_build/, the library to
-zeroplatform_b200/libzero_tensor.so (both git-ignored; the .so travels with the source tree).
+nvcc cross-compiles without a GPU.  Objects go to zeroplatform_b200/_build/, the libraries to
+zeroplatform_b200/*.so (git-ignored; the .so files travel with the source tree).
 """
 from __future__ import annotations
 
@@ -21,6 +22,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libzero_tensor.so")
+DISPATCH = os.path.join(PKG, "_dispatch.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -66,7 +68,29 @@ def build(clean: bool = False, verbose_ptxas: bool = False) -> str:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
+    build_dispatch()
     return LIB
+
+
+def build_dispatch() -> str:
+    """_dispatch.so: the CPython module that checks tensors and calls the serving-batch entries (csrc/dispatch.c)."""
+    import sysconfig
+
+    import torch
+    src = os.path.join(CSRC, "dispatch.c")
+    deps = [src, os.path.join(ROOT, "include", "zero_tensor_cuda.h")]
+    if os.path.exists(DISPATCH) and os.path.getmtime(DISPATCH) >= max(os.path.getmtime(p) for p in deps):
+        return DISPATCH
+    inc = [sysconfig.get_paths()["include"], os.path.join(os.path.dirname(torch.__file__), "include")]
+    cmd = ["gcc", "-O2", "-std=gnu11", "-shared", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wno-unused-parameter",
+           *[a for i in inc for a in ("-I", i)], src, "-o", DISPATCH + ".tmp", "-lm"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"gcc failed for {src}:\n{r.stdout}\n{r.stderr}")
+    if r.stderr:
+        sys.stderr.write(r.stderr)
+    os.replace(DISPATCH + ".tmp", DISPATCH)
+    return DISPATCH
 
 
 if __name__ == "__main__":

@@ -27,6 +27,7 @@ import torch
 
 import ctypes as C
 
+from . import _lib
 from ._lib import LogitsRules, ZcError, check, lib
 
 QK = 32
@@ -230,7 +231,9 @@ class LlmSampler:
         return out
 
 
-# ---- one step of a mixed serving batch (zcu_pages_*, zcu_append_kv, zcu_process_logits) ----
+# ---- one step of a mixed serving batch (zcu_pages_*, zcu_append_kv, zcu_sparse_paged_attention, zcu_lora_add,
+#      zcu_process_logits).  Each function first offers its arguments to _dispatch, which checks and calls in one step
+#      (True: enqueued); what that declines goes through the checks and the ctypes call below it. ----
 
 _FLOAT_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
@@ -300,12 +303,17 @@ def reserve_pages(page_table, seq_len, free_pages, free_count, n_new, page_size:
     stack free_pages [num_pages] of *free_count ids; int32, updated in place).  `tokens` is the length of the step's
     token arrays (room behind the last token is padding), taken from `out` (a PagePlan to write to) when that is
     given."""
-    dev, pool = _pool_args(page_table, seq_len, free_pages, free_count, page_size)
-    batch = n_new.shape[0]
     if out is None:
         if tokens is None:
             raise ZcError("reserve_pages needs tokens, the length of the step's token arrays, or out")
-        out = PagePlan.empty(batch, tokens, page_table.device)
+        out = PagePlan.empty(n_new.shape[0], tokens, page_table.device)
+        tokens = None
+    d = _lib.dispatch
+    if d and stream is None and tokens is None and d.reserve_pages(page_table, seq_len, free_pages, free_count,
+                                                                   page_size, n_new, rows, *out):
+        return out if isinstance(out, PagePlan) else PagePlan(*out)
+    dev, pool = _pool_args(page_table, seq_len, free_pages, free_count, page_size)
+    batch = n_new.shape[0]
     start, slots, positions, token_rows, ctx_len, granted = out
     n = slots.shape[0]
     if tokens is not None and tokens != n:
@@ -322,6 +330,9 @@ def reserve_pages(page_table, seq_len, free_pages, free_count, n_new, page_size:
 def trim_pages(page_table, seq_len, free_pages, free_count, new_len, page_size: int, rows=None, stream=None) -> None:
     """Row rows[b] (None: row b) keeps min(new_len[b], its length) tokens; the pages behind them go back to the stack
     (zcu_pages_trim).  new_len 0 frees a sequence; a shorter one takes rejected drafts back."""
+    d = _lib.dispatch
+    if d and stream is None and d.trim_pages(page_table, seq_len, free_pages, free_count, page_size, new_len, rows):
+        return
     dev, pool = _pool_args(page_table, seq_len, free_pages, free_count, page_size)
     batch = new_len.shape[0]
     _call(lib().zcu_pages_trim, "trim_pages", dev, stream, *pool, _arg("rows", rows, torch.int32, dev, (batch,)),
@@ -346,6 +357,9 @@ def append_kv(k, v, slots, k_pool, v_pool, bounds=None, scales=None, stream=None
     at slots [tokens] (int64; reserve_pages' slots, negative ones skipped).  bounds int8 [pages, hkv, 2, hd] and
     scales fp32 [pages, hkv] receive the 8-bit key bounds of the pages written, which sparse_paged_attention scores
     pages by (zcu_append_kv)."""
+    d = _lib.dispatch
+    if d and stream is None and d.append_kv(k, v, slots, k_pool, v_pool, bounds, scales):
+        return
     dev = _cuda("k", k)
     code, pages, hkv, page, hd, sp, ss, sh = _kv_pools(k_pool, v_pool, dev)
     shape, ks, vs = k.shape, k.stride(), v.stride()
@@ -373,6 +387,11 @@ def sparse_paged_attention(q, k_pool, v_pool, bounds, scales, page_table, ctx_le
     ctx_len [batch] int32; query b reads table row rows[b] (None: b; reserve_pages' token_rows), so several queries of
     one sequence may share a row.  max_ctx bounds ctx_len (default: what the table holds).  Returns (out [batch, hq,
     hd], sel [batch, hkv, budget]: the chosen pages as indices into the table row, ascending, -1 behind them)."""
+    d = _lib.dispatch
+    if d and stream is None and out is not None and sel is not None and d.sparse_paged_attention(
+            q, k_pool, v_pool, bounds, scales, page_table, ctx_len, budget, rows, sink, recent, scale, max_ctx, out,
+            sel):
+        return out, sel
     dev = _cuda("q", q)
     code, pages, hkv, page, hd, sp, ss, sh = _kv_pools(k_pool, v_pool, dev)
     shape, qs = q.shape, q.stride()
@@ -408,9 +427,12 @@ def lora_add(y, x, a, b, adapter, ranks=None, scales=None, out=None, stream=None
     x [rows, k], y [rows, n] fp32 (any row stride), a [adapters, rank, k], b [adapters, n, rank] fp32, fp16 or bf16,
     adapter [rows] int32; ranks [adapters] int32 for adapters that use fewer than rank, scales [adapters] fp32.  out
     defaults to y, in place."""
-    dev = _cuda("y", y)
     if out is None:
         out = y
+    d = _lib.dispatch
+    if d and stream is None and d.lora_add(y, x, a, b, adapter, ranks, scales, out):
+        return out
+    dev = _cuda("y", y)
     if y.dim() != 2 or x.dim() != 2 or a.dim() != 3 or b.dim() != 3:
         raise ZcError("x and y must be matrices, a and b stacks of matrices")
     rows, n = y.shape
@@ -440,13 +462,20 @@ def process_logits(logits, out=None, past=None, past_len=None, prompt_len=None, 
     positive logits (multiplies others) of every token seen, frequency and presence are subtracted for the ones behind
     the prompt, each [rows] fp32.  bias_start [rows + 1], bias_ids, bias: each row's biased tokens.  mask [m, words]
     int32: bit t % 32 of word t / 32 allows token t; row r uses mask_rows[r] (None: r; outside: unmasked)."""
+    if out is None and logits.dtype is torch.float32:
+        out = logits
+    d = _lib.dispatch
+    if d and stream is None and out is not None and d.process_logits(
+            logits, out, past, past_len, prompt_len, past_rows, repetition, frequency, presence, bias_start, bias_ids,
+            bias, mask, mask_rows):
+        return out
     dev = _cuda("logits", logits)
     code, xs = _FLOAT_CODE.get(logits.dtype), logits.stride()
     if len(xs) != 2 or code is None or (xs[1] != 1 and logits.numel()):
         raise ZcError("logits must be [rows, vocab] fp32, fp16 or bf16 with contiguous rows")
     rows, vocab = logits.shape
     if out is None:
-        out = torch.empty((rows, vocab), dtype=torch.float32, device=logits.device) if code else logits
+        out = torch.empty((rows, vocab), dtype=torch.float32, device=logits.device)
     os = out.stride()
     if out.shape != (rows, vocab) or out.dtype is not torch.float32 or out.get_device() != dev or \
             (os[1] != 1 and out.numel()):
