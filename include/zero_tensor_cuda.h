@@ -363,7 +363,7 @@ ZC_API int32_t zcu_moe_forward(void* moe, const float* xnorm, const float* route
  * trim: row rows[b] keeps min(new_len[b], its length) tokens (0 frees the sequence); pages behind them go back to the
  * stack, the last request's last page first, and their table entries become -1.  A reserve whose lengths are trimmed
  * back leaves the stack as it was.
- * -6 when batch and max_rows exceed one CTA's shared memory (20 bytes a request, and 4 a table row with `rows`, over
+ * -6 when batch and max_rows exceed one CTA's shared memory (24 bytes a request, and 4 a table row with `rows`, over
  * 220 KB). */
 ZC_API int32_t zcu_pages_reserve(int32_t* page_table, int32_t* seq_len, int32_t* free_pages, int32_t* free_count,
                                  int32_t max_rows, int32_t max_pages, int32_t num_pages, int32_t page_size,

@@ -66,31 +66,36 @@ __device__ __forceinline__ int pages_of(long long tokens, int page) { return (in
 // What both kernels keep per request in shared memory.
 struct Req {
   int* row;    // table row, -1: not usable (out of range, or a row that an earlier request of the call names)
-  int* old;    // tokens stored
+  int* arg;    // tokens to add, or the length to keep
+  int* old;    // tokens stored (trim: pages stored)
   int* first;  // pages stored (reserve) or kept (trim)
   int* poff;   // pages moved by the requests before it (trim: by reverse index, behind it)
   int* start;  // [batch + 1] first token (reserve only)
 };
 
-// Table rows of the requests; a row named twice belongs to the first request that names it.
+// Table rows, arguments and lengths of the requests: two loads one after the other, whatever else is checked.  A row
+// named twice belongs to the first request that names it.
 template <int PG_THREADS>
-__device__ void load_rows(const PagePool& p, const int32_t* rows, int batch, const Req& q, int* owner) {
-  if (!rows) {
-    for (int b = threadIdx.x; b < batch; b += PG_THREADS) q.row[b] = b;  // batch <= max_rows
-    __syncthreads();
-    return;
-  }
+__device__ void load_requests(const PagePool& p, const int32_t* rows, const int32_t* args, int batch, const Req& q,
+                              int* owner) {
   for (int b = threadIdx.x; b < batch; b += PG_THREADS) {
-    const int r = rows[b];
-    q.row[b] = (unsigned)r < (unsigned)p.max_rows ? r : -1;
-    if (q.row[b] >= 0) owner[r] = 0x7fffffff;
+    const int r = rows ? rows[b] : b;  // without rows batch <= max_rows
+    q.arg[b] = max(args[b], 0);
+    const bool in = (unsigned)r < (unsigned)p.max_rows;
+    q.row[b] = in ? r : -1;
+    q.old[b] = in ? max(p.len[r], 0) : 0;
+    if (in && rows) owner[r] = 0x7fffffff;
   }
   __syncthreads();
+  if (!rows) return;
   for (int b = threadIdx.x; b < batch; b += PG_THREADS)
     if (q.row[b] >= 0) atomicMin(&owner[q.row[b]], b);
   __syncthreads();
   for (int b = threadIdx.x; b < batch; b += PG_THREADS)
-    if (q.row[b] >= 0 && owner[q.row[b]] != b) q.row[b] = -1;
+    if (q.row[b] >= 0 && owner[q.row[b]] != b) {
+      q.row[b] = -1;
+      q.old[b] = 0;
+    }
   __syncthreads();
 }
 
@@ -119,26 +124,26 @@ __global__ void __launch_bounds__(PG_THREADS) reserve_kernel(PagePool p, const i
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = cluster.block_rank(), ranks = cluster.num_blocks();
   const int P = p.page_size;
-  const Req q{sm, sm + batch, sm + 2 * batch, sm + 3 * batch, sm + 4 * batch};
-  load_rows<PG_THREADS>(p, rows, batch, q, sm + 5 * batch + 1);
-  const int count = min(max(*p.free_count, 0), p.num_pages);
+  const Req q{sm, sm + batch, sm + 2 * batch, sm + 3 * batch, sm + 4 * batch, sm + 5 * batch};
+  const int held = *p.free_count;
+  load_requests<PG_THREADS>(p, rows, n_new, batch, q, sm + 6 * batch + 1);
+  const int count = min(max(held, 0), p.num_pages);
 
   // each thread owns `per` consecutive requests
   const int per = (batch + PG_THREADS - 1) / PG_THREADS;
   const int b0 = min(batch, (int)threadIdx.x * per), b1 = min(batch, b0 + per);
   long long sum = 0, total;
-  for (int b = b0; b < b1; ++b) sum += max(n_new[b], 0);
+  for (int b = b0; b < b1; ++b) sum += q.arg[b];
   long long at = block_prefix<PG_THREADS>(sum, red, &total);
   const long long whole = total;
   long long more = 0;
   for (int b = b0; b < b1; ++b) {
-    const int n = max(n_new[b], 0), r = q.row[b];
-    const int old = r >= 0 ? max(p.len[r], 0) : 0;
+    const int n = q.arg[b], old = q.old[b];
     q.start[b] = (int)min(at, (long long)0x7fffffff);
     at += n;
-    const bool fits = r >= 0 && (long long)old + n <= min((long long)p.max_pages * P, 0x7fffffffLL) && at <= tokens;
+    const bool fits = q.row[b] >= 0 && (long long)old + n <= min((long long)p.max_pages * P, 0x7fffffffLL) &&
+                      at <= tokens;
     const int have = pages_of(old, P);
-    q.old[b] = old;
     q.first[b] = fits ? have : -1;
     if (fits) more += pages_of((long long)old + n, P) - have;
   }
@@ -148,7 +153,7 @@ __global__ void __launch_bounds__(PG_THREADS) reserve_kernel(PagePool p, const i
   for (int b = b0; b < b1; ++b) {
     q.poff[b] = (int)min(off, (long long)count);
     if (q.first[b] < 0) continue;
-    const int n = max(n_new[b], 0), m = pages_of((long long)q.old[b] + n, P) - q.first[b];
+    const int m = pages_of((long long)q.old[b] + q.arg[b], P) - q.first[b];
     off += m;
     if (off > count)
       q.first[b] = -1;  // refused, as every later request that needs a page
@@ -164,7 +169,7 @@ __global__ void __launch_bounds__(PG_THREADS) reserve_kernel(PagePool p, const i
       const bool ok = q.first[b] >= 0;
       o.granted[b] = ok;
       o.start[b] = q.start[b];
-      if (ok) p.len[q.row[b]] = q.old[b] + max(n_new[b], 0);
+      if (ok) p.len[q.row[b]] = q.old[b] + q.arg[b];
     }
     if (threadIdx.x == 0) o.start[batch] = q.start[batch];
   }
@@ -226,17 +231,18 @@ __global__ void __launch_bounds__(PG_THREADS) trim_kernel(PagePool p, const int3
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = cluster.block_rank(), ranks = cluster.num_blocks();
   const int P = p.page_size;
-  const Req q{sm, sm + batch, sm + 2 * batch, sm + 3 * batch, nullptr};
-  load_rows<PG_THREADS>(p, rows, batch, q, sm + 4 * batch);
-  const int count = min(max(*p.free_count, 0), p.num_pages);
+  const Req q{sm, sm + batch, sm + 2 * batch, sm + 3 * batch, sm + 4 * batch, nullptr};
+  const int held = *p.free_count;
+  load_requests<PG_THREADS>(p, rows, new_len, batch, q, sm + 5 * batch);
+  const int count = min(max(held, 0), p.num_pages);
   const int per = (batch + PG_THREADS - 1) / PG_THREADS;
+  const int most = (int)min((long long)p.max_pages * P, 0x7fffffffLL);
   // requests in reverse order: index i is request batch - 1 - i
   const int i0 = min(batch, (int)threadIdx.x * per), i1 = min(batch, i0 + per);
   long long gone = 0, total;
   for (int i = i0; i < i1; ++i) {
-    const int b = batch - 1 - i, r = q.row[b];
-    const int old = r >= 0 ? min(max(p.len[r], 0), (int)min((long long)p.max_pages * P, 0x7fffffffLL)) : 0;
-    const int keep = min(max(new_len[b], 0), old);
+    const int b = batch - 1 - i, old = min(q.old[b], most), keep = min(q.arg[b], old);
+    q.arg[b] = keep;
     q.old[b] = pages_of(old, P);
     q.first[b] = pages_of(keep, P);
     gone += q.old[b] - q.first[b];
@@ -253,10 +259,7 @@ __global__ void __launch_bounds__(PG_THREADS) trim_kernel(PagePool p, const int3
   if (rank == 0) {
     if (threadIdx.x == 0) *p.free_count = count + back;
     for (int b = threadIdx.x; b < batch; b += PG_THREADS)
-      if (q.row[b] >= 0) {
-        const int r = q.row[b], old = p.len[r];
-        p.len[r] = max(min(max(new_len[b], 0), old), 0);
-      }
+      if (q.row[b] >= 0) p.len[q.row[b]] = q.arg[b];
   }
   const int tid = rank * PG_THREADS + threadIdx.x, step = ranks * PG_THREADS;
   const int moved = (int)min(total, 0x7fffffffLL);
@@ -293,7 +296,7 @@ int pages_reserve(const PagePool& p, const int32_t* rows, const int32_t* n_new, 
   if (tokens < 0 || !o.start || (batch > 0 && (!n_new || !o.granted))) return kBadArgument;
   if (tokens > 0 && (!o.slots || !o.positions || !o.token_rows || !o.ctx_len)) return kBadArgument;
   if (!rows && batch > p.max_rows) return kBadArgument;
-  const size_t smem = ((size_t)5 * batch + 1 + (rows ? p.max_rows : 0)) * sizeof(int);
+  const size_t smem = ((size_t)6 * batch + 1 + (rows ? p.max_rows : 0)) * sizeof(int);
   if (smem > PG_SMEM_MAX) return kTooLarge;
   const Shape f = shape_for(batch, tokens);
   auto kernel = f.threads == 256 ? reserve_kernel<256> : reserve_kernel<1024>;
@@ -308,7 +311,7 @@ int pages_trim(const PagePool& p, const int32_t* rows, const int32_t* new_len, i
   if (const int rc = check(p, batch)) return rc;
   if (batch == 0) return kOk;
   if (!new_len || (!rows && batch > p.max_rows)) return kBadArgument;
-  const size_t smem = ((size_t)4 * batch + (rows ? p.max_rows : 0)) * sizeof(int);
+  const size_t smem = ((size_t)5 * batch + (rows ? p.max_rows : 0)) * sizeof(int);
   if (smem > PG_SMEM_MAX) return kTooLarge;
   const Shape f = shape_for(batch, (long long)batch * 16);  // the host does not know how many pages go back
   auto kernel = f.threads == 256 ? trim_kernel<256> : trim_kernel<1024>;
