@@ -793,11 +793,12 @@ int launch(const SparseAttnArgs& a, cudaStream_t s) {
   d.a = a;
   d.cap_pages = (int)std::min<long long>(((long long)a.max_ctx + a.page_size - 1) / a.page_size, a.max_pages);
   const long long pairs = (long long)a.batch * a.hkv;
-  // CTAs per pair: as many as leave all of them resident, two an SM.  What a CTA does once whatever its share (query
-  // staging, threshold, joins: about 8 us) is then paid once in time; twice as many CTAs in two waves measured
-  // 113 us where one wave takes 97 (32 sequences of up to 32k tokens, 8 KV heads).
-  int S = 1;
-  while (S < SP_CLUSTER && pairs * S * 2 <= 2 * 148) S <<= 1;
+  // CTAs per pair: as many as are all resident at once, one an SM, since each pays a chain of about 10 us (lengths, ids,
+  // threshold, joins) whatever its share.  A cluster lives in one GPC, so the 148 SMs hold 14 clusters of 8, 32 of 4
+  // and 74 of 2; one more starts a second wave.  Sequences of 8k tokens, 64 pages: 14 pairs 14.1 us with 8 CTAs each,
+  // 15.1 with 4; 18 pairs 26.6 and 15.4; 32 pairs (16k, 128 pages) 24.4 and 22.1; 64 pairs 32.4 with 4, 30.2 with 2;
+  // 128 pairs 48.6 with 2, 45.2 with 1.
+  const int S = pairs <= 14 ? 8 : pairs <= 32 ? 4 : pairs <= 74 ? 2 : 1;
   d.key_words = d.cap_pages > a.budget ? (d.cap_pages + 3) / 4 * 4 : 0;
   d.share = (std::min(a.budget, d.cap_pages) + S - 1) / S;
   size_t smem = (size_t)SP_WARPS * 64 * HD + (size_t)d.key_words * 4 + SP_HEADS * HD * 4 + 16 * (2 * HD + 16) +
@@ -805,8 +806,8 @@ int launch(const SparseAttnArgs& a, cudaStream_t s) {
   d.id_words = smem + (size_t)d.key_words * 4 <= SP_SMEM_MAX ? d.key_words : 0;
   smem += (size_t)d.id_words * 4;
   if (smem > SP_SMEM_MAX || pairs * S > 0x7fffffffLL) return kTooLarge;
-  // One CTA an SM is left its registers: a single sequence of 8k tokens takes 13.3 us so, 16.3 us within 128 registers,
-  // which two CTAs an SM need.  Outputs of 256 dims leave room for one only.
+  // One CTA an SM is left its registers (8 pairs of 8k tokens 13.9 us so, 16.3 us within the 128 that two CTAs an SM
+  // need); more pairs than SMs share them.  Outputs of 256 dims leave room for one only.
   const bool two = HD <= 128 && pairs * S > 148;
   auto kernel = two ? sparse_attn_kernel<HD, HALF, HD <= 128 ? 2 : 1> : sparse_attn_kernel<HD, HALF, 1>;
   if (allow_smem(kernel, smem)) return kCudaError;
