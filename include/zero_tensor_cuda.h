@@ -401,7 +401,7 @@ ZC_API int32_t zcu_append_kv(const void* k, const void* v, int32_t in_dtype, int
  * s_q = max|q| / 32512 and qi = rint(q / s_q): whole numbers summed exactly and two fp32 products, so the choice
  * does not depend on the launch; the lower page wins among equal scores.
  * hd 64, 128 or 256, page_size a multiple of 8 (else -4); -6 when a CTA's shared memory does not hold the scores of
- * max_ctx tokens and its part of the budget (46,000 pages at hd 64, 35,000 at 128, 15,000 at 256), or when max_ctx and a
+ * max_ctx tokens and its part of the budget (44,000 pages at hd 64, 34,000 at 128, 14,000 at 256), or when max_ctx and a
  * page pass 2^30 tokens. */
 ZC_API int32_t zcu_sparse_paged_attention(const float* q, int64_t q_stride, const void* k_pool, const void* v_pool,
                                           int32_t kv_dtype, const int8_t* bounds, const float* scales,

@@ -25,7 +25,7 @@
 //   join    warps, then the cluster's CTAs, merge their (max, sum, output) states in shared memory.
 // Bound: HBM, bytes = pages * (2 hd + 4) + selected tokens * hd * 2 * sizeof(kv) per (row, KV head), behind a chain of
 // about 10 us that every row has (lengths, ids, bounds, threshold, keys, join).  32 sequences of 4k to 32k tokens,
-// 32 / 8 heads of 128, 128 pages of 16: 90 us for 350 MB (3.9 TB/s); 24 sequences of up to 2k tokens, 12 heads of 64,
+// 32 / 8 heads of 128, 128 pages of 16: 87 us for 350 MB (4.0 TB/s); 24 sequences of up to 2k tokens, 12 heads of 64,
 // fp32 pools, 32 pages: 26 us for 70 MB; one sequence of 8k tokens: 13.8 us, the chain.
 
 #include <cooperative_groups.h>
@@ -313,10 +313,14 @@ __global__ void __launch_bounds__(SP_THREADS, CTAS) sparse_attn_kernel(SparseDev
       }
       const float s_q = sq[g];
       const bool last = h0 + SP_HEADS >= group;
-      // Sixteen pages a stage, two stages in flight; lanes 0-15 hold the pages' ids, scales and whether they exist.
+      // Sixteen pages a stage, two stages in flight (four measured no better); lanes 0-15 hold the pages' ids, scales and
+      // whether they exist.
+      constexpr int STAGES = 2;
       int id = -1;
-      float scale[2] = {0.f, 0.f};
-      bool ok[2] = {false, false};
+      float scale[STAGES];
+      bool ok[STAGES];
+#pragma unroll
+      for (int i = 0; i < STAGES; ++i) scale[i] = 0.f, ok[i] = false;
       auto fetch_ids = [&](int p0) {
         const int p = p0 + lane;
         id = lane < 16 && p < p_end ? id_of(p) : -1;
@@ -329,26 +333,27 @@ __global__ void __launch_bounds__(SP_THREADS, CTAS) sparse_attn_kernel(SparseDev
           for (int i = 0; i < RP / 2; ++i) {
             const int r = (i * 32 + lane) / RP, piece = (i * 32 + lane) % RP;
             const size_t from = __shfl_sync(0xffffffffu, rec, r);
-            copy16(ring + buf * 16 * 2 * HD + r * 2 * HD + key_piece(r, piece) * 16, a.bounds + from * (2 * HD) + piece * 16,
-                   __shfl_sync(0xffffffffu, (int)in_pool, r));
+            copy16(ring + buf * 16 * 2 * HD + r * 2 * HD + key_piece(r, piece) * 16,
+                   a.bounds + from * (2 * HD) + piece * 16, __shfl_sync(0xffffffffu, (int)in_pool, r));
           }
         }
         copies_commit();
-        scale[0] = scale[1];
-        ok[0] = ok[1];
-        ok[1] = in_pool;
-        scale[1] = in_pool && last ? __ldg(a.scales + rec) : 0.f;
+#pragma unroll
+        for (int i = 0; i + 1 < STAGES; ++i) scale[i] = scale[i + 1], ok[i] = ok[i + 1];
+        ok[STAGES - 1] = in_pool;
+        scale[STAGES - 1] = in_pool && last ? __ldg(a.scales + rec) : 0.f;
       };
       constexpr int STEP = SP_WARPS * 16;
       const int first = p_begin + warp * 16;
-      fetch_ids(first);
-      issue(first, 0);
-      fetch_ids(first + STEP);
-      issue(first + STEP, 1);
-      fetch_ids(first + 2 * STEP);
+#pragma unroll
+      for (int i = 0; i < STAGES; ++i) {
+        fetch_ids(first + i * STEP);
+        issue(first + i * STEP, i);
+      }
+      fetch_ids(first + STAGES * STEP);
       int buf = 0;
       for (int p0 = first; p0 < p_end; p0 += STEP) {
-        copies_wait<1>();
+        copies_wait<STAGES - 1>();
         __syncwarp();
         int d2[2][4];
 #pragma unroll
@@ -368,9 +373,9 @@ __global__ void __launch_bounds__(SP_THREADS, CTAS) sparse_attn_kernel(SparseDev
         __syncwarp();
         const float sc = scale[0];
         const bool exists = ok[0];
-        issue(p0 + 2 * STEP, buf);
-        fetch_ids(p0 + 3 * STEP);
-        buf ^= 1;
+        issue(p0 + STAGES * STEP, buf);
+        fetch_ids(p0 + (STAGES + 1) * STEP);
+        buf = buf + 1 == STAGES ? 0 : buf + 1;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int(&d)[4] = d2[u];
@@ -566,21 +571,24 @@ __global__ void __launch_bounds__(SP_THREADS, CTAS) sparse_attn_kernel(SparseDev
       }
       copies_commit();
     };
-    long long off[NB];
-    int nv[NB];
+    constexpr int STRIDE = SP_WARPS * TB;  // tokens between a warp's blocks
+    unsigned char* const kbuf = ring;
+    unsigned char* const vbuf = ring + HALF_RING;
+    int nv[NB];  // tokens that the block in the buffer has
     int i0 = warp * TB;
     if (i0 < tokens) {
+      long long off[NB];
 #pragma unroll
       for (int u = 0; u < NB; ++u) nv[u] = locate(i0 + 8 * u, off[u]);
-      copy_rows(k_lane, ring, off, nv, true);
-      copy_rows(v_lane, ring + HALF_RING, off, nv, false);
+      copy_rows(k_lane, kbuf, off, nv, true);
+      copy_rows(v_lane, vbuf, off, nv, false);
     }
-    for (; i0 < tokens; i0 += SP_WARPS * TB) {
-      const bool more = i0 + SP_WARPS * TB < tokens;
+    for (; i0 < tokens; i0 += STRIDE) {
+      const bool more = i0 + STRIDE < tokens;
       long long off_next[NB];
       int nv_next[NB];
 #pragma unroll
-      for (int u = 0; u < NB; ++u) nv_next[u] = locate(i0 + SP_WARPS * TB + 8 * u, off_next[u]);
+      for (int u = 0; u < NB; ++u) nv_next[u] = locate(i0 + STRIDE + 8 * u, off_next[u]);
       copies_wait<1>();  // the keys
       __syncwarp();
       float s[2 * NB];
@@ -595,7 +603,7 @@ __global__ void __launch_bounds__(SP_THREADS, CTAS) sparse_attn_kernel(SparseDev
           for (int u = 0; u < 2; ++u) {
             // 32 dims a sum in the tensor core, whose accumulator truncates; the sums are added with rounding
             float d[4] = {0.f, 0.f, 0.f, 0.f};
-            const uint4 k = *reinterpret_cast<const uint4*>(ring + (8 * u + g) * ROWB + key_piece(g, 4 * j + c) * 16);
+            const uint4 k = *reinterpret_cast<const uint4*>(kbuf + (8 * u + g) * ROWB + key_piece(g, 4 * j + c) * 16);
             mma_f16(d, ah.x, al.x, ah.y, al.y, k.x, k.y);
             mma_f16(d, ah.z, al.z, ah.w, al.w, k.z, k.w);
             z[2 * u] += d[0] + d[2];
@@ -615,7 +623,7 @@ __global__ void __launch_bounds__(SP_THREADS, CTAS) sparse_attn_kernel(SparseDev
           float d[4] = {0.f, 0.f, 0.f, 0.f}, dl[4] = {0.f, 0.f, 0.f, 0.f};
           const uint4 ah = *reinterpret_cast<const uint4*>(qt + g * QA + 16 * j + 4 * c);
           const uint4 al = *reinterpret_cast<const uint4*>(qt + (g + 8) * QA + 16 * j + 4 * c);
-          const uint4 k = *reinterpret_cast<const uint4*>(ring + g * ROWB + key_piece(g, 4 * j + c) * 16);
+          const uint4 k = *reinterpret_cast<const uint4*>(kbuf + g * ROWB + key_piece(g, 4 * j + c) * 16);
           uint32_t h[4], l[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) tf32_pair(__uint_as_float(word(k, i)), h[i], l[i]);
@@ -631,7 +639,7 @@ __global__ void __launch_bounds__(SP_THREADS, CTAS) sparse_attn_kernel(SparseDev
       }
       __syncwarp();
       if (more)
-        copy_rows(k_lane, ring, off_next, nv_next, true);
+        copy_rows(k_lane, kbuf, off_next, nv_next, true);
       else
         copies_commit();  // an empty group, so that the wait below counts the same
       const float base = st.raise(s);
@@ -655,7 +663,7 @@ __global__ void __launch_bounds__(SP_THREADS, CTAS) sparse_attn_kernel(SparseDev
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const int r = 2 * c + (u & 1) + 8 * (u >> 1);
-            v[u] = *reinterpret_cast<const uint4*>(ring + HALF_RING + r * ROWB + value_piece(r, 8 * j + g) * 16);
+            v[u] = *reinterpret_cast<const uint4*>(vbuf + r * ROWB + value_piece(r, 8 * j + g) * 16);
           }
 #pragma unroll
           for (int e = 0; e < 8; ++e) {  // column n of tile (j, e) is dim 64 j + 8 n + e
@@ -677,7 +685,7 @@ __global__ void __launch_bounds__(SP_THREADS, CTAS) sparse_attn_kernel(SparseDev
           uint4 v[2];
 #pragma unroll
           for (int u = 0; u < 2; ++u)
-            v[u] = *reinterpret_cast<const uint4*>(ring + HALF_RING + (2 * c + u) * ROWB +
+            v[u] = *reinterpret_cast<const uint4*>(vbuf + (2 * c + u) * ROWB +
                                                    value_piece(2 * c + u, 8 * j + g) * 16);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {  // column n of tile (j, e) is dim 32 j + 4 n + e
@@ -691,14 +699,11 @@ __global__ void __launch_bounds__(SP_THREADS, CTAS) sparse_attn_kernel(SparseDev
       }
       __syncwarp();
       if (more)
-        copy_rows(v_lane, ring + HALF_RING, off_next, nv_next, false);
+        copy_rows(v_lane, vbuf, off_next, nv_next, false);
       else
         copies_commit();
 #pragma unroll
-      for (int u = 0; u < NB; ++u) {
-        off[u] = off_next[u];
-        nv[u] = nv_next[u];
-      }
+      for (int u = 0; u < NB; ++u) nv[u] = nv_next[u];
     }
     copies_wait<0>();
     __syncthreads();  // every warp is done with its buffer, where the outputs go now
