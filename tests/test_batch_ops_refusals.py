@@ -129,3 +129,25 @@ def test_logits_refuses_a_vocabulary_that_no_cluster_holds():
     assert logits(vocab=409601, xs=409632, os=409632) == -6
     assert logits(rows=0) == 0
     assert _lib.lib().zcu_process_logits(P, 0, 64, P, 64, 1, 64, None, None) == -2
+
+
+def test_dispatch_takes_cuda_tensors_only():
+    """The binding module is built and loaded with the library; whatever it is given here it declines (host tensors, other
+    objects, wrong counts), and the Python checks behind it name the fault."""
+    import torch
+
+    from zeroplatform_b200 import ops
+    from zeroplatform_b200._lib import ZcError
+    _lib.lib()
+    d = _lib.dispatch
+    assert d is not None
+    t, n = torch.zeros(2, 3), None
+    for f, count in ((d.reserve_pages, 13), (d.trim_pages, 7), (d.append_kv, 7), (d.sparse_paged_attention, 15),
+                     (d.lora_add, 8), (d.process_logits, 14)):
+        for args in ([t] * count, [n] * count, [3] * count, ["x"] * count, [np.zeros(3)] * count, [t] * (count - 1), []):
+            assert f(*args) is False
+    for call in (lambda: ops.process_logits(t), lambda: ops.lora_add(t, t, t, t, t), lambda: ops.append_kv(t, t, t, t, t),
+                 lambda: ops.trim_pages(t, t, t, t, t, 16), lambda: ops.process_logits(np.zeros((2, 3))),
+                 lambda: ops.sparse_paged_attention(t, t, t, t, t, t, t, 4)):
+        with pytest.raises(ZcError):
+            call()

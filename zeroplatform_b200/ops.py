@@ -261,6 +261,14 @@ def _arg(what: str, t, dtype, device: int, shape=None):
     return t.data_ptr()
 
 
+def _empty(shape, dtype, device, stream):
+    """A new tensor that belongs to the stream the call runs on."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 def _cuda(what: str, t) -> int:
     """The index of the CUDA device that a tensor is on."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda):
@@ -291,8 +299,8 @@ class PagePlan(NamedTuple):
     granted: torch.Tensor
 
     @staticmethod
-    def empty(batch: int, tokens: int, device="cuda") -> "PagePlan":
-        e = lambda n, t=torch.int32: torch.empty(n, dtype=t, device=device)  # noqa: E731
+    def empty(batch: int, tokens: int, device="cuda", stream=None) -> "PagePlan":
+        e = lambda n, t=torch.int32: _empty(n, t, device, stream)  # noqa: E731
         return PagePlan(e(batch + 1), e(tokens, torch.int64), e(tokens), e(tokens), e(tokens), e(batch))
 
 
@@ -306,7 +314,7 @@ def reserve_pages(page_table, seq_len, free_pages, free_count, n_new, page_size:
     if out is None:
         if tokens is None:
             raise ZcError("reserve_pages needs tokens, the length of the step's token arrays, or out")
-        out = PagePlan.empty(n_new.shape[0], tokens, page_table.device)
+        out = PagePlan.empty(n_new.shape[0], tokens, page_table.device, stream)
         tokens = None
     d = _lib.dispatch
     if d and stream is None and tokens is None and d.reserve_pages(page_table, seq_len, free_pages, free_count,
@@ -408,9 +416,9 @@ def sparse_paged_attention(q, k_pool, v_pool, bounds, scales, page_table, ctx_le
         max_ctx = min(max_pages * page, (1 << 30) - page)
     i, f = torch.int32, torch.float32
     if out is None:
-        out = torch.empty((batch, hq, hd), dtype=f, device=q.device)
+        out = _empty((batch, hq, hd), f, q.device, stream)
     if sel is None:
-        sel = torch.empty((batch, hkv, budget), dtype=i, device=q.device)
+        sel = _empty((batch, hkv, budget), i, q.device, stream)
     _call(lib().zcu_sparse_paged_attention, "sparse_paged_attention", dev, stream, q.data_ptr(), qs[0],
           k_pool.data_ptr(), v_pool.data_ptr(), code, _arg("bounds", bounds, torch.int8, dev, (pages, hkv, 2, hd)),
           _arg("scales", scales, f, dev, (pages, hkv)), _arg("page_table", page_table, i, dev), table_rows,
@@ -475,7 +483,7 @@ def process_logits(logits, out=None, past=None, past_len=None, prompt_len=None, 
         raise ZcError("logits must be [rows, vocab] fp32, fp16 or bf16 with contiguous rows")
     rows, vocab = logits.shape
     if out is None:
-        out = torch.empty((rows, vocab), dtype=torch.float32, device=logits.device)
+        out = _empty((rows, vocab), torch.float32, logits.device, stream)
     os = out.stride()
     if out.shape != (rows, vocab) or out.dtype is not torch.float32 or out.get_device() != dev or \
             (os[1] != 1 and out.numel()):
