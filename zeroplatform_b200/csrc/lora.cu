@@ -804,8 +804,13 @@ __global__ void __launch_bounds__(LR_THREADS, sizeof(W) == 2 && NT <= 8 ? 2 : 1)
 
 template <typename W, int LG>
 int launch_row(const LoraArgs& a, cudaStream_t s) {
-  // 8 CTAs a row while their parts of k and n are worth a cluster's two barriers (at least a warp's lanes along k)
-  int C = LR_CLUSTER;
+  // 8 CTAs a row while their parts of k and n are worth a cluster's two barriers (at least a warp's lanes along k).
+  // Many rows take smaller clusters; with 8 their CTAs come in waves of about 5 us.  200 rows of rank 64, k 1088, n 2317
+  // take 30 us with clusters of 8, 22 with 4, 18 with 2 (120 rows 12.8 with 4); of rank 16, k = n = 4096, where four CTAs
+  // fit an SM, 14.0, 10.5 and 13.7.  The cluster's size sets the order of t's sum, so up to 112 rows it stays 8: a row
+  // then has the same bits in all those batches (100 rows of the two shapes: 15.9 and 8.8 us with 8, 11.9 and 8.9 with
+  // 4).
+  int C = a.rows <= 112 ? LR_CLUSTER : a.rows <= (LG <= 2 ? 208 : 128) ? 4 : 2;
   while (C > 1 && a.k < 256 * C && a.n < 256 * C) C >>= 1;
   // Few rows take several clusters each, which all sum t and share n, until a CTA's part of n is what it fetches ahead
   // or the clusters (32 of 8 CTAs) no longer fit two CTAs an SM: one row of rank 32, n 11008, k 4096 takes 7.7 us with
@@ -833,9 +838,9 @@ int launch_tile(const LoraArgs& a, cudaStream_t s) {
 
 template <typename W, int LG>
 int launch(const LoraArgs& a, cudaStream_t s) {
-  // A cluster per row up to 256 rows: 0.16 us a row of rank 64 (0.06 of rank 16; k = n = 4096), whatever adapters the
+  // A cluster per row up to 256 rows: 0.15 us a row of rank 64 (0.06 of rank 16; k = n = 4096), whatever adapters the
   // rows use.  Tiles take 29 us (20) for 64 to 256 rows of runs and 38 (27) for 1024, but 130 (75) where every row has
-  // an adapter of its own, which only the device knows: 256 rows of rank 64 are 41 us against 29 or 132.
+  // an adapter of its own, which only the device knows: 256 rows of rank 64 are 39 us against 29 or 132.
   return a.rows <= 256 ? launch_row<W, LG>(a, s) : launch_tile<W, LG>(a, s);
 }
 
