@@ -181,16 +181,17 @@ __device__ void stage_query(const float* q, int heads, float scale_log2, void* q
   }
 }
 
-// One warp's attention state: rows of the accumulators are heads g (hi products) and g + 8 (lo products).
+// One warp's attention state: outputs of head lane / 4, two dims per tile of eight.  The tensor core's accumulator
+// truncates, so it holds one block's products only; a block's hi and lo rows are added to the state with rounding.
 template <int HD, bool HALF>
 struct State {
   static constexpr int NT = HD / 8;
-  float acc[NT][4];
+  float acc[NT][2];
   float m, l;  // head lane / 4: running maximum (log2 domain), this lane's share of the sum
 
   __device__ void init() {
 #pragma unroll
-    for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+    for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = 0.f;
     m = -INFINITY;
     l = 0.f;
   }
@@ -209,7 +210,7 @@ struct State {
       const float alpha = exp2f(m - base);
       l *= alpha;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) acc[i][0] *= alpha, acc[i][1] *= alpha, acc[i][2] *= alpha, acc[i][3] *= alpha;
+      for (int i = 0; i < NT; ++i) acc[i][0] *= alpha, acc[i][1] *= alpha;
     }
     m = mn;
     return base;
@@ -669,7 +670,10 @@ __global__ void __launch_bounds__(SP_THREADS, CTAS) sparse_attn_kernel(SparseDev
           for (int e = 0; e < 8; ++e) {  // column n of tile (j, e) is dim 64 j + 8 n + e
             const uint32_t b0 = __byte_perm(word(v[0], e / 2), word(v[1], e / 2), e & 1 ? 0x7632 : 0x5410);
             const uint32_t b1 = __byte_perm(word(v[2], e / 2), word(v[3], e / 2), e & 1 ? 0x7632 : 0x5410);
-            mma_f16(st.acc[8 * j + e], p_hi[0], p_lo[0], p_hi[1], p_lo[1], b0, b1);
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_f16(d, p_hi[0], p_lo[0], p_hi[1], p_lo[1], b0, b1);
+            st.acc[8 * j + e][0] += d[0] + d[2];
+            st.acc[8 * j + e][1] += d[1] + d[3];
           }
         }
       } else {
@@ -692,8 +696,11 @@ __global__ void __launch_bounds__(SP_THREADS, CTAS) sparse_attn_kernel(SparseDev
             uint32_t vh0, vl0, vh1, vl1;
             tf32_pair(__uint_as_float(word(v[0], e)), vh0, vl0);
             tf32_pair(__uint_as_float(word(v[1], e)), vh1, vl1);
-            mma_tf32(st.acc[4 * j + e], h0w, l0w, h1w, l1w, vh0, vh1);
-            mma_tf32(st.acc[4 * j + e], h0w, l0w, h1w, l1w, vl0, vl1);
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_tf32(d, h0w, l0w, h1w, l1w, vl0, vl1);
+            mma_tf32(d, h0w, l0w, h1w, l1w, vh0, vh1);
+            st.acc[4 * j + e][0] += d[0] + d[2];
+            st.acc[4 * j + e][1] += d[1] + d[3];
           }
         }
       }
@@ -724,10 +731,10 @@ __global__ void __launch_bounds__(SP_THREADS, CTAS) sparse_attn_kernel(SparseDev
 #pragma unroll
         for (int e = 0; e < E; e += 4) {
           float4 o;
-          o.x = st.acc[E * j + e][k] + st.acc[E * j + e][k + 2];
-          o.y = st.acc[E * j + e + 1][k] + st.acc[E * j + e + 1][k + 2];
-          o.z = st.acc[E * j + e + 2][k] + st.acc[E * j + e + 2][k + 2];
-          o.w = st.acc[E * j + e + 3][k] + st.acc[E * j + e + 3][k + 2];
+          o.x = st.acc[E * j + e][k];
+          o.y = st.acc[E * j + e + 1][k];
+          o.z = st.acc[E * j + e + 2][k];
+          o.w = st.acc[E * j + e + 3][k];
           so4[warp * PIECES + (((j * 2 + k) * (E / 4) + e / 4) * 32 + lane)] = o;
         }
     auto store = [&](int i, float4 O, float L) {  // piece i of the result
