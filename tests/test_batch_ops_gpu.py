@@ -470,6 +470,24 @@ def test_sparse_attention_long_sequence_many_pages():
     check_sparse(q, ks, vs, codes, scales, np.arange(n, dtype=np.int32)[None], [ctx], 50, 1, 1, out, sel)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_sparse_attention_long_sums_have_no_bias(dtype):
+    """Equal weights over 65,536 values in [1, 2), so that a weight, the sum of weights and hi parts are exact and an
+    output is a mean.  A block's sum in the tensor core may lose less than an ulp (2^-23) per addend, 16 products (8 of
+    fp32) and the accumulator; whatever is rounded to nearest errs to either side, by at most 2^-24 in each of the 1,024
+    additions of a warp, which six standard deviations of the mean over 19,200 outputs bound by 1e-7."""
+    batch, pages, page, hkv, hd = 150, 2048, 32, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(31)
+    v = (1 + torch.rand(pages, hkv, page, hd, device="cuda", generator=g)).to(dtype)
+    codes, scales = torch.zeros(pages, hkv, 2, hd, dtype=torch.int8, device="cuda"), torch.zeros(pages, hkv, device="cuda")
+    table = torch.stack([torch.randperm(pages, device="cuda", generator=g) for _ in range(batch)]).int()
+    q = torch.zeros(batch, hkv, hd, device="cuda")
+    out, _ = ops.sparse_paged_attention(q, v, v, codes, scales, table, ints([pages * page] * batch), pages)
+    want = v.double().mean((0, 2))
+    addends = 17 if dtype == torch.float16 else 9
+    assert abs(float((out.double() / want - 1).mean())) <= addends * 2.0 ** -23 + 1e-7
+
+
 def test_sparse_attention_in_a_captured_graph():
     rng = np.random.default_rng(13)
     ctx = [600, 350]
@@ -563,6 +581,24 @@ def test_lora_rows_do_not_meet(rows):
     want, mag = plain_lora(x, y, a.nan_to_num(0), b.nan_to_num(0, 0, 0), adapter, ranks, scales)
     assert (np.abs(out - want)[keep] <= 1e-5 * mag[keep]).all()
     assert (out[4] == y[4]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_lora_long_sums_have_no_bias(dtype):
+    """300 rows (tiles) of x in [1, 2), k 131,072, A in [1, 2), B the identity: an output is one sum over k.  A sum of 32
+    columns in the tensor core may lose less than an ulp (2^-23) per addend: two products of 16 and the accumulator (four
+    of 8 in fp32), the hi parts' lower terms beside that as little as they are; whatever is rounded to nearest errs to
+    either side, by at most 2^-22 in x's terms and 2^-24 in each of 270 additions, whose mean over 2,400 outputs stays
+    below 2e-7 (six standard deviations)."""
+    rows, k = 300, 131072
+    g = torch.Generator(device="cuda").manual_seed(32)
+    x = 1 + torch.rand(rows, k, device="cuda", generator=g)
+    a = (1 + torch.rand(1, 8, k, device="cuda", generator=g)).to(dtype)
+    b = torch.eye(8, device="cuda").to(dtype)[None]
+    got = ops.lora_add(torch.zeros(rows, 8, device="cuda"), x, a, b, ints([0] * rows))
+    want = x.double() @ a[0].double().t()
+    addends = 36 if dtype == torch.float32 else 34
+    assert abs(float((got.double() / want - 1).mean())) <= addends * 2.0 ** -23 + 2e-7
 
 
 def test_lora_same_rows_alone_and_in_a_batch():

@@ -25,7 +25,7 @@
 //   join    warps, then the cluster's CTAs, merge their (max, sum, output) states in shared memory.
 // Bound: HBM, bytes = pages * (2 hd + 4) + selected tokens * hd * 2 * sizeof(kv) per (row, KV head), behind a chain of
 // about 10 us that every row has (lengths, ids, bounds, threshold, keys, join).  32 sequences of 4k to 32k tokens,
-// 32 / 8 heads of 128, 128 pages of 16: 87 us for 350 MB (4.0 TB/s); 24 sequences of up to 2k tokens, 12 heads of 64,
+// 32 / 8 heads of 128, 128 pages of 16: 82 us for 350 MB (4.3 TB/s); 24 sequences of up to 2k tokens, 12 heads of 64,
 // fp32 pools, 32 pages: 26 us for 70 MB; one sequence of 8k tokens: 13.8 us, the chain.
 
 #include <cooperative_groups.h>

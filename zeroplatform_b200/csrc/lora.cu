@@ -14,10 +14,11 @@
 //   chain A -> t -> B of one launch.  k = n = 4096: one row of rank 16 4.1 us; 64 rows of rank 64 12.6 us, 64 MB from
 //   L2 at 5.3 TB/s.
 // lora_tile_kernel (many rows, as in prefill): 64 rows per cluster on the tensor cores (mma.sync), x and t split into
-//   terms of the weights' type that hold fp32 to 2^-22 (Step).  x and A, then y and B, pass through one cp.async ring,
+//   terms of the weights' type that hold fp32 to 2^-22 (Step); the accumulator truncates, so 32 columns are summed there
+//   and the sums added with rounding (k 16,384: 2e-7 off instead of 2.4e-6, 1 us of 47).  x and A, then y and B, pass through one cp.async ring,
 //   whose second filling starts before the cluster has summed t.  The adapter that most of a tile's rows name is
 //   staged; warps whose rows name others fetch those weights themselves, the first one's a turn ahead.  2048 rows of
-//   rank 64 and one adapter, k = n = 4096: fp16 47 us, 2.1 TB/s of x, y and out; bound by the instructions and barriers
+//   rank 64 and one adapter, k = n = 4096: fp16 48 us, 2.1 TB/s of x, y and out; bound by the instructions and barriers
 //   of a turn (about 300 per warp and 64 columns, 14 warps an SM), not by HBM (16 us) or the tensor pipe (9 us).
 
 #include <cooperative_groups.h>
@@ -302,10 +303,9 @@ struct Step<__half> {
   }
   __device__ __forceinline__ void mma(float (&d)[4], const Raw<__half>& w) const {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      mma_f16(d, lo[i], word_of(w.a, 2 * i), word_of(w.a, 2 * i + 1));
-      mma_f16(d, hi[i], word_of(w.a, 2 * i), word_of(w.a, 2 * i + 1));
-    }
+    for (int i = 0; i < 2; ++i) mma_f16(d, lo[i], word_of(w.a, 2 * i), word_of(w.a, 2 * i + 1));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) mma_f16(d, hi[i], word_of(w.a, 2 * i), word_of(w.a, 2 * i + 1));
   }
 };
 template <>
@@ -330,9 +330,9 @@ struct Step<__nv_bfloat16> {
   }
   __device__ __forceinline__ void mma(float (&d)[4], const Raw<__nv_bfloat16>& w) const {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int k = 2; k >= 0; --k)
 #pragma unroll
-      for (int k = 2; k >= 0; --k) mma_bf16(d, t[k][i], word_of(w.a, 2 * i), word_of(w.a, 2 * i + 1));
+      for (int i = 0; i < 2; ++i) mma_bf16(d, t[k][i], word_of(w.a, 2 * i), word_of(w.a, 2 * i + 1));
   }
 };
 template <>
@@ -357,7 +357,11 @@ struct Step<float> {
       const uint32_t h0 = tf32_of(p.x), h1 = tf32_of(p.y);
       mma_tf32(d, hi[i], tf32_of(p.x - __uint_as_float(h0)), tf32_of(p.y - __uint_as_float(h1)));
       mma_tf32(d, lo[i], h0, h1);
-      mma_tf32(d, hi[i], h0, h1);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 p = pair_of(w, i);
+      mma_tf32(d, hi[i], tf32_of(p.x), tf32_of(p.y));
     }
   }
 };
@@ -559,7 +563,10 @@ __global__ void __launch_bounds__(LR_THREADS, sizeof(W) == 2 && NT <= 8 ? 2 : 1)
           if (8 * i < main_rank) {
             Raw<W> m;
             load_raw(wt + i * 8 * T::AROW, m);
-            s.mma(acc[i], m);
+            float d[4] = {0.f, 0.f, 0.f, 0.f};  // the tensor core's accumulator truncates: 32 columns a sum
+            s.mma(d, m);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[i][k] += d[k];
           }
       } else {
         // Sums of their own: what an adapter holds reaches its own rows only.
