@@ -601,6 +601,22 @@ def test_lora_long_sums_have_no_bias(dtype):
     assert abs(float((got.double() / want - 1).mean())) <= addends * 2.0 ** -23 + 2e-7
 
 
+@pytest.mark.parametrize("w", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("rows,adapters", [(300, 5), (1500, 600)])
+def test_lora_order_of_a_large_batch_does_not_matter(rows, adapters, w):
+    """Rows of tiles are sorted by adapter: any order of the batch gives every row the same bits, in place too."""
+    rng = np.random.default_rng(23)
+    x, y, a, b, adapter, ranks, scales = lora_case(rng, rows, 160, 70, 24, adapters, w, 1)
+    d, kw = (a.cuda(), b.cuda()), dict(ranks=dev(ranks), scales=dev(scales))
+    out = ops.lora_add(dev(y), dev(x), *d, dev(adapter), **kw).cpu().numpy()
+    want, mag = plain_lora(x, y, a, b, adapter, ranks, scales)
+    assert (np.abs(out - want) <= 1e-5 * mag).all() and (out[adapter < 0] == y[adapter < 0]).all()
+    for order in (np.argsort(adapter, kind="stable"), rng.permutation(rows)):
+        place = dev(y[order])
+        ops.lora_add(place, dev(x[order]), *d, dev(adapter[order]), out=place, **kw)
+        assert (place.cpu().numpy() == out[order]).all()
+
+
 def test_lora_same_rows_alone_and_in_a_batch():
     """A row's bits do not depend on what shares the batch (same form of the kernel)."""
     rng = np.random.default_rng(22)

@@ -13,12 +13,12 @@
 //   the adapters' bytes from L2 (each row reads its own; rows that share an adapter meet there), at small sizes the
 //   chain A -> t -> B of one launch.  k = n = 4096: one row of rank 16 4.1 us; 64 rows of rank 64 12.6 us, 64 MB from
 //   L2 at 5.3 TB/s.
-// lora_tile_kernel (many rows, as in prefill): 64 rows per cluster on the tensor cores (mma.sync), x and t split into
+// lora_tile_kernel (many rows, as in prefill): 64 rows per cluster, sorted by adapter, on the tensor cores (mma.sync), x and t split into
 //   terms of the weights' type that hold fp32 to 2^-22 (Step); the accumulator truncates, so 32 columns are summed there
-//   and the sums added with rounding (k 16,384: 2e-7 off instead of 2.4e-6, 1 us of 47).  x and A, then y and B, pass through one cp.async ring,
-//   whose second filling starts before the cluster has summed t.  The adapter that most of a tile's rows name is
+//   and the sums added with rounding (k 16,384: 2e-7 off instead of 2.4e-6, 1 us of 44).  x and A, then y and B, pass
+//   through one cp.async ring, whose second filling starts before the cluster has summed t.  The adapter that most of a tile's rows name is
 //   staged; warps whose rows name others fetch those weights themselves, the first one's a turn ahead.  2048 rows of
-//   rank 64 and one adapter, k = n = 4096: fp16 48 us, 2.1 TB/s of x, y and out; bound by the instructions and barriers
+//   rank 64 and one adapter, k = n = 4096: fp16 44 us, 2.3 TB/s of x, y and out; bound by the instructions and barriers
 //   of a turn (about 300 per warp and 64 columns, 14 warps an SM), not by HBM (16 us) or the tensor pipe (9 us).
 
 #include <cooperative_groups.h>
@@ -420,6 +420,69 @@ struct Tile {
   static_assert(LT_ROWS * TS * 4 <= STAGE, "t takes the last stage's place");
 };
 
+// The rows of a tile: LT_CHUNK rows at a time are put in the order of their adapters (those that share a bucket stay in
+// the batch's order, rows without an adapter come last), so that a tile's rows name few of them whatever the batch's
+// order is: 2048 rows of rank 64, k = n = 4096, each with one of 12 adapters, take 56 us, in the batch's order 234.  A
+// stable counting sort that every CTA repeats for itself, about 1 us; a bucket may hold several adapters, which only
+// mixes them.  row[i] is the tile's i-th row, -1 behind the last one.  work: 8 x 256 counts.
+constexpr int LT_CHUNK = 1024;
+__device__ __forceinline__ void rows_of_tile(const LoraArgs& a, int tile, unsigned short* work, int (&row)[LT_ROWS]) {
+  static_assert(LR_THREADS == 256 && LT_CHUNK % (LR_WARPS * 32) == 0 && LT_CHUNK % LT_ROWS == 0, "");
+  constexpr int EACH = LT_CHUNK / LR_THREADS;
+  __shared__ int sums[LR_WARPS];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int chunk0 = tile / (LT_CHUNK / LT_ROWS) * LT_CHUNK, first = tile * LT_ROWS - chunk0;
+  int key[EACH], at[EACH];
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {  // a warp's rows in order: 32 j + lane
+    const int k = warp * (LT_CHUNK / LR_WARPS) + 32 * j + lane;
+    const int ad = k < a.rows - chunk0 ? adapter_of(a, chunk0 + k) : -2;
+    key[j] = ad >= 0 ? ad % 255 : ad == -1 ? 255 : -1;
+  }
+  unsigned short* mine = work + warp * 256;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) mine[lane + 32 * i] = 0;
+  if (tid < LT_ROWS) row[tid] = -1;
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    const unsigned same = __match_any_sync(0xffffffffu, key[j]);
+    const int before = key[j] >= 0 ? mine[key[j]] : 0;
+    at[j] = before + __popc(same & ((1u << lane) - 1));
+    __syncwarp();
+    if (key[j] >= 0 && (same >> lane) == 1u) mine[key[j]] = (unsigned short)(at[j] + 1);  // the last of them
+    __syncwarp();
+  }
+  __syncthreads();
+  int total = 0;  // of bucket tid; the warps' counts become what comes before them
+#pragma unroll
+  for (int w = 0; w < LR_WARPS; ++w) {
+    const int n = work[w * 256 + tid];
+    work[w * 256 + tid] = (unsigned short)total;
+    total += n;
+  }
+  int upto = total;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+  int start = upto - total;
+#pragma unroll
+  for (int w = 0; w < LR_WARPS; ++w) start += w < warp ? sums[w] : 0;
+#pragma unroll
+  for (int w = 0; w < LR_WARPS; ++w) work[w * 256 + tid] += (unsigned short)start;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    const int p = key[j] >= 0 ? mine[key[j]] + at[j] - first : -1;
+    if (p >= 0 && p < LT_ROWS) row[p] = chunk0 + warp * (LT_CHUNK / LR_WARPS) + 32 * j + lane;
+  }
+  __syncthreads();
+}
+
 template <typename W, int NT>
 __global__ void __launch_bounds__(LR_THREADS, sizeof(W) == 2 && NT <= 8 ? 2 : 1) lora_tile_kernel(LoraArgs a) {
   using T = Tile<W, NT>;
@@ -427,16 +490,17 @@ __global__ void __launch_bounds__(LR_THREADS, sizeof(W) == 2 && NT <= 8 ? 2 : 1)
   extern __shared__ __align__(16) unsigned char smem[];
   float* t = reinterpret_cast<float*>(smem + (LT_STAGES - 1) * T::STAGE);  // [LT_ROWS][TS]
   float* part = reinterpret_cast<float*>(smem + LT_STAGES * T::STAGE);     // [LT_ROWS][TS]: this CTA's part of k
-  __shared__ int ids[LT_ROWS];
+  __shared__ int ids[LT_ROWS], rows[LT_ROWS];
   __shared__ int s_main;
   pdl_trigger();
   pdl_wait();
   cg::cluster_group cluster = cg::this_cluster();
   const int cr = cluster.block_rank(), C = cluster.num_blocks();
-  const int row0 = (int)(blockIdx.x / C) * LT_ROWS, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, c = lane & 3;
   const int mt = warp & 3, half = warp >> 2;  // 16 rows, and a half of every 64 k or of the columns
-  if (tid < LT_ROWS) ids[tid] = adapter_of(a, row0 + tid);
+  rows_of_tile(a, (int)(blockIdx.x / C), reinterpret_cast<unsigned short*>(smem), rows);
+  if (tid < LT_ROWS) ids[tid] = rows[tid] >= 0 ? adapter_of(a, rows[tid]) : -1;
   if (tid == 0) s_main = 0;
   __syncthreads();
   if (tid < LT_ROWS && ids[tid] >= 0) {  // the adapter that most rows name, the lowest row among equals
@@ -449,7 +513,7 @@ __global__ void __launch_bounds__(LR_THREADS, sizeof(W) == 2 && NT <= 8 ? 2 : 1)
   // Its weights are staged with the rows; a warp whose rows name others fetches those weights itself.
   const int main_ad = s_main ? ids[LT_ROWS - 1 - s_main % LT_ROWS] : -1;
   const int main_rank = main_ad >= 0 ? rank_of(a, main_ad) : 0;
-  const int la = mt * 16 + g, lb = la + 8, ra = row0 + la, rb = row0 + lb;
+  const int la = mt * 16 + g, lb = la + 8, ra = rows[la], rb = rows[lb];
   const int ida = ids[la], idb = ids[lb];
   const unsigned low_id = __reduce_min_sync(0xffffffffu, min((unsigned)ida, (unsigned)idb));  // -1 is the highest
   const int high_id = __reduce_max_sync(0xffffffffu, max(ida, idb));
@@ -475,7 +539,8 @@ __global__ void __launch_bounds__(LR_THREADS, sizeof(W) == 2 && NT <= 8 ? 2 : 1)
   unsigned have = 0;  // bit i: row r16 + 16 i has an adapter
 #pragma unroll
   for (int i = 0; i < XN; ++i) have |= (ids[r16 + XROWS * i] >= 0 ? 1u : 0u) << i;
-  const float* x_src = a.x + (size_t)(row0 + r16) * a.x_stride + cr * LT_K + p16 * 4;
+  auto row_at = [&](int i) { return (size_t)max(rows[r16 + XROWS * i], 0); };
+  const float* x_src = a.x + cr * LT_K + p16 * 4;
   const W* a_src = reinterpret_cast<const W*>(a.a) + ((size_t)max(main_ad, 0) * a.rank + wr) * a.k + cr * LT_K + wp * EPP;
   unsigned char* const x_dst = smem + r16 * LT_XROW + p16 * 16;
   unsigned char* const a_dst = smem + LT_ROWS * LT_XROW + wr * T::AROW + wp * 16;
@@ -485,7 +550,7 @@ __global__ void __launch_bounds__(LR_THREADS, sizeof(W) == 2 && NT <= 8 ? 2 : 1)
       const bool in_x = p16 * 4 < k_left, in_a = wp * EPP < k_left;
 #pragma unroll
       for (int i = 0; i < XN; ++i)
-        copy16(x_dst + fill * T::STAGE + i * XROWS * LT_XROW, x_src + (size_t)i * XROWS * a.x_stride,
+        copy16(x_dst + fill * T::STAGE + i * XROWS * LT_XROW, x_src + row_at(i) * a.x_stride,
                in_x && (have >> i & 1u));
 #pragma unroll
       for (int i = 0; i < AN; ++i)
@@ -623,8 +688,8 @@ __global__ void __launch_bounds__(LR_THREADS, sizeof(W) == 2 && NT <= 8 ? 2 : 1)
   unsigned need = 0;  // bit i: row r16 + 16 i passes through
 #pragma unroll
   for (int i = 0; i < XN; ++i)
-    need |= (row0 + r16 + XROWS * i < a.rows && (move || ids[r16 + XROWS * i] >= 0) ? 1u : 0u) << i;
-  const float* y_src = a.y + (size_t)(row0 + r16) * a.y_stride + cr * 64 + p16 * 4;
+    need |= (rows[r16 + XROWS * i] >= 0 && (move || ids[r16 + XROWS * i] >= 0) ? 1u : 0u) << i;
+  const float* y_src = a.y + cr * 64 + p16 * 4;
   const W* b_src = reinterpret_cast<const W*>(a.b) + ((size_t)max(main_ad, 0) * a.n + cr * 64 + br) * a.rank + bp * EPP;
   unsigned char* const b_dst = smem + LT_ROWS * LT_XROW + br * T::BROW + bp * 16;
   int n_left = a.n - cr * 64;
@@ -635,7 +700,7 @@ __global__ void __launch_bounds__(LR_THREADS, sizeof(W) == 2 && NT <= 8 ? 2 : 1)
       const int in = n_left - p16 * 4;  // columns from this piece's first
 #pragma unroll
       for (int i = 0; i < XN; ++i) {
-        const float* from = y_src + (size_t)i * XROWS * a.y_stride;
+        const float* from = y_src + row_at(i) * a.y_stride;
         if (y16 && in >= 4) {
           copy16(to + i * XROWS * LT_XROW, from, need >> i & 1u);
         } else {
@@ -709,10 +774,10 @@ __global__ void __launch_bounds__(LR_THREADS, sizeof(W) == 2 && NT <= 8 ? 2 : 1)
 #pragma unroll
     for (int q = 0; q < STEPS; ++q) s[q].split(va[q], vb[q]);
   }
-  float* oa = a.out + (size_t)ra * a.out_stride;
-  float* ob = a.out + (size_t)rb * a.out_stride;
+  float* oa = a.out + (size_t)max(ra, 0) * a.out_stride;
+  float* ob = a.out + (size_t)max(rb, 0) * a.out_stride;
   constexpr int AT = STEPS * (int)sizeof(W) > 4 ? 1 : 4;  // column tiles whose weights are fetched at once
-  const bool wa = ra < a.rows && (ida >= 0 || move), wb = rb < a.rows && (idb >= 0 || move);
+  const bool wa = ra >= 0 && (ida >= 0 || move), wb = rb >= 0 && (idb >= 0 || move);
   __syncthreads();  // t is in registers
   const bool ragged = main_rank % 8 != 0;  // the last piece of B's rows holds ranks that are not this adapter's
   const bool bare = __any_sync(0xffffffffu, ida < 0 || idb < 0);
@@ -845,9 +910,10 @@ int launch_tile(const LoraArgs& a, cudaStream_t s) {
 
 template <typename W, int LG>
 int launch(const LoraArgs& a, cudaStream_t s) {
-  // A cluster per row up to 256 rows: 0.15 us a row of rank 64 (0.06 of rank 16; k = n = 4096), whatever adapters the
-  // rows use.  Tiles take 29 us (20) for 64 to 256 rows of runs and 38 (27) for 1024, but 130 (75) where every row has
-  // an adapter of its own, which only the device knows: 256 rows of rank 64 are 39 us against 29 or 132.
+  // A cluster per row up to 256 rows, whatever adapters they use: 256 rows of rank 64, k = n = 4096 take 34 us with 8
+  // adapters and 56 with 64 (of rank 16: 14 and 16).  Tiles take 31 us (22) for 64 to 256 rows in runs and 40 (29) for
+  // 1024, and where each row names one of 8 or 64 adapters 48 and 150 (33 and 81) for 256 rows, 88 (61) for 1024 and 64:
+  // how many meet in a tile only the device knows.
   return a.rows <= 256 ? launch_row<W, LG>(a, s) : launch_tile<W, LG>(a, s);
 }
 
