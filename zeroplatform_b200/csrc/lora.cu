@@ -13,13 +13,14 @@
 //   the adapters' bytes from L2 (each row reads its own; rows that share an adapter meet there), at small sizes the
 //   chain A -> t -> B of one launch.  k = n = 4096: one row of rank 16 4.1 us; 64 rows of rank 64 12.6 us, 64 MB from
 //   L2 at 5.3 TB/s.
-// lora_tile_kernel (many rows, as in prefill): 64 rows per cluster, sorted by adapter, on the tensor cores (mma.sync), x and t split into
-//   terms of the weights' type that hold fp32 to 2^-22 (Step); the accumulator truncates, so 32 columns are summed there
-//   and the sums added with rounding (k 16,384: 2e-7 off instead of 2.4e-6, 1 us of 44).  x and A, then y and B, pass
-//   through one cp.async ring, whose second filling starts before the cluster has summed t.  The adapter that most of a tile's rows name is
-//   staged; warps whose rows name others fetch those weights themselves, the first one's a turn ahead.  2048 rows of
-//   rank 64 and one adapter, k = n = 4096: fp16 44 us, 2.3 TB/s of x, y and out; bound by the instructions and barriers
-//   of a turn (about 300 per warp and 64 columns, 14 warps an SM), not by HBM (16 us) or the tensor pipe (9 us).
+// lora_tile_kernel (many rows, as in prefill): 64 rows per cluster, sorted by adapter, on the tensor cores (mma.sync), x
+//   and t split into terms of the weights' type that hold fp32 to 2^-22 (Step); the accumulator truncates, so 32 columns
+//   are summed there and the sums added with rounding (k 16,384: 2e-7 off instead of 2.4e-6, 1 us of 44).  x and A, then
+//   y and B, pass through one cp.async ring, whose second filling starts before the cluster has summed t.  The adapter
+//   that most of a tile's rows name is staged; warps whose rows name others fetch those weights themselves, the first
+//   one's a turn ahead.  2048 rows of rank 64 and one adapter, k = n = 4096: fp16 44 us, 2.3 TB/s of x, y and out; bound
+//   by the instructions and barriers of a turn (about 300 per warp and 64 columns, 14 warps an SM), not by HBM (16 us)
+//   or the tensor pipe (9 us).
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
