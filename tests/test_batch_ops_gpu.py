@@ -488,6 +488,48 @@ def test_sparse_attention_long_sums_have_no_bias(dtype):
     assert abs(float((out.double() / want - 1).mean())) <= addends * 2.0 ** -23 + 1e-7
 
 
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("batch", [1, 20, 80])
+@pytest.mark.parametrize("hq,hkv,hd,every", [(1, 1, 64, 1 << 20), (8, 2, 128, 128), (2, 2, 256, 1 << 20), (12, 1, 64, 16)])
+def test_sparse_attention_rows_carried_by_small_weights(hq, hkv, hd, every, batch, half):
+    """Tokens of value 0 (every `every`-th one) take nearly all of the softmax and give nothing to the output, which is
+    the sum of weights 12 to 30 nats below them: attention sinks.  Every other value lies in [0.5, 1.5], so outputs have no
+    cancellation and are compared relative to themselves.  A score is off by at most hd roundings of 2^-23 of the terms
+    it adds (|q| |k| scale <= gap + 2), which moves a weight by as much relatively, here in the numerator and in the
+    sink's weight; sums over T tokens add T / 8 roundings of 2^-23 and a constant, which holds a weight's two halves.
+    Weights of fp16 pools are held to 2^-50 of the largest one among 16 neighbours, where those have a sink among them."""
+    rng = np.random.default_rng(hq * hd + batch)
+    page, tokens = 16, 2040
+    n = -(-tokens // page)
+    dt = np.float16 if half else np.float32
+    k = np.zeros((n, hkv, page, hd), dt)
+    k[..., 1] = (-2 * rng.random((n, hkv, page))).astype(dt)
+    v = (0.5 + rng.random((n, hkv, page, hd))).astype(dt)
+    flat_k, flat_v = k.transpose(0, 2, 1, 3).reshape(n * page, hkv, hd).copy(), \
+        v.transpose(0, 2, 1, 3).reshape(n * page, hkv, hd).copy()
+    sinks = np.arange(3, tokens, every)
+    flat_k[sinks, :, 0], flat_k[sinks, :, 1], flat_v[sinks] = 1, 0, 0
+    k = flat_k.reshape(n, page, hkv, hd).transpose(0, 2, 1, 3)
+    v = flat_v.reshape(n, page, hkv, hd).transpose(0, 2, 1, 3)
+    gaps = np.linspace(12, 30, batch * hq).reshape(batch, hq) if batch > 1 else np.linspace(16, 22, hq)[None]
+    q = np.zeros((batch, hq, hd), np.float32)
+    q[..., 0], q[..., 1] = gaps, 1
+    codes, scales = key_bounds(k)
+    table = np.tile(np.arange(n, dtype=np.int32), (batch, 1))
+    out, _ = ops.sparse_paged_attention(dev(q), dev(k), dev(v), dev(codes), dev(scales), dev(table), ints([tokens] * batch),
+                                        n, scale=1.0)
+    out = out.cpu().numpy()
+    group = hq // hkv
+    for b in range(batch):
+        for h in range(hq):
+            ref, _ = plain_attention(q[b, h:h + 1], flat_k[:tokens, h // group], flat_v[:tokens, h // group], 1.0)
+            tol = 2 * hd * 2.0 ** -23 * (gaps[b, h] + 2) + (tokens / 8 + 64) * 2.0 ** -23
+            if half:
+                tol += min(1, 16 * len(sinks) / tokens) * 2.0 ** -50 * np.exp(gaps[b, h] + 2)
+            err = np.abs(out[b, h] / ref[0] - 1).max()
+            assert err <= tol, (b, h, gaps[b, h], err, tol)
+
+
 def test_sparse_attention_in_a_captured_graph():
     rng = np.random.default_rng(13)
     ctx = [600, 350]

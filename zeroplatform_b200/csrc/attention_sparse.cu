@@ -18,7 +18,8 @@
 //           select on the order-preserving bits, and takes its part of the chosen pages, in page order.
 //   attend  mma m16n8k16 on the raw fp16 keys and values, from the same buffer, with the fp32 query as hi + lo halves in
 //           rows 0-7 and 8-15 (a power of two of its own brings each head's query into fp16's range) and the fp32
-//           weights split the same way: products are exact and the result is fp32 to about 2^-22.  The accumulator
+//           weights split likewise, relative to the block's largest one: products are exact, and scores and weights
+//           hold fp32 to about 2^-22 (weights down to 2^-28 of their 16 neighbours' largest).  The accumulator
 //           layout of q.k is the operand layout of p.v, and the contraction index is permuted alike on both sides, so
 //           operands are 16-byte reads and nothing is exchanged between lanes but the row maxima.  fp32 pools take
 //           the same path with tf32 hi + lo pairs of both sides.
@@ -48,6 +49,7 @@ constexpr int SP_THREADS = SP_WARPS * 32;
 constexpr int SP_CLUSTER = 8;  // most CTAs of a cluster
 constexpr int SP_HEADS = 8;  // query heads per pass: half of an mma's 16 rows
 constexpr float SP_LOG2E = 1.4426950408889634f;
+constexpr float SP_P_BITS = 14.f, SP_LO = 2048.f;  // fp16 pools: power of two of a block's weights, factor of their lo halves
 constexpr size_t SP_SMEM_MAX = 220 * 1024;
 
 struct SparseDev {
@@ -195,10 +197,10 @@ struct State {
     m = -INFINITY;
     l = 0.f;
   }
-  // The new maximum over the tile's scores (N per lane); rescales what was summed so far.
+  // The new maximum over the tile's scores (N per lane), whose own maximum is t; rescales what was summed so far.
   template <int N>
-  __device__ float raise(const float (&s)[N]) {
-    float t = s[0];
+  __device__ float raise(const float (&s)[N], float& t) {
+    t = s[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) t = fmaxf(t, s[i]);
     t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
@@ -643,19 +645,28 @@ __global__ void __launch_bounds__(SP_THREADS, CTAS) sparse_attn_kernel(SparseDev
         copy_rows(k_lane, kbuf, off_next, nv_next, true);
       else
         copies_commit();  // an empty group, so that the wait below counts the same
-      const float base = st.raise(s);
+      float top;
+      const float base = st.raise(s, top);
       if constexpr (HALF) {
+        // fp16 ends at 2^-24, and a row may be carried by weights far below its largest one, whose value is 0 (an
+        // attention sink).  So a block's weights are relative to its own maximum, which gets 2^14 (SP_P_BITS); lo
+        // halves, below 2^3, are held times 2^11 (SP_LO).  That keeps 2^-22 of a weight down to 2^-28 of the largest
+        // among the block's 16 tokens, and 2^-50 of that one below.  `back` returns the block to the state's maximum.
+        const bool none = top == -INFINITY;
+        const float from = none ? 0.f : top - SP_P_BITS, back = none ? 0.f : exp2f(from - base);
         uint32_t p_hi[2], p_lo[2];
+        float sum = 0.f;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const float p0 = exp2f(s[2 * u] - base), p1 = exp2f(s[2 * u + 1] - base);
-          st.l += p0 + p1;
+          const float p0 = exp2f(s[2 * u] - from), p1 = exp2f(s[2 * u + 1] - from);
+          sum += p0 + p1;
           const __half2 h = __floats2half2_rn(p0, p1);
           const float2 hf = __half22float2(h);
-          const __half2 lo = __floats2half2_rn(p0 - hf.x, p1 - hf.y);
+          const __half2 lo = __floats2half2_rn((p0 - hf.x) * SP_LO, (p1 - hf.y) * SP_LO);
           p_hi[u] = *reinterpret_cast<const uint32_t*>(&h);
           p_lo[u] = *reinterpret_cast<const uint32_t*>(&lo);
         }
+        st.l = fmaf(sum, back, st.l);
         copies_wait<1>();  // the values
         __syncwarp();
 #pragma unroll
@@ -672,8 +683,8 @@ __global__ void __launch_bounds__(SP_THREADS, CTAS) sparse_attn_kernel(SparseDev
             const uint32_t b1 = __byte_perm(word(v[2], e / 2), word(v[3], e / 2), e & 1 ? 0x7632 : 0x5410);
             float d[4] = {0.f, 0.f, 0.f, 0.f};
             mma_f16(d, p_hi[0], p_lo[0], p_hi[1], p_lo[1], b0, b1);
-            st.acc[8 * j + e][0] += d[0] + d[2];
-            st.acc[8 * j + e][1] += d[1] + d[3];
+            st.acc[8 * j + e][0] = fmaf(fmaf(d[2], 1.f / SP_LO, d[0]), back, st.acc[8 * j + e][0]);
+            st.acc[8 * j + e][1] = fmaf(fmaf(d[3], 1.f / SP_LO, d[1]), back, st.acc[8 * j + e][1]);
           }
         }
       } else {
