@@ -530,6 +530,19 @@ def test_sparse_attention_rows_carried_by_small_weights(hq, hkv, hd, every, batc
             assert err <= tol, (b, h, gaps[b, h], err, tol)
 
 
+@pytest.mark.parametrize("half", [True, False])
+def test_sparse_attention_cuts_lengths_to_max_ctx(half):
+    """A length above max_ctx counts as max_ctx, which need not end a page; the tokens behind it are there."""
+    rng = np.random.default_rng(14)
+    ctx = [200, 100, 99, 640, 7]
+    q, k, v, codes, scales, table, d = sparse_case(rng, ctx, 8, 2, 64, 16, half)
+    for max_ctx in (0, 1, 15, 16, 100, 109, 333):
+        cut = [min(x, max_ctx) for x in ctx]
+        for budget in (4, 40):
+            out, sel = ops.sparse_paged_attention(dev(q), *d, ints(ctx), budget, max_ctx=max_ctx)
+            check_sparse(q, k, v, codes, scales, table, cut, budget, 1, 1, out, sel)
+
+
 def test_sparse_attention_in_a_captured_graph():
     rng = np.random.default_rng(13)
     ctx = [600, 350]

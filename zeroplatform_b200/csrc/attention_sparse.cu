@@ -259,9 +259,9 @@ __global__ void __launch_bounds__(SP_THREADS, CTAS) sparse_attn_kernel(SparseDev
   const int b = (int)(pair / a.hkv), kvh = (int)(pair % a.hkv);
   const int P = a.page_size, group = a.hq / a.hkv;
   const int row = a.rows ? a.rows[b] : b;
-  int ctx = (unsigned)row < (unsigned)a.table_rows ? max(a.ctx_len[b], 0) : 0;
-  const int n = (int)min(((long long)ctx + P - 1) / P, (long long)dv.cap_pages);
-  ctx = min(ctx, (int)min((long long)n * P, 0x7fffffffLL));
+  int ctx = (unsigned)row < (unsigned)a.table_rows ? min(max(a.ctx_len[b], 0), a.max_ctx) : 0;
+  const int n = min((ctx + P - 1) / P, dv.cap_pages);  // max_ctx and a page are within 2^30
+  ctx = (int)min((long long)ctx, (long long)n * P);    // a table shorter than max_ctx
   const int want = min(a.budget, n);
   const float* q = a.q + (size_t)b * a.q_stride + (size_t)kvh * group * HD;
   float* out = a.out + ((size_t)b * a.hq + (size_t)kvh * group) * HD;
