@@ -982,6 +982,128 @@ def test_operators_on_two_streams_at_once():
             assert torch.equal(a, b)
 
 
+def test_calls_from_two_host_threads():
+    """Calls whose kernels ask for different amounts of shared memory, from two threads at once: each is taken and gives
+    what it gives alone."""
+    import ctypes as C
+    import threading
+
+    from zeroplatform_b200 import _lib
+    L, page, hd = _lib.lib(), 16, 64
+    torch.manual_seed(7)
+
+    def sparse(max_ctx):
+        n = max_ctx // page
+        k = torch.randn((n, 1, page, hd), device="cuda").half()
+        codes, scales = (dev(x) for x in key_bounds(k.cpu().numpy()))
+        keep = [torch.randn((1, 1, hd), device="cuda"), k, codes, scales,
+                torch.arange(n, dtype=torch.int32, device="cuda"), ints([max_ctx]), torch.zeros((1, 1, hd), device="cuda"),
+                torch.zeros((1, 1, 8), dtype=torch.int32, device="cuda")]
+        q, k, codes, scales, table, ctx, out, sel = (t.data_ptr() for t in keep)
+
+        def call(stream, keep=keep):
+            return L.zcu_sparse_paged_attention(q, hd, k, k, 1, codes, scales, table, 1, None, ctx, out, sel, 1, 1, 1, hd,
+                                                page, n, n, page * hd, hd, page * hd, 0.125, max_ctx, 8, 1, 1, stream)
+        return call, keep[6]
+
+    def logits(vocab):
+        x = torch.randn((1, vocab), device="cuda")
+        out, rep = torch.zeros_like(x), torch.full((1,), 1.5, device="cuda")
+        past, plen = torch.randint(0, vocab, (1, 40000), device="cuda").int(), ints([40000])  # 32-bit counts
+        r = _lib.LogitsRules(past=past.data_ptr(), past_len=plen.data_ptr(), past_cap=40000, past_count=1,
+                             repetition=rep.data_ptr())
+
+        def call(stream, keep=(x, out, rep, past, plen)):
+            return L.zcu_process_logits(x.data_ptr(), 0, vocab, out.data_ptr(), vocab, 1, vocab, C.byref(r), stream)
+        return call, out
+
+    for pair in ((sparse(80000), sparse(240000)), (logits(200000), logits(400000))):
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        torch.cuda.synchronize()
+        alone = []
+        for (call, out), s in zip(pair, streams):
+            assert call(s.cuda_stream) == 0
+            torch.cuda.synchronize()
+            alone.append(out.clone())
+        go, bad = threading.Barrier(2), [[], []]
+
+        def work(i):
+            go.wait()
+            for turn in range(4000):
+                rc = pair[i][0](streams[i].cuda_stream)
+                if rc:
+                    bad[i].append((turn, rc))
+                if turn % 500 == 499:
+                    streams[i].synchronize()
+
+        threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert bad == [[], []]
+        for (_, out), ref in zip(pair, alone):
+            assert torch.equal(out, ref)
+
+
+_TRIM_THREADS = r"""
+#include <pthread.h>
+#include <stdint.h>
+typedef int32_t (*trim_t)(int32_t*, int32_t*, int32_t*, int32_t*, int32_t, int32_t, int32_t, int32_t, const int32_t*,
+                          const int32_t*, int32_t, void*);
+typedef int32_t (*sync_t)(void*);
+typedef struct {
+  trim_t trim;
+  sync_t sync;
+  int32_t* at[5];
+  int32_t batch, turns, bad;
+  void* stream;
+} work;
+static void* run(void* p) {
+  work* w = (work*)p;
+  for (int i = 0; i < w->turns; ++i) {
+    w->bad += w->trim(w->at[0], w->at[1], w->at[2], w->at[3], w->batch, 1, 1, 16, 0, w->at[4], w->batch, w->stream) != 0;
+    if (i % 256 == 255) w->bad += w->sync(w->stream) != 0;
+  }
+  return 0;
+}
+void both(work* w) {
+  pthread_t t[2];
+  for (int i = 0; i < 2; ++i) pthread_create(&t[i], 0, run, &w[i]);
+  for (int i = 0; i < 2; ++i) pthread_join(t[i], 0);
+}
+"""
+
+
+def test_calls_from_two_native_threads(tmp_path):
+    """The same without Python between the calls: two threads that free sequences of batches of two sizes."""
+    import ctypes as C
+    import subprocess
+
+    from zeroplatform_b200 import _lib
+    (tmp_path / "t.c").write_text(_TRIM_THREADS)
+    subprocess.run(["gcc", "-O1", "-shared", "-fPIC", "-pthread", str(tmp_path / "t.c"), "-o", str(tmp_path / "t.so")],
+                   check=True)
+
+    class Work(C.Structure):
+        _fields_ = [("trim", C.c_void_p), ("sync", C.c_void_p), ("at", C.c_void_p * 5), ("batch", C.c_int32),
+                    ("turns", C.c_int32), ("bad", C.c_int32), ("stream", C.c_void_p)]
+
+    sync = C.CFUNCTYPE(C.c_int32, C.c_void_p)(lambda s: torch.cuda.ExternalStream(s).synchronize() or 0)
+    streams, work, keep = [torch.cuda.Stream(), torch.cuda.Stream()], (Work * 2)(), []
+    for i, batch in enumerate((3000, 10000)):
+        pool = [torch.full((batch, 1), -1, dtype=torch.int32, device="cuda"), ints([0] * batch), ints([0]), ints([1]),
+                ints([0] * batch)]
+        keep.append(pool)
+        work[i] = Work(C.cast(_lib.lib().zcu_pages_trim, C.c_void_p), C.cast(sync, C.c_void_p),
+                       (C.c_void_p * 5)(*[t.data_ptr() for t in pool]), batch, 8192, 0, streams[i].cuda_stream)
+    torch.cuda.synchronize()
+    C.CDLL(str(tmp_path / "t.so")).both(work)
+    torch.cuda.synchronize()
+    assert [w.bad for w in work] == [0, 0]
+
+
 def test_operators_through_either_binding(monkeypatch):
     """What _dispatch takes and what goes through ctypes (its absence, a stream argument, tensor subclasses) is the same."""
     from zeroplatform_b200 import _lib

@@ -833,7 +833,7 @@ int launch(const SparseAttnArgs& a, cudaStream_t s) {
   // need); more pairs than SMs share them.  Outputs of 256 dims leave room for one only.
   const bool two = HD <= 128 && pairs * S > 148;
   auto kernel = two ? sparse_attn_kernel<HD, HALF, HD <= 128 ? 2 : 1> : sparse_attn_kernel<HD, HALF, 1>;
-  if (allow_smem(kernel, smem)) return kCudaError;
+  if (allow_smem(kernel, smem, SP_SMEM_MAX)) return kCudaError;
   return launch_cluster_pdl(kernel, dim3((unsigned)(pairs * S)), dim3(SP_THREADS), S, smem, s, d) == cudaSuccess
              ? kOk
              : kCudaError;

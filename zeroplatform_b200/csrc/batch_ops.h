@@ -133,11 +133,12 @@ inline cudaError_t launch_cluster_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 
 }
 
 // Raises a kernel's dynamic shared memory limit where dynamic and static memory (under 8 KB in these kernels) may
-// together pass the default 48 KB.
+// together pass the default 48 KB.  The limit belongs to the kernel, not to the launch that follows: it is raised to
+// `most`, what any call of the kernel asks for, so that a call on another host thread never lowers it in between.
 template <typename K>
-inline int allow_smem(K* kernel, size_t bytes) {
+inline int allow_smem(K* kernel, size_t bytes, size_t most) {
   if (bytes <= 40 * 1024) return 0;
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess ? 0 : -3;
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) == cudaSuccess ? 0 : -3;
 }
 
 }  // namespace zc

@@ -269,7 +269,7 @@ int launch(const LogitsArgs& a, cudaStream_t s) {
   const bool few = (long long)a.rows * ranks <= 256;
   auto kernel = few ? (vec ? logits_kernel<T, H, true, 512> : logits_kernel<T, H, false, 512>)
                     : (vec ? logits_kernel<T, H, true, 256> : logits_kernel<T, H, false, 256>);
-  if (allow_smem(kernel, smem)) return kCudaError;
+  if (allow_smem(kernel, smem, LG_SMEM_MAX)) return kCudaError;
   return launch_cluster_pdl(kernel, dim3(a.rows * ranks), dim3(few ? 512 : 256), ranks, smem, s, a, slice, in_place) ==
                  cudaSuccess
              ? kOk

@@ -902,7 +902,7 @@ int launch_tile(const LoraArgs& a, cudaStream_t s) {
   const int tiles = (a.rows + LT_ROWS - 1) / LT_ROWS;
   const size_t smem = Tile<W, NT>::BYTES;
   auto kernel = lora_tile_kernel<W, NT>;
-  if (allow_smem(kernel, smem)) return kCudaError;
+  if (allow_smem(kernel, smem, smem)) return kCudaError;
   if ((long long)tiles * LR_CLUSTER > 0x7fffffffLL) return kTooLarge;
   return launch_cluster_pdl(kernel, dim3(tiles * LR_CLUSTER), dim3(LR_THREADS), LR_CLUSTER, smem, s, a) == cudaSuccess
              ? kOk

@@ -300,7 +300,7 @@ int pages_reserve(const PagePool& p, const int32_t* rows, const int32_t* n_new, 
   if (smem > PG_SMEM_MAX) return kTooLarge;
   const Shape f = shape_for(batch, tokens);
   auto kernel = f.threads == 256 ? reserve_kernel<256> : reserve_kernel<1024>;
-  if (allow_smem(kernel, smem)) return kCudaError;
+  if (allow_smem(kernel, smem, PG_SMEM_MAX)) return kCudaError;
   return launch_cluster_pdl(kernel, dim3(f.cluster), dim3(f.threads), f.cluster, smem, s, p, rows, n_new, batch,
                             tokens, o) == cudaSuccess
              ? kOk
@@ -315,7 +315,7 @@ int pages_trim(const PagePool& p, const int32_t* rows, const int32_t* new_len, i
   if (smem > PG_SMEM_MAX) return kTooLarge;
   const Shape f = shape_for(batch, (long long)batch * 16);  // the host does not know how many pages go back
   auto kernel = f.threads == 256 ? trim_kernel<256> : trim_kernel<1024>;
-  if (allow_smem(kernel, smem)) return kCudaError;
+  if (allow_smem(kernel, smem, PG_SMEM_MAX)) return kCudaError;
   return launch_cluster_pdl(kernel, dim3(f.cluster), dim3(f.threads), f.cluster, smem, s, p, rows, new_len, batch) ==
                  cudaSuccess
              ? kOk
