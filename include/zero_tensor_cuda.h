@@ -380,7 +380,8 @@ ZC_API int32_t zcu_pages_trim(int32_t* page_table, int32_t* seq_len, int32_t* fr
  * bounds int8 [num_pages][hkv][2][hd] and scales fp32 [num_pages][hkv] (both or neither) receive, for every page
  * written, 8-bit bounds of its stored keys: scale = max|k| / 127, lo = floor(min k / scale), hi = ceil(max k / scale)
  * per dimension (0 for a page whose largest key is 0 or not finite).  A page holds its slots up to the last one that
- * the call writes; the tokens that a call writes to one page stand in consecutive entries and ascending slots.
+ * the call writes.  The tokens that a call writes to one page stand in ascending slots, gaps allowed, with no other page's
+ * tokens between them; skipped entries may stand anywhere.  -6 for more than 2^31 - 4097 tokens.
  * Pointers and strides in whole 4-element pieces (16 bytes of fp32, 8 of fp16). */
 ZC_API int32_t zcu_append_kv(const void* k, const void* v, int32_t in_dtype, int64_t k_stride, int64_t v_stride,
                              const int64_t* slots, int32_t tokens, void* k_pool, void* v_pool, int32_t kv_dtype,

@@ -275,6 +275,42 @@ def test_append_bounds_hold_the_keys_and_odd_values_stay_finite():
     assert (pools[0][4, 0, 0] == k[4, 0]).all()
 
 
+@pytest.mark.parametrize("src,dst", [("float32", "float16"), ("float16", "float32"), ("float32", "float32")])
+@pytest.mark.parametrize("hkv,hd,page,pages", [(2, 128, 16, 60), (1, 256, 8, 40), (12, 64, 64, 80), (3, 32, 200, 6),
+                                               (8, 128, 1, 30), (8, 256, 32, 90)])
+def test_append_pages_with_gaps_and_skipped_entries(hkv, hd, page, pages, src, dst):
+    """Tokens of a page in ascending slots that leave some out (which keep what they hold), with skipped entries, a few or
+    hundreds, between tokens of one page and of different ones: every row and every page's bounds as the host has
+    them."""
+    rng = np.random.default_rng(hkv * hd + page)
+    pool = [rng.standard_normal((pages, hkv, page, hd)).astype(dst) for _ in range(2)]
+    slots, last = [], {}
+    for p in rng.permutation(pages - 1):
+        for j in np.sort(rng.choice(page, rng.integers(1, page + 1), replace=False)):
+            if rng.random() < 0.25:
+                skipped = int(rng.choice([-1, -2 ** 40, pages * page, 2 ** 62]))
+                slots += [skipped] * int(rng.choice([1, 2, 40, 700], p=[0.6, 0.25, 0.13, 0.02]))
+            slots.append(int(p) * page + int(j))
+            last[p] = int(j) + 1
+    rows = [rng.standard_normal((len(slots), hkv, hd)).astype(src) for _ in range(2)]
+    kp, vp = dev(pool[0]), dev(pool[1])
+    bounds = torch.full((pages, hkv, 2, hd), 99, dtype=torch.int8, device="cuda")
+    scales = torch.full((pages, hkv), -7.0, device="cuda")
+    ops.append_kv(dev(rows[0]), dev(rows[1]), dev(np.array(slots, np.int64)), kp, vp, bounds, scales)
+    for t, s in enumerate(slots):
+        if 0 <= s < pages * page:
+            pool[0][s // page, :, s % page] = rows[0][t].astype(dst)
+            pool[1][s // page, :, s % page] = rows[1][t].astype(dst)
+    np.testing.assert_array_equal(kp.cpu().numpy(), pool[0])
+    np.testing.assert_array_equal(vp.cpu().numpy(), pool[1])
+    got_b, got_s = bounds.cpu().numpy(), scales.cpu().numpy()
+    for p in range(pages - 1):
+        want_b, want_s = key_bounds(pool[0][p, :, :last[p]])
+        np.testing.assert_array_equal(got_s[p], want_s)
+        np.testing.assert_array_equal(got_b[p], want_b)
+    assert (got_b[-1] == 99).all() and (got_s[-1] == -7).all()
+
+
 def test_append_without_bounds_and_of_nothing():
     k = torch.randn((3, 2, 128), device="cuda")
     pools = [torch.zeros((4, 2, 16, 128), device="cuda", dtype=torch.float16) for _ in range(2)]

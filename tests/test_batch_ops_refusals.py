@@ -64,6 +64,10 @@ def test_append_covers_four_head_sizes():
     assert append(tokens=0, k=None, v=None, slots=None) == 0
 
 
+def test_append_refuses_more_tokens_than_it_indexes():
+    assert append(tokens=2 ** 31 - 4096) == -6 and append(tokens=2 ** 31 - 1) == -6
+
+
 def sparse(q=P, qs=1024, kp=P, vp=P, kv_dtype=1, bounds=P, scales=P, table=P, table_rows=2, rows=None, ctx=P, out=P,
            sel=P, batch=2, hq=8, hkv=2, hd=128, page=16, max_pages=64, pages=128, sp=4096, ss=128, sh=2048,
            max_ctx=1024, budget=8, sink=1, recent=1):

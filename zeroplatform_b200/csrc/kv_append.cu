@@ -7,8 +7,9 @@
 // so that lo * s <= k <= hi * s (a largest |k| that the rounding of s leaves an ulp outside is clamped to 127).  The
 // quotients are floored exactly: the sign of the fused residual tells on which side of an integer the real one lies.
 //
-// One warp takes one run of tokens (consecutive slots of one page) of one head: it stores the run, keeps the running
-// min and max in registers, adds the keys that the page held before, and writes the codes.  The keys are therefore
+// One warp takes all tokens of one page and one head, run by run (consecutive entries in consecutive slots; entries that
+// are skipped and gaps between slots may lie between runs): it stores a run, keeps the running min and max in
+// registers, adds the keys that the page held before, and writes the codes after the last run.  The keys are therefore
 // read once and the bounds need no state of their own, no atomics and no second pass.  Bound: HBM for prompts
 // (8 bytes of input and 4 of pool per element with fp32 rows and fp16 pools), latency for single tokens.
 
@@ -24,6 +25,7 @@ namespace {
 constexpr int KA_WARPS = 8;
 constexpr int KA_UNROLL = 4;  // token rows of K and V in flight per lane
 constexpr int KA_HELD = 8;    // stored keys likewise
+constexpr int KA_SKIP = 32;   // windows of 32 slots likewise, over skipped entries
 
 // Four elements of a row as they lie in memory.
 template <typename T>
@@ -79,6 +81,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) kv_append_kernel(KvAppendArg
   constexpr int LPR = VEC < 32 ? VEC : 32;          // lanes per row
   constexpr int ROWS = 32 / LPR;                    // rows a warp takes at once
   constexpr int PCS = VEC / LPR;                    // pieces per lane
+  // rows: fp32 rows of 256 dims would spill with as many as 128 take
+  constexpr int UNROLL = sizeof(IN) == 4 ? KA_UNROLL / PCS : KA_UNROLL, HELD = KA_HELD / PCS;
   pdl_trigger();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -92,27 +96,59 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) kv_append_kernel(KvAppendArg
   const IN* kin = reinterpret_cast<const IN*>(a.k) + (size_t)h * HD + col;
   const IN* vin = reinterpret_cast<const IN*>(a.v) + (size_t)h * HD + col;
 
-  for (int t = t_begin; t < t_end;) {
-    const int64_t slot = a.slots[t];
-    if (slot < 0 || slot >= pool_slots) {
-      ++t;
-      continue;
+  auto slot_at = [&](int t) -> int64_t {  // -1 where an entry is skipped or there is none
+    const int64_t s = (unsigned)t < (unsigned)a.tokens ? a.slots[t] : -1;
+    return s < pool_slots ? s : -1;
+  };
+  // Over skipped entries, which may be many: windows at, at +- 32, .. of 32 entries (at +- lane), up to the first that has
+  // an entry; w: that window.  Returns its start, outside [0, tokens) if none.  Padding is negative, which the high
+  // words tell: KA_SKIP windows of them are on their way at once.
+  auto look = [&](int at, int step, int64_t& w) {
+    for (;;) {
+      int high[KA_SKIP];
+#pragma unroll
+      for (int u = 0; u < KA_SKIP; ++u) {
+        const int t = at + step * (32 * u + lane);
+        high[u] = (unsigned)t < (unsigned)a.tokens ? reinterpret_cast<const int*>(a.slots + t)[1] : -1;
+      }
+      int first = KA_SKIP;  // this lane's first window with a candidate
+#pragma unroll
+      for (int u = KA_SKIP - 1; u >= 0; --u)
+        if (high[u] >= 0) first = u;
+      first = __reduce_min_sync(0xffffffffu, first);
+      at += step * 32 * first;
+      if ((unsigned)at >= (unsigned)a.tokens) break;
+      if (first == KA_SKIP) continue;
+      w = slot_at(at + step * lane);
+      if (__any_sync(0xffffffffu, w >= 0)) return at;
+      at += 32 * step;  // slots behind the pool
     }
-    const int page = (int)(slot / P), s0 = (int)(slot - (int64_t)page * P);
-    // the run that this token continues, if any, belongs to its first token's warp
-    bool inner = false;
-    if (t == t_begin && t > 0) inner = s0 > 0 && a.slots[t - 1] == slot - 1;
-    const int most = min(P - s0, a.tokens - t);
-    int n = 1;
-    for (unsigned next = 0xffffffffu; next == 0xffffffffu;) {  // 32 slots of the run at a time
-      const int i = n + lane;
-      next = __ballot_sync(0xffffffffu, i < most && a.slots[t + i] == slot + i);
-      n += next == 0xffffffffu ? 32 : __ffs(~next) - 1;
+    w = -1;
+    return at;
+  };
+  int base = t_begin;
+  int64_t win = slot_at(base + lane);  // entries base .. base + 31, one a lane
+  int64_t w = slot_at(t_begin - 1 - lane);
+  unsigned mine = __ballot_sync(0xffffffffu, win >= 0 && lane < t_end - t_begin);
+  if (!mine) return;
+  int t = t_begin + __ffs(mine) - 1;
+  int64_t slot = __shfl_sync(0xffffffffu, win, t - base);
+  // A page belongs to the warp of its first entry: what continues the page of the entry before this tile is not ours.
+  if (t_begin > 32 && !__any_sync(0xffffffffu, w >= 0)) look(t_begin - 33, -1, w);
+  int page = (int)(slot / P);
+  int64_t page0 = (int64_t)page * P;
+  if (const unsigned some = __ballot_sync(0xffffffffu, w >= 0)) {
+    const int64_t prev = __shfl_sync(0xffffffffu, w, __ffs(some) - 1);
+    if ((uint64_t)(prev - page0) < (uint64_t)P) {
+      mine &= __ballot_sync(0xffffffffu, (uint64_t)(win - page0) >= (uint64_t)P);
+      if (!mine) return;
+      t = t_begin + __ffs(mine) - 1;
+      slot = __shfl_sync(0xffffffffu, win, t - base);
+      page = (int)(slot / P);
+      page0 = (int64_t)page * P;
     }
-    if (inner) {
-      t += n;
-      continue;
-    }
+  }
+  for (;;) {
     KV* kp = reinterpret_cast<KV*>(a.k_pool) + page * a.page_stride + h * a.head_stride + col;
     KV* vp = reinterpret_cast<KV*>(a.v_pool) + page * a.page_stride + h * a.head_stride + col;
     float4 lo[PCS], hi[PCS];
@@ -121,51 +157,77 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) kv_append_kernel(KvAppendArg
       lo[p] = make_float4(INFINITY, INFINITY, INFINITY, INFINITY);
       hi[p] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     }
-    // the run's first rows and the keys that earlier calls stored are on their way together
-    Row<IN> kr[KA_UNROLL][PCS], vr[KA_UNROLL][PCS];
-    auto load_run = [&](int i0) {
-#pragma unroll
-      for (int u = 0; u < KA_UNROLL; ++u) {
-        const int i = i0 + u * ROWS;
-        if (i < n)
-#pragma unroll
-          for (int p = 0; p < PCS; ++p) {
-            kr[u][p] = fetch(kin + (long long)(t + i) * a.k_stride + p * 128);
-            vr[u][p] = fetch(vin + (long long)(t + i) * a.v_stride + p * 128);
-          }
+    int seen = 0;  // slots of the page up to here are in lo and hi
+    do {
+      const int s0 = (int)(slot - page0), most = P - s0;
+      int n;  // tokens of this run
+      for (;;) {
+        const int i = base + lane - t;
+        const unsigned in = __ballot_sync(0xffffffffu, i <= 0 || (i < most && win == slot + i));
+        n = base - t + __ffs(~in) - 1;
+        if (in != 0xffffffffu) break;
+        base += 32;
+        win = slot_at(base + lane);
       }
-    };
-    load_run(sub);
-    if (a.bounds)
-      for (int i0 = sub; i0 < s0; i0 += ROWS * KA_HELD) {
-        Row<KV> hr[KA_HELD][PCS];
+      // the run's first rows and the keys that earlier calls stored are on their way together
+      Row<IN> kr[UNROLL][PCS], vr[UNROLL][PCS];
+      auto load_run = [&](int i0) {
 #pragma unroll
-        for (int u = 0; u < KA_HELD; ++u)
-          if (i0 + u * ROWS < s0)
+        for (int u = 0; u < UNROLL; ++u) {
+          const int i = i0 + u * ROWS;
+          if (i < n)
 #pragma unroll
-            for (int p = 0; p < PCS; ++p) hr[u][p] = fetch(kp + (long long)(i0 + u * ROWS) * a.slot_stride + p * 128);
+            for (int p = 0; p < PCS; ++p) {
+              kr[u][p] = fetch(kin + (long long)(t + i) * a.k_stride + p * 128);
+              vr[u][p] = fetch(vin + (long long)(t + i) * a.v_stride + p * 128);
+            }
+        }
+      };
+      load_run(sub);
+      const int end = t + n;  // the next entry, of this page or another
+      unsigned some = __ballot_sync(0xffffffffu, win >= 0 && base + lane >= end);
+      if (a.bounds)
+        for (int i0 = seen + sub; i0 < s0; i0 += ROWS * HELD) {
+          Row<KV> hr[HELD][PCS];
 #pragma unroll
-        for (int u = 0; u < KA_HELD; ++u)
-          if (i0 + u * ROWS < s0)
+          for (int u = 0; u < HELD; ++u)
+            if (i0 + u * ROWS < s0)
 #pragma unroll
-            for (int p = 0; p < PCS; ++p) widen(lo[p], hi[p], floats(hr[u][p]));
+              for (int p = 0; p < PCS; ++p) hr[u][p] = fetch(kp + (long long)(i0 + u * ROWS) * a.slot_stride + p * 128);
+#pragma unroll
+          for (int u = 0; u < HELD; ++u)
+            if (i0 + u * ROWS < s0)
+#pragma unroll
+              for (int p = 0; p < PCS; ++p) widen(lo[p], hi[p], floats(hr[u][p]));
+        }
+      for (int i0 = sub;;) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+          const int i = i0 + u * ROWS;
+          if (i < n)
+#pragma unroll
+            for (int p = 0; p < PCS; ++p) {
+              const long long at = (long long)(s0 + i) * a.slot_stride + p * 128;
+              widen(lo[p], hi[p], store4(kp + at, floats(kr[u][p])));
+              store4(vp + at, floats(vr[u][p]));
+            }
+        }
+        i0 += ROWS * UNROLL;
+        if (i0 >= n) break;
+        load_run(i0);
       }
-    for (int i0 = sub;;) {
-#pragma unroll
-      for (int u = 0; u < KA_UNROLL; ++u) {
-        const int i = i0 + u * ROWS;
-        if (i < n)
-#pragma unroll
-          for (int p = 0; p < PCS; ++p) {
-            const long long at = (long long)(s0 + i) * a.slot_stride + p * 128;
-            widen(lo[p], hi[p], store4(kp + at, floats(kr[u][p])));
-            store4(vp + at, floats(vr[u][p]));
-          }
+      seen = max(seen, s0 + n);
+      if (!some && base + 32 < a.tokens) {
+        base = look(base + 32, 1, win);
+        some = __ballot_sync(0xffffffffu, win >= 0);
       }
-      i0 += ROWS * KA_UNROLL;
-      if (i0 >= n) break;
-      load_run(i0);
-    }
+      if (!some) {  // no entry is left
+        t = a.tokens;
+        break;
+      }
+      t = base + __ffs(some) - 1;
+      slot = __shfl_sync(0xffffffffu, win, t - base);
+    } while ((uint64_t)(slot - page0) < (uint64_t)P);
     if (a.bounds) {
       float top = 0.f;
 #pragma unroll
@@ -202,7 +264,9 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) kv_append_kernel(KvAppendArg
         }
       if (lane == 0) a.scales[(size_t)page * a.hkv + h] = s;
     }
-    t += n;
+    if (t >= t_end) return;
+    page = (int)(slot / P);
+    page0 = (int64_t)page * P;
   }
 }
 
@@ -210,7 +274,7 @@ template <int HD, typename IN, typename KV>
 int launch(const KvAppendArgs& a, cudaStream_t s) {
   // Tokens per warp: it walks its tile's runs one after another, so single tokens while that leaves fewer than 64
   // warps an SM (a decode step), and a common page's worth of a prompt beyond, where most warps of a finer split would
-  // find that their token belongs to a run before it.
+  // find that their token belongs to a page before it.
   const int tile = (long long)a.tokens * a.hkv <= 148 * 64 ? 1 : 16;
   const long long units = (long long)((a.tokens + tile - 1) / tile) * a.hkv;
   const long long blocks = (units + KA_WARPS - 1) / KA_WARPS;
@@ -232,6 +296,7 @@ int launch_hd(const KvAppendArgs& a, cudaStream_t s) {
 int kv_append(const KvAppendArgs& a, cudaStream_t s) {
   if (a.tokens < 0 || a.hkv <= 0 || a.hd <= 0 || a.page_size <= 0 || a.num_pages <= 0) return kBadArgument;
   if (a.tokens == 0) return kOk;
+  if (a.tokens > 0x7fffffff - 4096) return kTooLarge;  // windows of slots reach past the last entry
   if (!a.k || !a.v || !a.slots || !a.k_pool || !a.v_pool || (!a.bounds != !a.scales)) return kBadArgument;
   // 4-element pieces of every row and 4-byte code words
   const size_t ia = a.half_input ? 8 : 16, pa = a.kv_half ? 8 : 16;
