@@ -357,7 +357,9 @@ ZC_API int32_t zcu_moe_forward(void* moe, const float* xnorm, const float* route
  * max_rows).  Its tokens are entries [start[b], start[b + 1]) of the step's token arrays, `tokens` long; its pages
  * come off the top of the stack, in request order.  granted[b] is 0, and nothing of the request changes, when its row
  * is out of range or named by an earlier request of the call, when it would pass max_pages pages or the end of the
- * token arrays, or when the stack does not hold its pages and those of the requests before it.  Per token: slots =
+ * token arrays, or when the stack does not hold its pages and those of the requests before it: after the first request
+ * that finds too few, all later ones are refused, those that need no page among them, so requests come in the order of
+ * their claim (decode before prompts).  Per token: slots =
  * page * page_size + slot, positions, token_rows (its table row) and ctx_len = position + 1; tokens of refused
  * requests and behind the last request get slot -1, position 0, row -1, ctx_len 0.
  * trim: row rows[b] keeps min(new_len[b], its length) tokens (0 frees the sequence); pages behind them go back to the

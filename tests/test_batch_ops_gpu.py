@@ -157,6 +157,20 @@ def test_pages_taken_back_leave_the_stack_as_it_was():
         assert torch.equal(a, b)
 
 
+def test_pages_run_out_for_a_request_and_all_behind_it():
+    """A prompt larger than the stack stops whoever comes after it, with or without a page to take; put last, it stops
+    nobody."""
+    pool = lambda: (torch.full((3, 8), -1, dtype=torch.int32, device="cuda"), ints([5, 0, 5]), ints([3, 1, 2, 0]),  # noqa: E731
+                    ints([2]))
+    d = pool()
+    d[0][0, 0], d[0][2, 0] = 2, 0
+    plan = ops.reserve_pages(*d, ints([1, 100, 1]), 16, tokens=102)
+    assert plan.granted.tolist() == [1, 0, 0] and d[1].tolist() == [6, 0, 5] and d[3].item() == 2
+    assert plan.slots[0].item() == 2 * 16 + 5 and (plan.slots[1:] == -1).all()
+    plan = ops.reserve_pages(*d, ints([1, 1, 100]), 16, rows=ints([0, 2, 1]), tokens=102)
+    assert plan.granted.tolist() == [1, 1, 0] and d[1].tolist() == [7, 0, 6] and d[3].item() == 2
+
+
 def test_pages_slots_pass_32_bits():
     """A pool of few pages that are very long: the slot is page * page_size in 64 bits."""
     page = 1 << 30

@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(PG_THREADS) reserve_kernel(PagePool p, const i
     const int m = pages_of((long long)q.old[b] + q.arg[b], P) - q.first[b];
     off += m;
     if (off > count)
-      q.first[b] = -1;  // refused, as every later request that needs a page
+      q.first[b] = -1;  // refused, as every later request, whether it needs a page or not
     else if (m > 0)
       atomicMax(&s_used, (int)off);
   }

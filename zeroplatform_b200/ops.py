@@ -308,7 +308,8 @@ def reserve_pages(page_table, seq_len, free_pages, free_count, n_new, page_size:
                   stream=None) -> PagePlan:
     """Block tables and slot maps from request lengths, on the device (zcu_pages_reserve): request b adds n_new[b]
     tokens to table row rows[b] (None: row b) of the pool (page_table [max_rows, max_pages], seq_len [max_rows], the
-    stack free_pages [num_pages] of *free_count ids; int32, updated in place).  `tokens` is the length of the step's
+    stack free_pages [num_pages] of *free_count ids; int32, updated in place).  The first request that finds too few pages
+    and all behind it are refused, so those with the first claim come first.  `tokens` is the length of the step's
     token arrays (room behind the last token is padding), taken from `out` (a PagePlan to write to) when that is
     given."""
     if out is None:
