@@ -1179,6 +1179,25 @@ def test_operators_through_either_binding(monkeypatch):
         assert torch.equal(a, b)
 
 
+def test_numbers_beyond_32_bits_raise():
+    """A size whose low 32 bits are a good one is refused by the functions, whichever binding they take."""
+    pool = (torch.full((1, 4), -1, dtype=torch.int32, device="cuda"), ints([0]), ints([0, 1, 2, 3]), ints([4]))
+    before = [t.clone() for t in pool]
+    for page in ((1 << 32) + 16, 16.0, "16"):
+        with pytest.raises(ZcError):
+            ops.reserve_pages(*pool, ints([3]), page, tokens=3)
+        with pytest.raises(ZcError):
+            ops.trim_pages(*pool, ints([0]), page)
+    k = torch.zeros((4, 1, 16, 64), device="cuda")
+    bounds, scales = torch.zeros((4, 1, 2, 64), dtype=torch.int8, device="cuda"), torch.zeros((4, 1), device="cuda")
+    args = (torch.zeros((1, 1, 64), device="cuda"), k, k, bounds, scales, pool[0], ints([3]), 2)
+    for bad in (dict(sink=(1 << 32) + 1), dict(recent=(1 << 32) + 1), dict(max_ctx=(1 << 32) + 16), dict(sink=1.0)):
+        with pytest.raises(ZcError):
+            ops.sparse_paged_attention(*args, **bad)
+    for a, b in zip(pool, before):
+        assert torch.equal(a, b)
+
+
 def test_dispatch_declines_what_it_must_not_take():
     """Wrong types, shapes, devices, strides and argument counts are declined before anything is enqueued."""
     from zeroplatform_b200 import _lib

@@ -135,6 +135,21 @@ def test_logits_refuses_a_vocabulary_that_no_cluster_holds():
     assert _lib.lib().zcu_process_logits(P, 0, 64, P, 64, 1, 64, None, None) == -2
 
 
+@pytest.mark.parametrize("call,good", [
+    (reserve, dict(max_rows=4, max_pages=8, num_pages=16, page=16, batch=2, tokens=8)),
+    (trim, dict(max_rows=4, max_pages=8, num_pages=16, page=16, batch=2)),
+    (append, dict(in_dtype=0, tokens=2, kv_dtype=1, hkv=2, hd=128, page=16, pages=4)),
+    (sparse, dict(kv_dtype=1, table_rows=2, batch=2, hq=8, hkv=2, hd=128, page=16, max_pages=64, pages=128, max_ctx=1024,
+                  budget=8, sink=1, recent=1)),
+    (lora, dict(w=1, rows=2, k=64, n=40, adapters=3, rank=8)), (logits, dict(dtype=0, rows=2, vocab=64))])
+def test_numbers_beyond_32_bits_are_refused_not_cut(call, good):
+    """ctypes keeps the low 32 bits of a larger number; 2^32 + 16 must not pass for a page size of 16."""
+    for name, v in good.items():
+        for off in (1 << 32, -(1 << 32), 1 << 63):
+            with pytest.raises(C.ArgumentError, match="32 bits"):
+                call(**{name: v + off})
+
+
 def test_dispatch_takes_cuda_tensors_only():
     """The binding module is built and loaded with the library; whatever it is given here it declines (host tensors, other
     objects, wrong counts), and the Python checks behind it name the fault."""

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from operator import index
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libzero_tensor.so")
@@ -157,15 +158,26 @@ class LogitsRules(C.Structure):
                 ("mask_stride", i64)]
 
 
+class n32:
+    """An int32 argument that refuses what 32 bits do not hold (ctypes' own keeps the low bits)."""
+
+    @staticmethod
+    def from_param(value):
+        value = index(value)
+        if not -0x80000000 <= value <= 0x7fffffff:
+            raise ValueError(f"{value} does not fit 32 bits")
+        return value
+
+
 SIGNATURES.update({
-    "zcu_pages_reserve": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, vp, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp]),
-    "zcu_pages_trim": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, vp, vp, i32, vp]),
-    "zcu_append_kv": (i32, [vp, vp, i32, i64, i64, vp, i32, vp, vp, i32, i32, i32, i32, i32, i64, i64, i64, vp, vp,
+    "zcu_pages_reserve": (i32, [vp, vp, vp, vp, n32, n32, n32, n32, vp, vp, n32, n32, vp, vp, vp, vp, vp, vp, vp]),
+    "zcu_pages_trim": (i32, [vp, vp, vp, vp, n32, n32, n32, n32, vp, vp, n32, vp]),
+    "zcu_append_kv": (i32, [vp, vp, n32, i64, i64, vp, n32, vp, vp, n32, n32, n32, n32, n32, i64, i64, i64, vp, vp,
                             vp]),
-    "zcu_sparse_paged_attention": (i32, [vp, i64, vp, vp, i32, vp, vp, vp, i32, vp, vp, vp, vp] + [i32] * 7 +
-                                   [i64, i64, i64, f32, i32, i32, i32, i32, vp]),
-    "zcu_lora_add": (i32, [vp, i64, vp, i64, vp, i64, vp, vp, i32, vp, vp, vp] + [i32] * 5 + [vp]),
-    "zcu_process_logits": (i32, [vp, i32, i64, vp, i64, i32, i32, C.POINTER(LogitsRules), vp]),
+    "zcu_sparse_paged_attention": (i32, [vp, i64, vp, vp, n32, vp, vp, vp, n32, vp, vp, vp, vp] + [n32] * 7 +
+                                   [i64, i64, i64, f32, n32, n32, n32, n32, vp]),
+    "zcu_lora_add": (i32, [vp, i64, vp, i64, vp, i64, vp, vp, n32, vp, vp, vp] + [n32] * 5 + [vp]),
+    "zcu_process_logits": (i32, [vp, n32, i64, vp, i64, n32, n32, C.POINTER(LogitsRules), vp]),
 })
 
 

@@ -240,11 +240,14 @@ _FLOAT_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 def _call(fn, what: str, device: int, stream, *args):
     """fn(*args, stream) on CUDA device `device`, whichever is current; the stream defaults to that device's current one."""
-    if device == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream)
-    else:
-        with torch.cuda.device(device):
+    try:
+        if device == torch._C._cuda_getDevice():
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream)
+        else:
+            with torch.cuda.device(device):
+                rc = fn(*args, torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream)
+    except C.ArgumentError as e:  # a number of the wrong kind or beyond 32 bits
+        raise ZcError(f"{what}: {e}") from None
     if rc:
         check(rc, what)
 
@@ -494,6 +497,8 @@ def process_logits(logits, out=None, past=None, past_len=None, prompt_len=None, 
     n, cap = (0, 0) if past is None else past.shape
     masks, words = (0, 0) if mask is None else mask.shape
     n_bias = 0 if bias is None else bias.shape[0]
+    if max(n, cap, masks, n_bias) > 0x7fffffff:
+        raise ZcError("past, mask and bias must have fewer than 2^31 rows and entries a row")
     if past is not None and past_rows is None and n < rows:
         raise ZcError(f"past has {n} rows for {rows} rows of logits and no past_rows")
     if (bias_start is None) != (bias is None) or (bias_ids is None) != (bias is None):
