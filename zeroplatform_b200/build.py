@@ -1,5 +1,5 @@
-"""Builds libzero_tensor.so (the C-ABI library with every CUDA kernel) in-tree for sm_100a, and _dispatch.so (the
-CPython module beside it).
+"""Builds libzero_tensor.so (the C-ABI library with every CUDA kernel) in-tree for sm_100a, and the CPython module
+_dispatch beside it.
 
     python -m zeroplatform_b200.build          # incremental
     python -m zeroplatform_b200.build --clean  # from scratch
@@ -16,13 +16,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libzero_tensor.so")
-DISPATCH = os.path.join(PKG, "_dispatch.so")
+DISPATCH = os.path.join(PKG, "_dispatch" + sysconfig.get_config_var("EXT_SUFFIX"))
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -72,24 +73,41 @@ def build(clean: bool = False, verbose_ptxas: bool = False) -> str:
     return LIB
 
 
-def build_dispatch() -> str:
-    """_dispatch.so: the CPython module that checks tensors and calls the serving-batch entries (csrc/dispatch.c)."""
-    import sysconfig
-
+def build_dispatch():
+    """The CPython module that checks tensors and calls the serving-batch entries (csrc/dispatch.c), for this interpreter
+    and PyTorch.  ops.py makes the same calls through ctypes without it, so where it does not compile (no gcc, a PyTorch
+    without the exchange table) this says so, leaves no module and returns None."""
     import torch
-    src = os.path.join(CSRC, "dispatch.c")
+
+    src, made_for = os.path.join(CSRC, "dispatch.c"), os.path.join(BUILD, "dispatch.torch")
     deps = [src, os.path.join(ROOT, "include", "zero_tensor_cuda.h")]
-    if os.path.exists(DISPATCH) and os.path.getmtime(DISPATCH) >= max(os.path.getmtime(p) for p in deps):
-        return DISPATCH
+    old = os.path.join(PKG, "_dispatch.so")  # an earlier build's, which any interpreter would load
+    if os.path.exists(old):
+        os.remove(old)
+    if os.path.exists(DISPATCH):
+        if os.path.getmtime(DISPATCH) >= max(os.path.getmtime(p) for p in deps) and os.path.exists(made_for):
+            with open(made_for) as f:
+                if f.read() == torch.__version__:
+                    return DISPATCH
+        os.remove(DISPATCH)
     inc = [sysconfig.get_paths()["include"], os.path.join(os.path.dirname(torch.__file__), "include")]
+    tmp = DISPATCH + ".tmp"
     cmd = ["gcc", "-O2", "-std=gnu11", "-shared", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wno-unused-parameter",
-           *[a for i in inc for a in ("-I", i)], src, "-o", DISPATCH + ".tmp", "-lm"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"gcc failed for {src}:\n{r.stdout}\n{r.stderr}")
-    if r.stderr:
-        sys.stderr.write(r.stderr)
-    os.replace(DISPATCH + ".tmp", DISPATCH)
+           *[a for i in inc for a in ("-I", i)], src, "-o", tmp, "-lm"]
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        failed, said = r.returncode != 0, r.stdout + r.stderr
+    except OSError as e:  # no gcc
+        failed, said = True, str(e)
+    if said:
+        sys.stderr.write(said.rstrip("\n") + "\n")
+    if failed:
+        sys.stderr.write(f"{os.path.basename(DISPATCH)} not built: its calls go through ctypes\n")
+        return None
+    os.replace(tmp, DISPATCH)
+    os.makedirs(BUILD, exist_ok=True)
+    with open(made_for, "w") as f:
+        f.write(torch.__version__)
     return DISPATCH
 
 
