@@ -1007,6 +1007,66 @@ def test_steps_of_a_mixed_batch(captured):
         same_pool(step.host, step.pool)
 
 
+def test_documented_step_runs():
+    """The step that the integration guide shows, as it stands there: a prompt step and a decode step with padding, checked
+    stage by stage on the stage's own inputs."""
+    import os
+    import re
+
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")).read()
+    code = re.search(r"```python\n(.*?)```", text[text.index("## 9. "):], re.S).group(1)
+    rng = np.random.default_rng(61)
+    f = lambda *s: dev(rng.standard_normal(s).astype(np.float32))  # noqa: E731
+    hq, hkv, hd, dim, vocab, T, max_pos = 4, 2, 64, 128, 320, 48, 64
+    weight = lambda n, k: ops.QuantizedWeight.upload(8, ops.quantize(8, f(n, k) / k ** 0.5), n, k)  # noqa: E731
+    host = Pool(rng, 5, 4, 20, 16)
+    angle = np.arange(max_pos)[:, None] * 10000.0 ** (-np.arange(hd // 2) * 2 / hd)
+    env = dict(zip(("page_table", "seq_len", "free_pages", "free_count"), upload(host)), rows=ints([4, 1, 2]), T=T, hq=hq,
+               hkv=hkv, hd=hd, max_pos=max_pos, cos=dev(np.cos(angle).astype(np.float32)),
+               sin=dev(np.sin(angle).astype(np.float32)), w_qkv=weight((hq + 2 * hkv) * hd, dim),
+               w_head=weight(vocab, hq * hd), lora_a=f(3, 8, dim) / dim ** 0.5, lora_b=f(3, (hq + 2 * hkv) * hd, 8),
+               lora_scale=f(3), k_pool=torch.zeros((20, hkv, 16, hd), dtype=torch.float16, device="cuda"),
+               v_pool=torch.zeros((20, hkv, 16, hd), dtype=torch.float16, device="cuda"),
+               bounds=torch.zeros((20, hkv, 2, hd), dtype=torch.int8, device="cuda"),
+               scales=torch.zeros((20, hkv), device="cuda"), history=dev(rng.integers(0, vocab, (5, 30)), torch.int32),
+               history_len=ints([30, 3, 0, 7, 12]), rep=torch.full((T,), 1.2, device="cuda"),
+               freq=torch.full((T,), 0.1, device="cuda"), pres=torch.full((T,), 0.1, device="cuda"),
+               grammar=torch.full((1, 10), -2, dtype=torch.int32, device="cuda"), state=ints([0] * T))
+    for new in ([30, 5, 9], [1, 2, 1]):
+        x, adapter = rng.standard_normal((T, dim)).astype(np.float32), rng.integers(-1, 3, T)
+        keep = host.lens[[4, 1, 2]] + new
+        env.update(x=dev(x), n_new=ints(new), adapter_of_token=ints(adapter), accepted_len=ints(keep))
+        exec(code, env)
+        want = host.reserve([4, 1, 2], new, T)
+        same_plan(env["plan"], want)
+        same_pool(host, tuple(env[n] for n in ("page_table", "seq_len", "free_pages", "free_count")))
+        dq = env["w_qkv"].qs.double() * env["w_qkv"].d.view(torch.float16).double().repeat_interleave(32, 1)
+        y = (env["x"].double() @ dq.t()).cpu().numpy()
+        ref, mag = plain_lora(x, y, env["lora_a"].cpu(), env["lora_b"].cpu(), adapter, [8] * 3,
+                              env["lora_scale"].tolist())
+        # the GEMM rounds each weight to fp16 (2^-11 of it): that much of the sum of the products' sizes
+        slack = np.abs(x).astype(np.float64) @ np.abs(dq.cpu().numpy().T) * 2.0 ** -11
+        assert (np.abs(env["qkv"].cpu().numpy() - ref) <= (64 * 2.0 ** -23 + 2.0 ** -21) * mag + slack).all()
+        z = env["qkv"].double().cpu().numpy().reshape(T, -1, hd)
+        a = angle[want[2]][:, None]
+        rot = np.stack([z[..., ::2] * np.cos(a) - z[..., 1::2] * np.sin(a),
+                        z[..., ::2] * np.sin(a) + z[..., 1::2] * np.cos(a)], -1).reshape(z.shape)
+        for name, part in (("q", rot[:, :hq]), ("k", rot[:, hq:hq + hkv]), ("v", z[:, hq + hkv:])):
+            assert np.abs(env[name].cpu().numpy() - part).max() <= 4 * 2.0 ** -24 * 1.5 * np.abs(z).max(), name
+        kv = [env[n].cpu().numpy() for n in ("k_pool", "v_pool")]
+        for t, s in enumerate(want[1]):
+            if s >= 0:
+                for i, n in enumerate("kv"):
+                    np.testing.assert_array_equal(kv[i][s // 16, :, s % 16], env[n][t].half().cpu().numpy())
+        check_sparse(env["q"].cpu().numpy(), *kv, env["bounds"].cpu().numpy(), env["scales"].cpu().numpy(), host.table,
+                     want[4], 128, 1, 4, env["out"], env["pages"], rows=want[3])
+        lg = env["logits"].cpu()
+        assert torch.isinf(lg[:, ::32]).all() and torch.isfinite(lg[:, 1:32]).all()
+        assert torch.equal(env["token"].cpu().long(), lg.argmax(1))
+        host.trim([4, 1, 2], keep)
+        same_pool(host, tuple(env[n] for n in ("page_table", "seq_len", "free_pages", "free_count")))
+
+
 def test_operators_on_two_streams_at_once():
     """Two steps on streams of their own, interleaved call by call, give what each gives alone."""
     def make(seed):
