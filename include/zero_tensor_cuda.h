@@ -403,6 +403,10 @@ ZC_API int32_t zcu_append_kv(const void* k, const void* v, int32_t in_dtype, int
  * score(page) = scale_page * max over the KV head's query heads of s_q * sum_d max(qi_d lo_d, qi_d hi_d), with
  * s_q = max|q| / 32512 and qi = rint(q / s_q): whole numbers summed exactly and two fp32 products, so the choice
  * does not depend on the launch; the lower page wins among equal scores.
+ * The attention is fp32 through pairs for the tensor cores.  A query element is held to 2^-22 of itself or 2^-32 of its
+ * head's largest (fp32 pools: 2^-22), keys and values of fp16 pools exactly and of fp32 pools to 2^-22, a softmax weight
+ * to 2^-22 (fp16 pools: down to 2^-28 of the largest among its block of 16 tokens, below to 2^-50 of that one).  A key or
+ * value that is not finite and is attended to makes its heads' outputs NaN or infinite.
  * hd 64, 128 or 256, page_size a multiple of 8 (else -4); -6 when a CTA's shared memory does not hold the scores of
  * max_ctx tokens and its part of the budget (44,000 pages at hd 64, 34,000 at 128, 14,000 at 256), or when max_ctx and a
  * page pass 2^30 tokens. */
@@ -419,9 +423,10 @@ ZC_API int32_t zcu_sparse_paged_attention(const float* q, int64_t q_stride, cons
  *   out[r] = y[r] + scales[e] * (x[r] A_e^T) B_e^T,  e = adapter[r];  a row whose adapter is outside [0, adapters): y[r]
  * x [rows][k_cols], y and out [rows][n_rows] fp32 with strides in elements; out may be y itself (no other overlap).
  * a [adapters][rank][k_cols] and b [adapters][n_rows][rank] (w_dtype 0 = fp32, 1 = fp16, 2 = bf16); of adapter e the
- * first ranks[e] of `rank` are used (NULL: all), scales NULL: 1.  fp32 arithmetic up to
- * 256 rows, beyond on the tensor cores with x and x A^T split into terms that hold fp32 to 2^-22; what another row or its
- * adapter holds, NaN included, does not reach a row.
+ * first ranks[e] of `rank` are used (NULL: all), scales NULL: 1.  fp32 arithmetic up to 256 rows, beyond on the tensor
+ * cores with x and x A^T split into terms that hold each element to 2^-22 (fp16 adapters: or to 2^-31 of the row's largest;
+ * fp32 adapters are split alike).  What another row or its adapter holds, NaN included, does not reach a row; where x or
+ * the adapter is not finite, neither is the row.
  * rank a multiple of 8 up to 128, k_cols a multiple of 32 (else -4); x, a and b 16-byte aligned, x_stride a multiple
  * of 4. */
 ZC_API int32_t zcu_lora_add(const float* x, int64_t x_stride, const float* y, int64_t y_stride, float* out,

@@ -18,9 +18,9 @@
 //   are summed there and the sums added with rounding (k 16,384: 2e-7 off instead of 2.4e-6, 1 us of 44).  x and A, then
 //   y and B, pass through one cp.async ring, whose second filling starts before the cluster has summed t.  The adapter
 //   that most of a tile's rows name is staged; warps whose rows name others fetch those weights themselves, the first
-//   one's a turn ahead.  2048 rows of rank 64 and one adapter, k = n = 4096: fp16 44 us, 2.3 TB/s of x, y and out; bound
-//   by the instructions and barriers of a turn (about 300 per warp and 64 columns, 14 warps an SM), not by HBM (16 us)
-//   or the tensor pipe (9 us).
+//   one's a turn ahead.  2048 rows of rank 64, k = n = 4096, all but 250 with the same adapter: fp16 44 us (2.3 TB/s of
+//   x, y and out), bf16 57, fp32 109; bound by the instructions and barriers of a turn (about 300 per warp and 64
+//   columns, 14 warps an SM), not by HBM (16 us) or the tensor pipe (9 us).
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -423,7 +423,7 @@ struct Tile {
 
 // The rows of a tile: LT_CHUNK rows at a time are put in the order of their adapters (those that share a bucket stay in
 // the batch's order, rows without an adapter come last), so that a tile's rows name few of them whatever the batch's
-// order is: 2048 rows of rank 64, k = n = 4096, each with one of 12 adapters, take 56 us, in the batch's order 234.  A
+// order is: 2048 rows, k = n = 4096, six of seven with one of 12 adapters of rank 64, take 56 us, in their own order 234.  A
 // stable counting sort that every CTA repeats for itself, about 1 us; a bucket may hold several adapters, which only
 // mixes them.  row[i] is the tile's i-th row, -1 behind the last one.  work: 8 x 256 counts.
 constexpr int LT_CHUNK = 1024;
