@@ -381,7 +381,7 @@ ZC_API int32_t zcu_pages_trim(int32_t* page_table, int32_t* seq_len, int32_t* fr
  * slots[t] = page * page_size + slot; slots outside [0, num_pages * page_size) are skipped.  hd 32, 64, 128 or 256.
  * bounds int8 [num_pages][hkv][2][hd] and scales fp32 [num_pages][hkv] (both or neither) receive, for every page
  * written, 8-bit bounds of its stored keys: scale = max|k| / 127, lo = floor(min k / scale), hi = ceil(max k / scale)
- * per dimension (0 for a page whose largest key is 0 or not finite).  A page holds its slots up to the last one that
+ * per dimension (0 for a page whose largest key is 0 or infinite; NaN keys are passed over).  A page holds its slots up to the last one that
  * the call writes.  The tokens that a call writes to one page stand in ascending slots, gaps allowed, with no other page's
  * tokens between them; skipped entries may stand anywhere.  -6 for more than 2^31 - 4097 tokens.
  * Pointers and strides in whole 4-element pieces (16 bytes of fp32, 8 of fp16). */
@@ -402,7 +402,8 @@ ZC_API int32_t zcu_append_kv(const void* k, const void* v, int32_t in_dtype, int
  *   sel int32 [batch][hkv][budget] receives the chosen pages (indices into the table row, ascending), -1 behind them.
  * score(page) = scale_page * max over the KV head's query heads of s_q * sum_d max(qi_d lo_d, qi_d hi_d), with
  * s_q = max|q| / 32512 and qi = rint(q / s_q): whole numbers summed exactly and two fp32 products, so the choice
- * does not depend on the launch; the lower page wins among equal scores.
+ * does not depend on the launch; the lower page wins among equal scores, and a page whose scale is infinite is chosen
+ * before all others.
  * The attention is fp32 through pairs for the tensor cores.  A query element is held to 2^-22 of itself or 2^-32 of its
  * head's largest (fp32 pools: 2^-22), keys and values of fp16 pools exactly and of fp32 pools to 2^-22, a softmax weight
  * to 2^-22 (fp16 pools: down to 2^-28 of the largest among its block of 16 tokens, below to 2^-50 of that one).  A key or

@@ -497,6 +497,24 @@ def test_sparse_attention_equal_pages_go_to_the_lower_one():
         assert sel[0, 0].tolist() == sorted(high + list(range(budget - len(high))))
 
 
+def test_sparse_attention_pages_with_infinite_keys_come_first():
+    """As append_kv leaves them: codes 0 and an infinite scale, for queries of either sign and of zeros."""
+    page, hd = 16, 64
+    k = torch.randn((40, 1, page, hd), device="cuda")
+    k[17, 0, 3, 9], k[30, 0, 0, 0], k[33, 0, 5, 4] = float("inf"), -float("inf"), float("nan")
+    pools = [torch.zeros((40, 1, page, hd), device="cuda") for _ in range(2)]
+    bounds, scales = torch.zeros((40, 1, 2, hd), dtype=torch.int8, device="cuda"), torch.zeros((40, 1), device="cuda")
+    rows = k.transpose(1, 2).reshape(-1, 1, hd)
+    ops.append_kv(rows, rows, torch.arange(640, device="cuda"), *pools, bounds, scales)
+    assert torch.isfinite(scales).flatten().logical_not().nonzero().flatten().tolist() == [17, 30]
+    q = torch.randn((3, 1, hd), device="cuda")
+    q[1] *= -1e-20
+    q[2] = 0
+    table = torch.arange(40, dtype=torch.int32, device="cuda").expand(3, 40).contiguous()
+    _, sel = ops.sparse_paged_attention(q, *pools, bounds, scales, table, ints([640] * 3), 2, sink=0, recent=0)
+    assert sel.flatten(1).tolist() == [[17, 30]] * 3
+
+
 def test_sparse_attention_long_sequence_many_pages():
     """More pages than one CTA scores, in a pool whose far pages lie beyond 32-bit element offsets."""
     rng = np.random.default_rng(12)

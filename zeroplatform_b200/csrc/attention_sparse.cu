@@ -110,10 +110,13 @@ __device__ __forceinline__ int key_piece(int row, int piece) { return piece ^ ((
 __device__ __forceinline__ int value_piece(int row, int piece) { return piece ^ (row & 6); }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// Unsigned key whose order is the float's (NaN above everything, -0 below 0: callers pass sums that are never -0).
+// Unsigned key whose order is the float's (NaN, the score of a page with an infinite key, above everything; -0 below 0:
+// callers pass sums that are never -0).  The asm keeps these bits from the compiler, which would set the sign by a
+// floating-point negation and so lose a NaN's.
 __device__ __forceinline__ uint32_t order_key(float f) {
-  const uint32_t u = __float_as_uint(f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  uint32_t u;
+  asm("mov.b32 %0, %1;" : "=r"(u) : "f"(f));
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
 // The score operand of a head tile: rows 0-7 the high bytes of qi, rows 8-15 the low bytes (qi = 256 high + low, both
