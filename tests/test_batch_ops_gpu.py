@@ -599,6 +599,30 @@ def test_sparse_attention_rows_carried_by_small_weights(hq, hkv, hd, every, batc
 
 
 @pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("large", [1e3, 1e6, 1e20])
+def test_sparse_attention_query_element_that_dwarfs_the_rest(half, large):
+    """A query whose largest element meets keys of 0: scores come from the others, held to 2^-22 of themselves or 2^-32 of
+    the largest (fp32 pools: 2^-22).  Tolerance as in check_sparse, with the terms that are added up, and the latter."""
+    rng = np.random.default_rng(15)
+    hd, page, n = 64, 16, 20
+    dt = np.float16 if half else np.float32
+    k, v = (rng.standard_normal((n, 1, page, hd)).astype(dt) for _ in range(2))
+    k[..., 9] = 0
+    q = rng.standard_normal((1, 4, hd)).astype(np.float32)
+    codes, scales = key_bounds(k)
+    q[..., 9] = large
+    out, _ = ops.sparse_paged_attention(dev(q), dev(k), dev(v), dev(codes), dev(scales), ints([list(range(n))]),
+                                        ints([n * page]), n)
+    kk, vv = k[:, 0].reshape(-1, hd), v[:, 0].reshape(-1, hd)
+    ref, mag = plain_attention(q[0], kk, vv, 1 / np.sqrt(hd))
+    lost = np.abs(kk.astype(np.float64)).sum(-1).max() / np.sqrt(hd) * np.float64(large) * 2.0 ** -32 if half else 0.0
+    tol = np.abs(vv.astype(np.float64)).max() * (2 * hd * 2.0 ** -23 * mag + 2 * lost + (n * page / 8 + 64) * 2.0 ** -23)
+    if 2 * lost < 0.5:  # beyond, the weights are anybody's
+        assert np.abs(out[0].cpu().numpy() - ref).max() <= tol
+    assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("half", [True, False])
 def test_sparse_attention_cuts_lengths_to_max_ctx(half):
     """A length above max_ctx counts as max_ctx, which need not end a page; the tokens behind it are there."""
     rng = np.random.default_rng(14)
@@ -738,6 +762,32 @@ def test_lora_order_of_a_large_batch_does_not_matter(rows, adapters, w):
         place = dev(y[order])
         ops.lora_add(place, dev(x[order]), *d, dev(adapter[order]), out=place, **kw)
         assert (place.cpu().numpy() == out[order]).all()
+
+
+@pytest.mark.parametrize("w", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("rows", [7, 300])
+@pytest.mark.parametrize("large,at", [(1e3, 5), (1e6, 5), (1e6, 700), (1e9, 1000)])
+def test_lora_element_that_dwarfs_the_rest(rows, large, at, w):
+    """Rows with an element far above the others, which meets weights of 0, at the row's start or far into it: the others
+    are held to 2^-22 of themselves or, with fp16 adapters over many rows, 2^-31 of the row's largest.  Tolerance as in
+    test_lora, and the latter through both products."""
+    rng = np.random.default_rng(rows + at)
+    k, n, rank = 1024, 130, 16
+    x, y = rng.standard_normal((rows, k)).astype(np.float32), rng.standard_normal((rows, n)).astype(np.float32)
+    a = torch.from_numpy(rng.standard_normal((2, rank, k)).astype(np.float32) / k ** 0.5)
+    a[..., at] = 0
+    a, b = a.to(getattr(torch, w)), torch.from_numpy(rng.standard_normal((2, n, rank)).astype(np.float32)).to(
+        getattr(torch, w))
+    adapter = rng.integers(-1, 2, rows)
+    x[:, at] = large
+    ref, mag = plain_lora(x, y, a, b, adapter, [rank] * 2, [1.0] * 2)
+    lost = np.zeros((rows, n))
+    if w == "float16" and rows > 256:
+        for e in range(2):
+            A, B = a[e].double().abs().numpy(), b[e].double().abs().numpy()
+            lost[adapter == e] = large * 2.0 ** -31 * (B @ A.sum(-1))
+    out = ops.lora_add(dev(y), dev(x), a.cuda(), b.cuda(), ints(adapter)).cpu().numpy()
+    assert (np.abs(out - ref) <= ((k / 8 + 40) * 2.0 ** -23 + 2.0 ** -21) * mag + lost).all()
 
 
 def test_lora_same_rows_alone_and_in_a_batch():
