@@ -359,9 +359,9 @@ ZC_API int32_t zcu_moe_forward(void* moe, const float* xnorm, const float* route
  * is out of range or named by an earlier request of the call, when it would pass max_pages pages or the end of the
  * token arrays, or when the stack does not hold its pages and those of the requests before it: after the first request
  * that finds too few, all later ones are refused, those that need no page among them, so requests come in the order of
- * their claim (decode before prompts).  Per token: slots =
- * page * page_size + slot, positions, token_rows (its table row) and ctx_len = position + 1; tokens of refused
- * requests and behind the last request get slot -1, position 0, row -1, ctx_len 0.
+ * their claim (decode before prompts).  Per token: slots = page * page_size + slot, positions, token_rows (its table row)
+ * and ctx_len = position + 1; tokens of refused requests and behind the last request get slot -1, position 0, row -1,
+ * ctx_len 0.
  * trim: row rows[b] keeps min(new_len[b], its length) tokens (0 frees the sequence); pages behind them go back to the
  * stack, the last request's last page first, and their table entries become -1.  A reserve whose lengths are trimmed
  * back leaves the stack as it was.
@@ -381,9 +381,9 @@ ZC_API int32_t zcu_pages_trim(int32_t* page_table, int32_t* seq_len, int32_t* fr
  * slots[t] = page * page_size + slot; slots outside [0, num_pages * page_size) are skipped.  hd 32, 64, 128 or 256.
  * bounds int8 [num_pages][hkv][2][hd] and scales fp32 [num_pages][hkv] (both or neither) receive, for every page
  * written, 8-bit bounds of its stored keys: scale = max|k| / 127, lo = floor(min k / scale), hi = ceil(max k / scale)
- * per dimension (0 for a page whose largest key is 0 or infinite; NaN keys are passed over).  A page holds its slots up to the last one that
- * the call writes.  The tokens that a call writes to one page stand in ascending slots, gaps allowed, with no other page's
- * tokens between them; skipped entries may stand anywhere.  -6 for more than 2^31 - 4097 tokens.
+ * per dimension (0 for a page whose largest key is 0 or infinite; NaN keys are passed over).  A page holds its slots up
+ * to the last one that the call writes.  The tokens that a call writes to one page stand in ascending slots, gaps allowed,
+ * with no other page's tokens between them; skipped entries may stand anywhere.  -6 for more than 2^31 - 4097 tokens.
  * Pointers and strides in whole 4-element pieces (16 bytes of fp32, 8 of fp16). */
 ZC_API int32_t zcu_append_kv(const void* k, const void* v, int32_t in_dtype, int64_t k_stride, int64_t v_stride,
                              const int64_t* slots, int32_t tokens, void* k_pool, void* v_pool, int32_t kv_dtype,
@@ -426,8 +426,8 @@ ZC_API int32_t zcu_sparse_paged_attention(const float* q, int64_t q_stride, cons
  * a [adapters][rank][k_cols] and b [adapters][n_rows][rank] (w_dtype 0 = fp32, 1 = fp16, 2 = bf16); of adapter e the
  * first ranks[e] of `rank` are used (NULL: all), scales NULL: 1.  fp32 arithmetic up to 256 rows, beyond on the tensor
  * cores with x and x A^T split into terms that hold each element to 2^-22 (fp16 adapters: or to 2^-31 of the row's largest;
- * fp32 adapters are split alike).  What another row or its adapter holds, NaN included, does not reach a row; where x or
- * the adapter is not finite, neither is the row.
+ * fp32 adapters are split alike).  What another row or its adapter holds, NaN included, does not reach a row; an element
+ * of its own x, A_e or B_e that is not finite makes what it reaches NaN or infinite.
  * rank a multiple of 8 up to 128, k_cols a multiple of 32 (else -4); x, a and b 16-byte aligned, x_stride a multiple
  * of 4. */
 ZC_API int32_t zcu_lora_add(const float* x, int64_t x_stride, const float* y, int64_t y_stride, float* out,

@@ -367,9 +367,8 @@ def _kv_pools(k_pool, v_pool, dev):
 def append_kv(k, v, slots, k_pool, v_pool, bounds=None, scales=None, stream=None) -> None:
     """Keys and values [tokens, hkv, hd] (fp32 or fp16; any token stride) into paged pools [pages, hkv, page size, hd]
     at slots [tokens] (int64; reserve_pages' slots, negative ones skipped; the tokens of one page in ascending slots with
-    no other page's tokens between them).  bounds int8 [pages, hkv, 2, hd] and
-    scales fp32 [pages, hkv] receive the 8-bit key bounds of the pages written, which sparse_paged_attention scores
-    pages by (zcu_append_kv)."""
+    no other page's tokens between them).  bounds int8 [pages, hkv, 2, hd] and scales fp32 [pages, hkv] receive the 8-bit
+    key bounds of the pages written, which sparse_paged_attention scores pages by (zcu_append_kv)."""
     d = _lib.dispatch
     if d and stream is None and d.append_kv(k, v, slots, k_pool, v_pool, bounds, scales):
         return
